@@ -220,6 +220,98 @@ int attn_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
                         float scale, int dtype, void* stream);
 
 /*
+ * The 4-bit key/value cache.  No counterpart in the reference, which has no key/value cache
+ * (generate.py:611-628); it serves the decode that attn_decode serves from a bf16 or float32 cache
+ * in 4.5 bits per value (head_dim 64 and 128).
+ *
+ * Format.  A row is the D values of one (sequence, head, position), D = 16, 32, 64 or 128, in groups
+ * of g = min(D, 64).  A group keeps s = float16((max - min) / 15) and m = float16(min) (float32
+ * arithmetic, the division as a product with the float32 nearest to 1/15, saturating at 65504) and, for
+ * each x, the code n in 0..15 nearest to (x - m) / s in exact arithmetic, ties to even; it stands for
+ * n*s + m.  A group holding an infinity or a NaN reads back as
+ * NaN.
+ *   codes   uint8   row r at codes + r * D/2: element d = 2i in the low nibble of byte i, 2i+1 in the high
+ *   params  float16 row r at params + r * 2 * D/g: (s, m) of every group
+ * Row r of (which, b, h, slot) is which*c_si + b*c_sb + h*c_sh + slot, which = 0 for keys and 1 for
+ * values.  capacity (the slots of one head) and the strides, all in rows, are multiples of 16; both
+ * arrays are 16-byte aligned.  int32 arrays of one entry per sequence live on the device, so that a
+ * captured step reads them anew at every replay.
+ *
+ * attn_kv4_store quantises k and v (ATTN_F32 or ATTN_BF16, element (b, t, h, d) at
+ * k[b*k_sb + t*k_st + h*k_sh + d]) into slots starts[b] + start + t, t < counts[b] (starts NULL: 0;
+ * counts NULL: T).  Rows that fall outside 0 .. capacity-1 are not written.  weights and positions
+ * (each may be NULL; element (b, h, slot) at b*w_sb + h*w_sh + slot) receive 0 and the token's
+ * position seen[b] + seen0 + t (seen NULL: 0) at the slots written.
+ * attn_kv4_load writes the same rows back as numbers (element (b, t, h, d) at k[b*o_sb + t*o_st +
+ * h*o_sh + d]; zeros for t >= counts[b] and for slots outside the cache).
+ */
+int attn_kv4_store(const void* k, const void* v, int dtype, int B, int T, int NH, int D,
+                   int64_t k_sb, int64_t k_st, int64_t k_sh, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                   void* codes, void* params, int64_t c_si, int64_t c_sb, int64_t c_sh, int capacity,
+                   const int* starts, int start, const int* counts,
+                   float* weights, int* positions, int64_t w_sb, int64_t w_sh,
+                   const int* seen, int seen0, void* stream);
+int attn_kv4_load(const void* codes, const void* params, int64_t c_si, int64_t c_sb, int64_t c_sh,
+                  int capacity, int B, int T, int NH, int D, const int* starts, int start,
+                  const int* counts, void* k, void* v, int dtype,
+                  int64_t o_sb, int64_t o_st, int64_t o_sh, void* stream);
+
+/* Bytes of workspace attn_kv4_decode needs (weights: whether weights_out is given). */
+size_t attn_kv4_decode_workspace_size(int B, int NH, int L, int D, int weights);
+
+/*
+ * Single-query decode over a 4-bit cache: for each of the NH query heads of each sequence, attention
+ * of one query row over the n = lengths[b] (clamped to 0..L; lengths NULL: L) cached rows of its key
+ * head, NH / NKV consecutive query heads to a key head.  q, o: element (b, h, d) at ptr[b*sb + h*sh + d],
+ * ATTN_F32 or ATTN_BF16.  lse [B, NH] may be NULL.  With weights_out (element (b, key head, slot) at
+ * b*w_sb + h*w_sh + slot), weights_out = weights_in (NULL: 0; may be the same array) + the sum over the
+ * key head's query heads of the attention weights, for slots below L; slots from n on get weights_in.
+ * A sequence of no rows gives o = 0, lse = -infinity and no weight.
+ */
+int attn_kv4_decode(const void* q, const void* codes, const void* params, void* o, float* lse,
+                    int B, int NH, int NKV, int L, int D, int64_t q_sb, int64_t q_sh,
+                    int64_t o_sb, int64_t o_sh, int64_t c_si, int64_t c_sb, int64_t c_sh, int capacity,
+                    const int* lengths, const float* weights_in, float* weights_out,
+                    int64_t w_sb, int64_t w_sh, float scale, int dtype,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Accumulated attention weights of a causal prompt: weights_out[b, h, j] = weights_in[b, h, j] (NULL: 0;
+ * may be the same array) + the sum over the NH / NKV query heads of key head h and the queries
+ * i, max(j, first_query) <= i < lengths[b] (NULL: T), of exp(scale q_i . k_j - lse_i), with the lse
+ * [B, NH, T] that attn_fwd wrote: the column sums of attn_probs' matrix without storing it.  Keys
+ * from lengths[b] on get weights_in.  q: element (b, t, h, d) at q[b*q_sb + t*q_st + h*q_sh + d], k
+ * likewise; element (b, h, j) of the weights at b*w_sb + h*w_sh + j.  head_dim up to 128.  ATTN_TF32:
+ * q and k truncated to tf32, as attn_fwd's tf32 path reads them (head_dim <= 32).
+ */
+int attn_key_weights(const void* q, const void* k, const float* lse, const float* weights_in,
+                     float* weights_out, int B, int NH, int NKV, int T, int D,
+                     int64_t q_sb, int64_t q_st, int64_t q_sh, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                     int64_t w_sb, int64_t w_sh, int first_query, const int* lengths,
+                     float scale, int dtype, void* stream);
+
+/* Bytes of workspace attn_kv4_evict needs. */
+size_t attn_kv4_evict_workspace_size(int B, int NH, int L, int keep);
+
+/*
+ * Eviction: of the n = lengths[b] (clamped to 0..L; NULL: L) rows of every (sequence, head) of a 4-bit
+ * cache, keep min(n, keep): first those whose position is at least seen[b] + seen0 - recent (positions
+ * NULL: the slot is the position), then those of the largest accumulated weight, among equals the lowest
+ * slot (NaN last).  Kept rows below slot `keep` stay in their slots; those from slot `keep` on fill, in
+ * order, the slots below it that were given up.  slots [B, NH, keep] receives the row each slot holds
+ * afterwards (-1 from min(n, keep) on).  Codes, params, weights and positions move together: in place
+ * (dst_codes NULL; the other dst arguments are then ignored), or into another cache, whose slots from
+ * min(n, keep) on are left as they were.  recent <= keep.
+ */
+int attn_kv4_evict(void* codes, void* params, float* weights, int* positions,
+                   int64_t c_si, int64_t c_sb, int64_t c_sh, int capacity, int64_t w_sb, int64_t w_sh,
+                   void* dst_codes, void* dst_params, float* dst_weights, int* dst_positions,
+                   int64_t d_si, int64_t d_sb, int64_t d_sh, int dst_capacity, int64_t dw_sb, int64_t dw_sh,
+                   int B, int NH, int L, int D, int keep, int recent, const int* lengths,
+                   const int* seen, int seen0, int* slots, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/*
  * Projection GEMM: C[M,N] = op(A)[M,K] . op(B)[K,N] (+ bias[N]) ; with accumulate, C += ...
  * Replaces matmul_2d_kernel (core/kernels.py:119-140) and the projection-gradient GEMMs of
  * model/gpt.py:666-689 (dWo = ctx^T dY, dCtx = dY Wo^T, dWqkv = x^T dQKV, dX = dQKV Wqkv^T).

@@ -1,0 +1,62 @@
+// The 4-bit key/value cache: layout, and the arithmetic of one group, shared by the store, load,
+// decode and eviction kernels.
+//
+// A cached row holds the D values of one (sequence, head, position) in groups of g = min(D, 64).  A
+// group keeps s = f16((max - min) / 15) and m = f16(min), both computed in float32 (the division as a
+// product with the float32 nearest to 1/15), and per value the code n in 0..15 nearest to (x - m) / s in exact arithmetic (ties to even); it stands for n*s + m.
+//   codes  [2][B][NH][cap][D / 2] bytes   (0 keys, 1 values; element d = 2i in the low nibble of byte i)
+//   params [2][B][NH][cap][D / g] half2   (s, m)
+// Rows of one (sequence, head) are contiguous, so that a run of keys is one contiguous copy; the other
+// axes are strided, in rows, with the same strides for codes and params.  cap and the strides are
+// multiples of 16 rows, which keeps every 16th row 16-byte aligned in both arrays for every D.
+#pragma once
+
+#include "common.cuh"
+#include <cuda_fp16.h>
+
+namespace attn {
+
+constexpr int KV4_ALIGN_ROWS = 16;
+
+__host__ __device__ constexpr int kv4_group(int D) { return D < 64 ? D : 64; }
+__host__ __device__ constexpr int kv4_groups(int D) { return D / kv4_group(D); }
+inline bool kv4_head_dim_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128; }
+
+struct Kv4View {
+  uint8_t* codes;
+  __half2* params;
+  int64_t si, sb, sh;  // strides in rows: keys -> values, sequence, head
+  int cap;             // rows per (sequence, head)
+};
+
+// Checks shared by the entry points that take a cache.
+int kv4_check(const char* fn, const Kv4View& c, int B, int NH, int D);
+
+// An int32 per sequence: base[b] + add, or add alone when base is NULL.
+__device__ __forceinline__ int64_t seq_value(const int* base, int b, int add) {
+  return (base ? (int64_t)base[b] : 0) + add;
+}
+
+// Rows of sequence b: lengths[b] clamped to 0..most, or most when lengths is NULL.
+__device__ __forceinline__ int seq_length(const int* lengths, int b, int most) {
+  return lengths ? min(max(lengths[b], 0), most) : most;
+}
+
+// The code of x in a group (s, m): the n in 0..15 nearest to (x - m) / s, ties to even, decided in
+// exact arithmetic.  x - m is split into its float32 rounding d and the rounding's error e (Knuth's
+// two-sum), and the borders (n +- 1/2) s are exact in float32 (5 + 11 bits); a division can only
+// place a value near a border on the wrong side of it, which the comparisons put right.
+__device__ __forceinline__ uint32_t kv4_code(float x, float s, float m, float inv) {
+  if (!(s > 0.f)) return 0;
+  const float d = __fsub_rn(x, m);
+  const float bb = __fsub_rn(d, x);
+  const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(d, bb)), -__fadd_rn(m, bb));
+  float n = fminf(fmaxf(rintf(__fmul_rn(d, inv)), 0.f), 15.f);
+  const float hi = __fmul_rn(n + 0.5f, s), lo = __fmul_rn(n - 0.5f, s);
+  const bool odd = ((int)n & 1) != 0;
+  if (d > hi || (d == hi && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
+  else if (d < lo || (d == lo && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
+  return (uint32_t)fminf(fmaxf(n, 0.f), 15.f);
+}
+
+}  // namespace attn

@@ -1,0 +1,227 @@
+// Quantise keys and values into the 4-bit cache (store) and read rows back as numbers (load).
+//
+// The reference has no key/value cache (generate.py:611-628 runs the whole context again for every
+// token); these fill and read the one attn_kv4_decode attends over.  Both are one pass: the store
+// reads each value once and writes 4 bits and 1/16 of a scale pair for it, so HBM traffic bounds the
+// prompt's store and launch latency a single token's.
+//
+// A row is taken by D / 8 lanes of 8 values each (16 bytes of bf16 per lane); a group's minimum and
+// maximum come from shuffles among its 2, 4 or 8 lanes.  Rows are walked with the position fastest, so
+// that a warp's codes (and scale pairs) of consecutive positions are one contiguous write while its
+// reads are whole rows of the token layout.
+#include "kv4.cuh"
+#include <math.h>
+
+namespace attn {
+
+constexpr int KV4_THREADS = 256;
+
+int kv4_check(const char* fn, const Kv4View& c, int B, int NH, int D) {
+  ATTN_REQUIRE(c.codes && c.params, "%s: null cache pointer", fn);
+  ATTN_REQUIRE(B > 0 && NH > 0 && c.cap > 0, "%s: B, NH and capacity must be positive", fn);
+  if (!kv4_head_dim_ok(D)) {
+    set_error("%s: head_dim %d not supported by the 4-bit cache (16, 32, 64 or 128)", fn, D);
+    return ATTN_ERR_UNSUPPORTED;
+  }
+  ATTN_REQUIRE(c.cap % KV4_ALIGN_ROWS == 0 && c.si % KV4_ALIGN_ROWS == 0 && c.sb % KV4_ALIGN_ROWS == 0 &&
+                   c.sh % KV4_ALIGN_ROWS == 0,
+               "%s: the cache's capacity and strides must be multiples of %d rows", fn, KV4_ALIGN_ROWS);
+  ATTN_REQUIRE(c.si >= 0 && c.sb >= 0 && c.sh >= c.cap, "%s: bad cache strides", fn);
+  ATTN_REQUIRE(aligned(c.codes, 16) && aligned(c.params, 16), "%s: the cache must be 16-byte aligned", fn);
+  return ATTN_OK;
+}
+
+struct Kv4Rows {
+  const void *k, *v;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  uint32_t T, NH, rows;  // rows = B * NH * T
+};
+
+struct Kv4Slots {
+  const int* starts;  // first slot of each sequence: starts[b] + start
+  int start;
+  const int* counts;  // tokens of each sequence (NULL: T)
+};
+
+struct Kv4Marks {
+  float* weights;  // zeroed at the stored slots (may be NULL)
+  int* positions;  // token positions, seen[b] + seen0 + t (may be NULL)
+  int64_t sb, sh;
+  const int* seen;
+  int seen0;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, float* x) {
+  if constexpr (VEC) {
+    const float4 a = load4(p), b = load4(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::load(p + i);
+  }
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(KV4_THREADS)
+kv4_store_kernel(const Kv4Rows in, const Kv4View c, const Kv4Slots sl, const Kv4Marks mk) {
+  constexpr int LPR = D / 8;             // lanes per row
+  constexpr int LPG = kv4_group(D) / 8;  // lanes per group
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
+  const int sub = threadIdx.x % LPR;
+  const bool value = blockIdx.y != 0;
+  const uint32_t r = min(row, in.rows - 1);
+  const uint32_t bh = r / in.T, t = r - bh * in.T;
+  const uint32_t b = bh / in.NH, h = bh - b * in.NH;
+  const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
+  const bool put = row < in.rows && slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : in.T);
+  float x[8];
+  if (put) {
+    const T* src = value ? (const T*)in.v + b * in.v_sb + t * in.v_st + h * in.v_sh
+                         : (const T*)in.k + b * in.k_sb + t * in.k_st + h * in.k_sh;
+    load8<T, VEC>(src + sub * 8, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  }
+  float lo = x[0], hi = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    finite = finite && fabsf(x[i]) <= 3.4028234664e38f;
+  }
+  int fin = finite;
+#pragma unroll
+  for (int off = LPG / 2; off > 0; off >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    fin &= __shfl_xor_sync(0xffffffffu, fin, off);
+  }
+  if (!put) return;
+  // scale and minimum saturate at float16's largest value; a group holding an infinity or a NaN reads
+  // back as NaN
+  const __half s = __float2half_rn(fin ? fminf(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), 65504.f) : NAN);
+  const __half m = __float2half_rn(fin ? fminf(fmaxf(lo, -65504.f), 65504.f) : NAN);
+  const float sf = __half2float(s), mf = __half2float(m);
+  const float inv = sf > 0.f ? __fdiv_rn(1.f, sf) : 0.f;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w |= kv4_code(x[i], sf, mf, inv) << (4 * i);
+  const int64_t dst = (value ? c.si : 0) + b * c.sb + h * c.sh + slot;
+  *reinterpret_cast<uint32_t*>(c.codes + dst * (D / 2) + sub * 4) = w;
+  if (sub % LPG == 0) c.params[dst * kv4_groups(D) + sub / LPG] = __halves2half2(s, m);
+  if (!value && sub == 0) {
+    const int64_t at = b * mk.sb + h * mk.sh + slot;
+    if (mk.weights) mk.weights[at] = 0.f;
+    if (mk.positions) mk.positions[at] = (int)(seq_value(mk.seen, b, mk.seen0) + t);
+  }
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(KV4_THREADS)
+kv4_load_kernel(const Kv4Rows out, const Kv4View c, const Kv4Slots sl) {
+  constexpr int LPR = D / 8;
+  constexpr int LPG = kv4_group(D) / 8;
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
+  if (row >= out.rows) return;
+  const int sub = threadIdx.x % LPR;
+  const bool value = blockIdx.y != 0;
+  const uint32_t bh = row / out.T, t = row - bh * out.T;
+  const uint32_t b = bh / out.NH, h = bh - b * out.NH;
+  const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : out.T)) {
+    const int64_t src = (value ? c.si : 0) + b * c.sb + h * c.sh + slot;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(c.codes + src * (D / 2) + sub * 4);
+    const float2 p = __half22float2(c.params[src * kv4_groups(D) + sub / LPG]);
+    // n*s is exact (4 + 11 bits), so the sum is rounded once
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), p.x, p.y);
+  }
+  T* dst = value ? (T*)out.v + b * out.v_sb + t * out.v_st + h * out.v_sh
+                 : (T*)out.k + b * out.k_sb + t * out.k_st + h * out.k_sh;
+  dst += sub * 8;
+  if constexpr (VEC) {
+    store4(dst, make_float4(x[0], x[1], x[2], x[3]));
+    store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) Elem<T>::store(dst + i, x[i]);
+  }
+}
+
+template <typename T, int D, bool VEC>
+static int kv4_rows_launch(const Kv4Rows& r, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
+  constexpr uint32_t per = KV4_THREADS / (D / 8);
+  const dim3 grid((r.rows + per - 1) / per, 2);
+  const cudaError_t e = mk ? launch_pdl(kv4_store_kernel<T, D, VEC>, grid, dim3(KV4_THREADS), 0, s, r, c, sl, *mk)
+                           : launch_pdl(kv4_load_kernel<T, D, VEC>, grid, dim3(KV4_THREADS), 0, s, r, c, sl);
+  count_launch();
+  return check_launch(mk ? "kv4_store_kernel" : "kv4_load_kernel", e);
+}
+
+template <typename T>
+static int kv4_rows_t(const Kv4Rows& r, int D, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
+  // vector accesses where every lane's first value is aligned for them (4 values: 8 bytes of bf16, 16 of float32)
+  const bool vec = aligned(r.k, 4 * sizeof(T)) && aligned(r.v, 4 * sizeof(T)) && r.k_sb % 4 == 0 && r.k_st % 4 == 0 &&
+                   r.k_sh % 4 == 0 && r.v_sb % 4 == 0 && r.v_st % 4 == 0 && r.v_sh % 4 == 0;
+#define KV4_ROWS(DD)                                                       \
+  case DD:                                                                 \
+    return vec ? kv4_rows_launch<T, DD, true>(r, c, sl, mk, s) : kv4_rows_launch<T, DD, false>(r, c, sl, mk, s);
+  switch (D) { KV4_ROWS(16) KV4_ROWS(32) KV4_ROWS(64) KV4_ROWS(128) }
+#undef KV4_ROWS
+  return ATTN_ERR_UNSUPPORTED;
+}
+
+static int kv4_rows(const char* fn, const Kv4Rows& r, int B, int D, int dtype, const Kv4View& c, const Kv4Slots& sl,
+                    const Kv4Marks* mk, cudaStream_t s) {
+  if (int rc = kv4_check(fn, c, B, (int)r.NH, D)) return rc;
+  ATTN_REQUIRE(r.k && r.v, "%s: null pointer argument", fn);
+  ATTN_REQUIRE(dtype == ATTN_F32 || dtype == ATTN_BF16, "%s: dtype must be ATTN_F32 or ATTN_BF16", fn);
+  ATTN_REQUIRE(aligned(r.k, dtype == ATTN_BF16 ? 2 : 4) && aligned(r.v, dtype == ATTN_BF16 ? 2 : 4), "%s: misaligned tensor", fn);
+  const int64_t st[6] = {r.k_sb, r.k_st, r.k_sh, r.v_sb, r.v_st, r.v_sh};
+  for (int i = 0; i < 6; ++i) ATTN_REQUIRE(st[i] >= 0, "%s: strides must not be negative", fn);
+  ATTN_REQUIRE(sl.starts || (sl.start >= 0 && (int64_t)sl.start + r.T <= c.cap),
+               "%s: positions %d .. %lld exceed the capacity of %d", fn, sl.start, (long long)sl.start + r.T - 1, c.cap);
+  return dtype == ATTN_BF16 ? kv4_rows_t<__nv_bfloat16>(r, D, c, sl, mk, s) : kv4_rows_t<float>(r, D, c, sl, mk, s);
+}
+
+}  // namespace attn
+
+using namespace attn;
+
+extern "C" int attn_kv4_store(const void* k, const void* v, int dtype, int B, int T, int NH, int D, int64_t k_sb,
+                              int64_t k_st, int64_t k_sh, int64_t v_sb, int64_t v_st, int64_t v_sh, void* codes,
+                              void* params, int64_t c_si, int64_t c_sb, int64_t c_sh, int capacity, const int* starts,
+                              int start, const int* counts, float* weights, int* positions, int64_t w_sb, int64_t w_sh,
+                              const int* seen, int seen0, void* stream) {
+  clear_error();
+  ATTN_REQUIRE(B > 0 && T > 0 && NH > 0, "attn_kv4_store: sizes must be positive");
+  ATTN_REQUIRE((int64_t)B * NH * T < (int64_t)1 << 31, "attn_kv4_store: B*NH*T must be below 2^31");
+  ATTN_REQUIRE(!(weights || positions) || (w_sb >= 0 && w_sh >= 0), "attn_kv4_store: bad strides");
+  const Kv4Rows r = {k, v, k_sb, k_st, k_sh, v_sb, v_st, v_sh, (uint32_t)T, (uint32_t)NH, (uint32_t)(B * NH * T)};
+  const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
+  ATTN_REQUIRE(c_si >= capacity && (B == 1 || c_sb >= capacity), "attn_kv4_store: cache rows must not overlap");
+  const Kv4Marks mk = {weights, positions, w_sb, w_sh, seen, seen0};
+  return kv4_rows("attn_kv4_store", r, B, D, dtype, c, Kv4Slots{starts, start, counts}, &mk, as_stream(stream));
+}
+
+extern "C" int attn_kv4_load(const void* codes, const void* params, int64_t c_si, int64_t c_sb, int64_t c_sh,
+                             int capacity, int B, int T, int NH, int D, const int* starts, int start, const int* counts,
+                             void* k, void* v, int dtype, int64_t o_sb, int64_t o_st, int64_t o_sh, void* stream) {
+  clear_error();
+  ATTN_REQUIRE(B > 0 && T > 0 && NH > 0, "attn_kv4_load: sizes must be positive");
+  ATTN_REQUIRE((int64_t)B * NH * T < (int64_t)1 << 31, "attn_kv4_load: B*NH*T must be below 2^31");
+  const Kv4Rows r = {k, v, o_sb, o_st, o_sh, o_sb, o_st, o_sh, (uint32_t)T, (uint32_t)NH, (uint32_t)(B * NH * T)};
+  const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
+  return kv4_rows("attn_kv4_load", r, B, D, dtype, c, Kv4Slots{starts, start, counts}, nullptr, as_stream(stream));
+}

@@ -33,6 +33,7 @@ import torch
 from . import dp
 from . import mha_ops as ops
 from ._lib import check_device_error, watch_device_error
+from .kv4 import KV4Cache
 from .mha_ops import HeadView, ptr
 
 
@@ -341,7 +342,7 @@ class MultiHeadAttention:
 
     # ---------------------------------------------------------------- forward
     @device_checked
-    def forward(self, gpu_input, B: int, T: int, kv_cache: "KVCache | None" = None):
+    def forward(self, gpu_input, B: int, T: int, kv_cache: "KVCache | KV4Cache | None" = None):
         """x [B*T, C] float32 (device) -> DeviceBuffer [B*T, C] float32 (caller frees).
 
         With ``kv_cache`` (from ``new_kv_cache``) the prompt's keys and values are also stored in
@@ -438,6 +439,8 @@ class MultiHeadAttention:
         scale = 1.0 / math.sqrt(D)
         with self._rng("attn_fwd"):
             ops.attention_forward(qv, kv, vv, ov, lse, B, NH, T, D, scale, mm)
+        if isinstance(kv_cache, KV4Cache):
+            kv_cache.add_prompt_weights(qkv.view(B, T, 3 * C), lse, mm)
         with self._rng("gemm_out"):
             ops.gemm(ctx.data_ptr(), C, False, w_o.data_ptr(), C, False, mm, out.data_ptr(), C,
                      torch.float32, M, C, C, bias=self.c_proj_b.weights.data_ptr(), accumulate=accumulate)
@@ -554,14 +557,20 @@ class MultiHeadAttention:
         return self._qkv_heads(2)
 
     # ---------------------------------------------------------------- incremental decoding
-    def new_kv_cache(self, B: int, max_len: int) -> "KVCache":
+    def new_kv_cache(self, B: int, max_len: int, bits: int | None = None, track_weights: bool = False,
+                     prompt_window: int | None = None) -> "KVCache | KV4Cache":
         """A key/value cache for ``B`` sequences of up to ``max_len`` tokens, in this module's
-        compute precision."""
+        compute precision, or, with ``bits=4``, in 4 bits per value (``KV4Cache``; head_dim 16, 32, 64 or
+        128), where ``track_weights`` and ``prompt_window`` serve its eviction."""
         C, NH, D = self._shape()
+        if bits == 4:
+            return KV4Cache(B, max_len, NH, D, track_weights=track_weights, prompt_window=prompt_window)
+        if bits is not None or track_weights or prompt_window is not None:
+            raise ValueError("new_kv_cache: bits must be 4 or None (the module's precision); weights are tracked at 4 bits")
         return KVCache(B, max_len, NH, D, self._dt)
 
     @device_checked
-    def forward_decode(self, gpu_input, B: int, kv_cache: "KVCache"):
+    def forward_decode(self, gpu_input, B: int, kv_cache: "KVCache | KV4Cache"):
         """One new token per sequence: x [B, C] float32 -> DeviceBuffer [B, C] float32.
 
         Equals the last rows of ``forward`` over the whole sequence (causal attention, the new
@@ -587,8 +596,11 @@ class MultiHeadAttention:
         ops.gemm(x_op.data_ptr(), C, False, w_qkv.data_ptr(), 3 * C, False, mm, qkv.data_ptr(), 3 * C, dt,
                  B, 3 * C, C, bias=self.c_attn_b.weights.data_ptr())
         kv_cache.store(qkv.view(B, 1, 3 * C), L)
-        q = qkv[:, :C].contiguous().view(B, NH, D)  # q and the output share one layout
-        ctx = ops.decode(q, kv_cache.k[:, :L + 1], kv_cache.v[:, :L + 1], 1.0 / math.sqrt(D))
+        if isinstance(kv_cache, KV4Cache):
+            ctx = kv_cache.attend(qkv.view(B, 3, NH, D)[:, 0])
+        else:
+            q = qkv[:, :C].contiguous().view(B, NH, D)  # q and the output share one layout
+            ctx = ops.decode(q, kv_cache.k[:, :L + 1], kv_cache.v[:, :L + 1], 1.0 / math.sqrt(D))
         out = torch.empty((B, C), dtype=torch.float32, device="cuda")
         ops.gemm(ctx.data_ptr(), C, False, w_o.data_ptr(), C, False, mm, out.data_ptr(), C, torch.float32,
                  B, C, C, bias=self.c_proj_b.weights.data_ptr())

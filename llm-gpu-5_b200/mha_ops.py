@@ -127,6 +127,266 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scale:
     return out
 
 
+# ---------------------------------------------------------------- 4-bit key/value cache
+# codes: uint8 [2, B, NH, cap, D/2]; params: float16 [2, B, NH, cap, D/min(D, 64), 2], index 0 keys and
+# 1 values (the format is described in include/attn_b200.h).  Views along the sequence and head axes
+# are taken as they are; both arrays must be the same view.
+
+KV4_HEAD_DIMS = (16, 32, 64, 128)
+KV4_ROWS = 16  # capacity and strides are multiples of this many rows
+
+
+def kv4_groups(D: int) -> int:
+    """Scale pairs per cached row of D values."""
+    return D // min(D, 64)
+
+
+def kv4_empty(B: int, NH: int, capacity: int, D: int, device="cuda"):
+    """Uninitialised (codes, params) of a cache of ``capacity`` rows (rounded up to a multiple of 16)
+    per sequence and head."""
+    if D not in KV4_HEAD_DIMS:
+        raise ValueError(f"the 4-bit cache takes head_dim 16, 32, 64 or 128, got {D}")
+    cap = (capacity + KV4_ROWS - 1) // KV4_ROWS * KV4_ROWS
+    return (torch.empty((2, B, NH, cap, D // 2), dtype=torch.uint8, device=device),
+            torch.empty((2, B, NH, cap, kv4_groups(D), 2), dtype=torch.float16, device=device))
+
+
+def _kv4_view(codes: torch.Tensor, params: torch.Tensor):
+    """(B, NH, cap, D, strides in rows) of a cache's two arrays, checked."""
+    if codes.dtype != torch.uint8 or params.dtype != torch.float16:
+        raise TypeError(f"4-bit cache: codes must be uint8 and params float16, got {codes.dtype} and {params.dtype}")
+    if codes.dim() != 5 or params.dim() != 6 or params.device != codes.device or not codes.is_cuda:
+        raise ValueError("4-bit cache: expected CUDA codes [2, B, NH, cap, D/2] and params [2, B, NH, cap, groups, 2]")
+    two, B, NH, cap, half = codes.shape
+    D = 2 * half
+    if D not in KV4_HEAD_DIMS:
+        raise ValueError(f"the 4-bit cache takes head_dim 16, 32, 64 or 128, got {D}")
+    G = kv4_groups(D)
+    if two != 2 or params.shape != (2, B, NH, cap, G, 2):
+        raise ValueError(f"4-bit cache: codes {tuple(codes.shape)} and params {tuple(params.shape)} do not match")
+    cs, ps = codes.stride(), params.stride()
+    si, sb, sh = cs[0] // half, cs[1] // half if B > 1 else NH * cap, cs[2] // half if NH > 1 else cap
+    if cs[3:] != (half, 1) or ps[3:] != (2 * G, 2, 1) or cs[0] % half or ps[0] != si * 2 * G \
+            or (B > 1 and (cs[1] % half or ps[1] != sb * 2 * G)) or (NH > 1 and (cs[2] % half or ps[2] != sh * 2 * G)):
+        raise ValueError("4-bit cache: rows must be contiguous and both arrays the same view")
+    return B, NH, cap, D, si, sb, sh
+
+
+def _kv4_marks(name, t, dtype, B, NH, rows, device):
+    """(address, sequence stride, head stride) of a [B, NH, >= rows] array beside the cache."""
+    if t is None:
+        return None, 0, 0
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != NH or t.shape[2] < rows or t.device != device:
+        raise ValueError(f"{name}: expected [{B}, {NH}, >= {rows}] on {device}, got {tuple(t.shape)} on {t.device}")
+    st = t.stride()
+    if st[2] != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    return t.data_ptr(), st[0], st[1]
+
+
+def _per_sequence(name, x, B, device):
+    """(device address or None, int to add) of an int or an int32 tensor of one entry per sequence."""
+    if not isinstance(x, torch.Tensor):
+        return None, int(x)
+    if x.dtype != torch.int32:
+        raise TypeError(f"{name}: expected an int or int32, got {x.dtype}")
+    if x.shape != (B,) or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{name}: expected {B} contiguous entries on {device}, got {tuple(x.shape)} on {x.device}")
+    return x.data_ptr(), 0
+
+
+def _call_on(device, name, *args):
+    """Call an entry point on the current stream of the tensors' device."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _scratch(workspace, need: int, device):
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous tensor on {device}")
+    return workspace
+
+
+def _token_rows(name, x, B, NH, D, device):
+    """Strides of a [B, T, NH, D] operand with contiguous rows."""
+    if x.dim() != 4 or x.shape[0] != B or x.shape[2] != NH or x.shape[3] != D or x.device != device:
+        raise ValueError(f"{name}: expected [{B}, T, {NH}, {D}] on {device}, got {tuple(x.shape)} on {x.device}")
+    st = x.stride()
+    if st[3] != 1:
+        raise ValueError(f"{name}: head_dim must be contiguous")
+    return st
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, pos, counts=None,
+              weights=None, positions=None, seen=None):
+    """Quantise keys and values [B, T, NH, D] (float32 or bfloat16, any strides with contiguous rows)
+    into slots pos .. pos+T-1 of a 4-bit cache.
+
+    ``pos`` is an int or an int32 tensor [B]; ``counts`` (int32 [B]) leaves the rows of shorter
+    sequences as they were.  ``weights`` (float32) and ``positions`` (int32), [B, NH, >= capacity], get 0 and
+    the token positions seen, seen+1, ... (``seen``: int or int32 [B], by default ``pos``)."""
+    B, NH, cap, D, si, sb, sh = _kv4_view(codes, params)
+    dev = codes.device
+    ks, vs = _token_rows("k", k, B, NH, D, dev), _token_rows("v", v, B, NH, D, dev)
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"kv4_store: k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+    T = k.shape[1]
+    if T == 0 or B == 0:
+        return
+    wp, wsb, wsh = _kv4_marks("weights", weights, torch.float32, B, NH, cap, dev)
+    pp, psb, psh = _kv4_marks("positions", positions, torch.int32, B, NH, cap, dev)
+    if wp is not None and pp is not None and (wsb, wsh) != (psb, psh):
+        raise ValueError("kv4_store: weights and positions must have the same strides")
+    if wp is None:
+        wsb, wsh = psb, psh
+    starts, start = _per_sequence("pos", pos, B, dev)
+    seen_p, seen0 = _per_sequence("seen", pos if seen is None else seen, B, dev)
+    counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
+    _call_on(dev, "attn_kv4_store", k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), B, T, NH, D, ks[0], ks[1], ks[2],
+             vs[0], vs[1], vs[2], codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, starts, start, counts_p, wp, pp,
+             wsb, wsh, seen_p, seen0)
+
+
+def kv4_load(codes: torch.Tensor, params: torch.Tensor, pos, T: int, dtype: torch.dtype = torch.float32, counts=None):
+    """The numbers held in slots pos .. pos+T-1 of a 4-bit cache: (k, v), each [B, T, NH, D] of
+    ``dtype``; zeros for the rows from ``counts`` on and for slots outside the cache."""
+    B, NH, cap, D, si, sb, sh = _kv4_view(codes, params)
+    dev = codes.device
+    k = torch.empty((B, T, NH, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if k.numel() == 0:
+        return k, v
+    starts, start = _per_sequence("pos", pos, B, dev)
+    counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
+    _call_on(dev, "attn_kv4_load", codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, B, T, NH, D, starts, start,
+             counts_p, k.data_ptr(), v.data_ptr(), dtype_code(dtype), T * NH * D, NH * D, D)
+    return k, v
+
+
+def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, length: int, lengths=None,
+               scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+               weights: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None):
+    """Single-query decode over a 4-bit cache: q [B, NH, D] -> out [B, NH, D] of q's dtype.
+
+    The cache's heads are shared by NH / (its heads) consecutive query heads.  Every sequence
+    attends over its first ``length`` rows, or ``lengths[b]`` (int32 [B], at most ``length``; none
+    gives zeros and lse -inf).  With ``weights`` (float32 [B, cached heads, >= length]) the attention
+    weights are added to it, in place or into ``weights_out``; with ``weights_out`` alone they are set."""
+    B, NKV, cap, D, si, sb, sh = _kv4_view(codes, params)
+    dev = codes.device
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.device != dev:
+        raise ValueError(f"q: expected [{B}, NH, {D}] on {dev}, got {tuple(q.shape)} on {q.device}")
+    NH = q.shape[1]
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("out: must have q's shape, dtype and device")
+    if lse is not None and (lse.shape != (B, NH) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev):
+        raise ValueError(f"lse: expected contiguous float32 [{B}, {NH}] on {dev}")
+    qs, os_ = q.stride(), out.stride()
+    if qs[2] != 1 or os_[2] != 1:
+        raise ValueError("kv4_decode: head_dim must be contiguous in q and out")
+    w_in, wsb, wsh = _kv4_marks("weights", weights, torch.float32, B, NKV, length, dev)
+    if weights_out is None or weights_out is weights:
+        w_out = w_in
+    else:
+        w_out, osb, osh = _kv4_marks("weights_out", weights_out, torch.float32, B, NKV, length, dev)
+        if w_in is not None and (osb, osh) != (wsb, wsh):
+            raise ValueError("kv4_decode: weights and weights_out must have the same strides")
+        wsb, wsh = osb, osh
+    lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    workspace = _scratch(workspace, lib.attn_kv4_decode_workspace_size(B, NH, length, D, w_out is not None), dev)
+    _call_on(dev, "attn_kv4_decode", q.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(),
+             lse.data_ptr() if lse is not None else None, B, NH, NKV, length, D, qs[0], qs[1], os_[0], os_[1], si, sb, sh,
+             cap, lengths_p, w_in, w_out, wsb, wsh, 1.0 / math.sqrt(D) if scale is None else float(scale),
+             dtype_code(q.dtype), workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return out
+
+
+def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: float | None = None, first_query: int = 0,
+                lengths=None, weights: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                dtype=None) -> torch.Tensor:
+    """Accumulated attention weights of a causal prompt, without its T x T matrix: [B, NKV, T] float32.
+
+    q [B, T, NH, D], k [B, T, NKV, D] (NH / NKV query heads to a key head), lse [B, NH, T] from
+    ``attention_forward``: each key's attention weight summed over the queries from ``first_query``
+    on (those from ``lengths[b]`` on excluded) and its query heads, added to ``weights`` when given.
+    ``dtype`` "tf32" for an lse that came from the tf32 forward."""
+    if q.dim() != 4 or k.dim() != 4 or q.dtype != k.dtype:
+        raise ValueError("key_weights: expected q [B, T, NH, D] and k [B, T, NKV, D] of one dtype")
+    B, T, NH, D = q.shape
+    NKV, dev = k.shape[2], q.device
+    qs, ks = _token_rows("q", q, B, NH, D, dev), _token_rows("k", k, B, NKV, D, dev)
+    if k.shape[1] != T:
+        raise ValueError(f"key_weights: q holds {T} tokens, k {k.shape[1]}")
+    if lse.shape != (B, NH, T) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
+        raise ValueError(f"lse: expected contiguous float32 [{B}, {NH}, {T}] on {dev}")
+    if out is None:
+        out = weights if weights is not None else torch.empty((B, NKV, T), dtype=torch.float32, device=dev)
+    w_out, wsb, wsh = _kv4_marks("out", out, torch.float32, B, NKV, T, dev)
+    w_in = None
+    if weights is not None:
+        w_in, isb, ish = _kv4_marks("weights", weights, torch.float32, B, NKV, T, dev)
+        if (isb, ish) != (wsb, wsh):
+            raise ValueError("key_weights: weights and out must have the same strides")
+    lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    _call_on(dev, "attn_key_weights", q.data_ptr(), k.data_ptr(), lse.data_ptr(), w_in, w_out, B, NH, NKV, T, D,
+             qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, int(first_query), lengths_p,
+             1.0 / math.sqrt(D) if scale is None else float(scale), dtype_code(q.dtype if dtype is None else dtype))
+    return out
+
+
+def kv4_evict(codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, positions, length: int, keep: int,
+              recent: int = 0, seen=None, lengths=None, out=None, slots: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Keep the ``keep`` best of the ``length`` (or ``lengths[b]``) rows of every head of a 4-bit cache:
+    those of the last ``recent`` of ``seen`` token positions, then those of the largest accumulated
+    weight (lowest slot among equals).  Kept rows below slot ``keep`` stay; the others fill the slots
+    given up below it.  Codes, params, weights and positions (int32, or None where a slot is its
+    position) move together, in place or into ``out`` = (codes, params, weights, positions) of another
+    cache.  ``seen``: int or int32 [B], by default ``length``.  Returns slots [B, NH, keep] int32: the
+    row each slot holds afterwards, -1 where there is none."""
+    B, NH, cap, D, si, sb, sh = _kv4_view(codes, params)
+    dev = codes.device
+    wp, wsb, wsh = _kv4_marks("weights", weights, torch.float32, B, NH, length, dev)
+    if wp is None:
+        raise ValueError("kv4_evict: weights are required")
+    pp, psb, psh = _kv4_marks("positions", positions, torch.int32, B, NH, length, dev)
+    if pp is not None and (psb, psh) != (wsb, wsh):
+        raise ValueError("kv4_evict: weights and positions must have the same strides")
+    dst = [None, None, None, None, 0, 0, 0, 0, 0, 0]
+    if out is not None:
+        oB, oNH, ocap, oD, osi, osb, osh = _kv4_view(out[0], out[1])
+        if (oB, oNH, oD) != (B, NH, D) or out[0].device != dev:
+            raise ValueError("kv4_evict: the destination's batch, heads or head_dim differ")
+        ow, owsb, owsh = _kv4_marks("out weights", out[2], torch.float32, B, NH, keep, dev)
+        op, opsb, opsh = _kv4_marks("out positions", out[3], torch.int32, B, NH, keep, dev)
+        if op is not None and (opsb, opsh) != (owsb, owsh):
+            raise ValueError("kv4_evict: the destination's weights and positions must have the same strides")
+        dst = [out[0].data_ptr(), out[1].data_ptr(), ow, op, osi, osb, osh, ocap, owsb, owsh]
+    if slots is None:
+        slots = torch.empty((B, NH, max(keep, 0)), dtype=torch.int32, device=dev)
+    elif slots.shape != (B, NH, keep) or slots.dtype != torch.int32 or not slots.is_contiguous() or slots.device != dev:
+        raise ValueError(f"slots: expected contiguous int32 [{B}, {NH}, {keep}] on {dev}")
+    seen_p, seen0 = _per_sequence("seen", length if seen is None else seen, B, dev)
+    if seen is None and lengths is not None:
+        seen_p, seen0 = _per_sequence("lengths", lengths, B, dev)
+    lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    workspace = _scratch(workspace, lib.attn_kv4_evict_workspace_size(B, NH, length, keep), dev)
+    _call_on(dev, "attn_kv4_evict", codes.data_ptr(), params.data_ptr(), wp, pp, si, sb, sh, cap, wsb, wsh, *dst,
+             B, NH, length, D, keep, recent, lengths_p, seen_p, seen0, slots.data_ptr(), workspace.data_ptr(),
+             workspace.numel() * workspace.element_size())
+    return slots
+
+
 def gemm(A: int, lda: int, a_trans: bool, B: int, ldb: int, b_trans: bool, ab_dtype: torch.dtype,
          C: int, ldc: int, c_dtype: torch.dtype, M: int, N: int, K: int, bias: int | None = None,
          accumulate: bool = False, max_ctas: int = 0):
