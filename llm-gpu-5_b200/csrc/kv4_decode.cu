@@ -3,20 +3,43 @@
 // For every query head h of sequence b, with n = lengths[b] cached rows of its key head,
 //   s_j = scale * q . k_j,  lse = log sum_j exp(s_j),  p_j = exp(s_j - lse),  o = sum_j p_j v_j,
 // and weights_out[j] = weights_in[j] + sum over the key head's query heads of p_j.  No rows: o = 0,
-// lse = -inf, no weight.  In a group, k = n s + m, so q . k_j = s sum_d q_d n_d + m sum_d q_d, and the
-// codes enter the products as small integers.  All sums and softmax statistics are float32.
+// lse = -inf, no weight.  In a group k = n s + m, so
+//   q . k_j = s_j sum_d q_d n_jd + m_j sum_d q_d          (the first sum a product with small integers)
+//   o_d     = sum_j (p_j s_j) n_jd + sum_j p_j m_j        (likewise; the second sum has no d)
+// A row of 64 values is 36 bytes, so at the HBM rate an SM receives a key and its value every 3 cycles: too
+// fast for 128 multiply-adds and as many conversions on the CUDA cores.  Both integer products go to
+// mma.sync (m16n8k16, f16 operands, f32 accumulation; a matrix with one useful column of eight for a
+// single query, which the idle tensor pipe does not mind), with the codes as the A operand:
+//   - n as a float16 costs no conversion: its four bits in the mantissa of a float16 with a zero exponent
+//     are a subnormal number, exactly n times a power of two.  The tensor core aligns products by their
+//     operands' exponents, -14 for any subnormal, and drops what lies 24 bits below the largest: codes
+//     at the top of the mantissa (n * 2^-18) keep float32's accuracy and take a shift and an AND per pair;
+//     codes left where they are (n * 2^-24, or 16 n * 2^-24 in the next nibble) take one AND, a shift for
+//     every other pair, and keep 2^-17.  Scores, and the value product of a float32 output, use the
+//     first; the value product of a bfloat16 output (2^-9 itself) the second.
+//   - which element sits in which k slot does not matter as long as the query agrees, so a lane takes
+//     consecutive codes of a key's row.
+//   - q is scaled by a power of two to below 2^12 and p s to below 2^15, which keeps float16's 11 bits at
+//     2^-35 of the largest and above.  bfloat16 queries are exact.  float32 ones go as two float16 parts
+//     in two columns of the same product, and so does p s for a float32 output (its second part 2^11
+//     times too large, so that small weights keep it too), so their products are good to 2^-22.
 //
-// The length is split over CTAs; each writes an unnormalised partial state (m, l, o[D]) and, where
-// weights are wanted, its p relative to its own maximum; the combine kernel merges the states and adds
-// the weights.
+// A warp takes tiles of 64 keys through a ring of its own of cp.async stages (no barrier between warps):
+// scores into shared memory, then one key per lane for the softmax, whose running maximum moves only
+// when it grows by more than 2^8 (the accumulators are rescaled then), then p s back as the B operand.
+// The length is split over CTAs; each writes an unnormalised partial state (m, l, o[D]) and the combine
+// kernel merges them and adds the weights.  A call with one split finishes in the first kernel.
+#include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
 
 namespace attn {
 
-constexpr int KD_THREADS = 128;
-constexpr int KD_CHUNK = 256;    // keys per split
+constexpr int KD_WARPS = 4;
+constexpr int KD_THREADS = KD_WARPS * 32;
+constexpr int KD_TILE = 64;      // keys per warp step
 constexpr int KD_WCHUNK = 1024;  // keys per combine CTA
+constexpr int KD_SPLIT = KD_TILE * KD_WARPS;  // keys a CTA takes in one round of its warps
 
 struct Kv4Decode {
   const void* q;
@@ -26,14 +49,535 @@ struct Kv4Decode {
   const float* w_in;
   float* w_out;
   int64_t q_sb, q_sh, o_sb, o_sh, w_sb, w_sh;
-  int NH, NKV, G, L, ns;
-  float scale_log2;
-  float* states;  // [B*NH][ns][D + 2]: max (log2 units), sum, unnormalised o
-  float* probs;   // [B*NH][L]: 2^(s - the split's max); NULL without weights
+  int NH, NKV, G, L;
+  int ns, per;     // splits, keys per split (a multiple of KD_TILE)
+  int nq, chunks;  // query heads per CTA, and CTAs' chunks of them per key head
+  float scale, scale_log2;
+  float* states;  // [B*NH][ns][D + 2]: max (log2 units), sum, unnormalised o; unused with one split
+  float* scores;  // [B*NH][L]: scores in log2 units; NULL without weights
 };
 
-static int kd_splits(int L) { return (L + KD_CHUNK - 1) / KD_CHUNK; }
-static size_t kd_states(int64_t BH, int L, int D) { return ((size_t)BH * kd_splits(L) * (D + 2) + 3) / 4 * 4; }
+// The most splits a call's keys are cut into: rounds of a CTA's warps, at least the two that a call
+// with weights and several chunks of query heads takes, and at most KD_MOST_SPLITS.
+constexpr int KD_MOST_SPLITS = 128;
+static int kd_most_splits(int L) {
+  const int rounds = (L + KD_SPLIT - 1) / KD_SPLIT;
+  return rounds < 2 ? 2 : rounds < KD_MOST_SPLITS ? rounds : KD_MOST_SPLITS;
+}
+static size_t kd_states(int64_t BH, int L, int D) { return ((size_t)BH * kd_most_splits(L) * (D + 2) + 3) / 4 * 4; }
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// max over the warp (NaN ignored)
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Codes in place: nibbles 0 and 1 of each half word (n * 2^-24 and 16 n * 2^-24 as float16).
+constexpr uint32_t KD_LOW = 0x000f000fu, KD_HIGH = 0x00f000f0u;
+// Nibble I of each half word at the top of a float16's mantissa: n * 2^-18.
+template <int I>
+__device__ __forceinline__ uint32_t kd_top(uint32_t w) {
+  constexpr int SHIFT = 6 - 4 * I;
+  return (SHIFT > 0 ? w << (SHIFT > 0 ? SHIFT : 0) : w >> (SHIFT > 0 ? 0 : -SHIFT)) & 0x03c003c0u;
+}
+// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs, in place or at the top.
+template <bool TOP, int PAIR>
+__device__ __forceinline__ void kd_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
+  if constexpr (TOP) {
+    a = kd_top<2 * PAIR>(w);
+    b = kd_top<2 * PAIR + 1>(w);
+  } else {
+    const uint32_t x = PAIR ? w >> 8 : w;
+    a = x & KD_LOW;
+    b = x & KD_HIGH;
+  }
+}
+// acc += (codes of one value row pair) * (p s): x holds four elements of two keys, y of two more.
+template <bool TOP, int PAIR>
+__device__ __forceinline__ void kd_value_mma(float (&acc)[4], uint32_t x, uint32_t y, uint32_t b0, uint32_t b1) {
+  uint32_t xa, xb, ya, yb;
+  kd_pairs<TOP, PAIR>(x, xa, xb);
+  kd_pairs<TOP, PAIR>(y, ya, yb);
+  mma_f16(acc, xa, xb, ya, yb, b0, b1);
+}
+
+// Sizes of a warp's shared memory for head_dim D and NQ queries.
+template <int D, int NQ, bool F32>
+struct KdTile {
+  static constexpr int GROUPS = kv4_groups(D);
+  static constexpr int COLS = F32 ? 2 * NQ : NQ;         // columns of the products
+  static constexpr int CODE_BYTES = KD_TILE * D / 2;     // one of K, V
+  static constexpr int PARAM_BYTES = KD_TILE * GROUPS * 4;
+  static constexpr int STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
+  static constexpr int STAGES = D >= 128 ? 2 : 3;
+  static constexpr int SC_LD = 68;                       // floats per query of the score tile (no bank conflicts)
+  static constexpr int P_LD = 80;                        // halves per column of the p s tile (likewise)
+  static constexpr int SC_BYTES = NQ * SC_LD * 4;
+  static constexpr int P_BYTES = GROUPS * COLS * P_LD * 2;
+  static constexpr int WARP = STAGES * STAGE + SC_BYTES + P_BYTES;
+  static constexpr int Q_FLOATS = NQ * D + NQ * (1 + GROUPS);
+  static constexpr int MERGE = KD_WARPS * NQ * (D + 2) * 4;  // the warps' states, over the stages at the end
+  static constexpr int BYTES = KD_WARPS * WARP + Q_FLOATS * 4;
+  static_assert(STAGE % 16 == 0 && SC_BYTES % 16 == 0 && P_BYTES % 16 == 0, "alignment");
+  static_assert(MERGE <= KD_WARPS * WARP, "the merge reuses the stages");
+};
+
+// o, lse and the accumulated weights of one query head from its merged maximum and sum.
+__device__ __forceinline__ float kd_lse(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY; }
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c, const Kv4Decode p) {
+  constexpr bool F32 = sizeof(T) == 4;
+  using S = KdTile<D, NQ, F32>;
+  constexpr int GROUPS = S::GROUPS, GS = kv4_group(D);
+  constexpr int MT = D / 16;   // 16-row tiles of the value product
+  constexpr int KS = D / 16;   // 16-deep steps of the score product
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int g = lane / 4, t = lane % 4;
+  uint8_t* ws = smem + warp * S::WARP;
+  float* sc = reinterpret_cast<float*>(ws + S::STAGES * S::STAGE);
+  __half* sp = reinterpret_cast<__half*>(ws + S::STAGES * S::STAGE + S::SC_BYTES);
+  float* sq = reinterpret_cast<float*>(smem + KD_WARPS * S::WARP);  // [NQ][D]
+  float* sfac = sq + NQ * D;                                        // [NQ]: score per unit of the product
+  float* ssum = sfac + NQ;                                          // [NQ][GROUPS]: scale * sum of q
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int split = blockIdx.x % p.ns;
+  const int unit = blockIdx.x / p.ns;  // (sequence, key head, chunk of its query heads)
+  const int chunk = unit % p.chunks, bk = unit / p.chunks;
+  const int b = bk / p.NKV, kvh = bk % p.NKV;
+  const int h0 = kvh * p.G + chunk * NQ, nq = min(NQ, p.G - chunk * NQ);
+  const int n = seq_length(p.lengths, b, p.L);
+  const int j0 = split * p.per, j1 = min(n, j0 + p.per);
+  const int tiles = j1 > j0 ? (j1 - j0 + KD_TILE - 1) / KD_TILE : 0;
+  const int64_t row0 = b * c.sb + kvh * c.sh;
+
+  // tile i of this warp: keys j0 + (i * KD_WARPS + warp) * KD_TILE on, rows rounded up to 16 (the
+  // capacity and the strides are multiples of 16 rows, so every copy is whole 16-byte pieces in bounds)
+  auto fetch = [&](int i) {
+    const int tile = i * KD_WARPS + warp;
+    if (tile < tiles) {
+      const int j = j0 + tile * KD_TILE;
+      const int rows = min(KD_TILE, (j1 - j + 15) / 16 * 16);
+      uint8_t* st = ws + (i % S::STAGES) * S::STAGE;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const int64_t row = which * c.si + row0 + j;
+        const uint8_t* src = c.codes + row * (D / 2);
+        uint8_t* dst = st + which * S::CODE_BYTES;
+#pragma unroll
+        for (int k = 0; k < S::CODE_BYTES / 512; ++k)
+          if ((k * 32 + lane) * 16 < rows * (D / 2)) cp_async16(dst + (k * 32 + lane) * 16, src + (k * 32 + lane) * 16);
+        const uint8_t* psrc = reinterpret_cast<const uint8_t*>(c.params + row * GROUPS);
+        uint8_t* pdst = st + 2 * S::CODE_BYTES + which * S::PARAM_BYTES;
+        if (lane * 16 < rows * GROUPS * 4) cp_async16(pdst + lane * 16, psrc + lane * 16);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
+
+  // the queries: float32 rows, each row's power of two, its groups' sums
+  for (int q = warp; q < NQ; q += KD_WARPS) {
+    float big = 0.f, sum[GROUPS];
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) sum[k] = 0.f;
+    float x[(D + 31) / 32];
+#pragma unroll
+    for (int k = 0; k < (D + 31) / 32; ++k) {
+      const int d = k * 32 + lane;
+      x[k] = q < nq && d < D ? Elem<T>::load((const T*)p.q + b * p.q_sb + (int64_t)(h0 + q) * p.q_sh + d) : 0.f;
+      big = fmaxf(big, fabsf(x[k]));
+      sum[k * 32 / GS] += x[k];
+    }
+    big = warp_max(big);
+    // 2^(11 - exponent of the largest), so that the scaled row is below 2^12; exponents are kept to
+    // where both powers are normal numbers
+    int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+    e = min(max(e, -110), 113);
+    const float up = __uint_as_float((uint32_t)(127 + 11 - e) << 23);
+#pragma unroll
+    for (int k = 0; k < (D + 31) / 32; ++k)
+      if (k * 32 + lane < D) sq[q * D + k * 32 + lane] = x[k] * up;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      const float total = warp_sum(sum[k]);
+      if (lane == 0) ssum[q * GROUPS + k] = total * p.scale_log2;
+    }
+    // the product carries the codes' 2^-18 and the row's `up`
+    if (lane == 0) sfac[q] = p.scale_log2 * __uint_as_float((uint32_t)(127 + 7 + e) << 23);
+  }
+  __syncthreads();
+
+  // B operand of the score product: column g holds query g (or part g % 2 of query g / 2), in the
+  // order in which lane t finds the codes of its part of a row
+  uint32_t qb[KS][2];
+  {
+    const int q = F32 ? g / 2 : g;
+    const bool use = g < S::COLS;
+    auto part = [&](float x) -> float {
+      const float hi = __half2float(__float2half_rn(x));
+      return F32 ? ((g & 1) ? x - hi : hi) : x;
+    };
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      // lane t's codes: D / 4 elements per row in runs of min(D / 4, 16) (a run per group); step s
+      // takes four of them: registers (e0, e1) and (e2, e3) at register-pair offsets
+      int e0, e1, e2, e3;
+      if constexpr (D >= 32) {
+        const int per_group = GS / 4;                       // elements of a group per lane
+        const int base = (s * 4 / per_group) * GS + t * per_group + (s * 4 % per_group) / 8 * 8;
+        const int o = (s & 1) * 2;                          // word nibbles 0,4 | 1,5 then 2,6 | 3,7
+        e0 = base + o; e1 = base + o + 4; e2 = base + o + 1; e3 = base + o + 5;
+      } else {
+        e0 = 4 * t; e1 = 4 * t + 2; e2 = 4 * t + 1; e3 = 4 * t + 3;
+      }
+      const float* row = sq + (use ? q : 0) * D;
+      qb[s][0] = use ? pack_h2(part(row[e0]), part(row[e1])) : 0u;
+      qb[s][1] = use ? pack_h2(part(row[e2]), part(row[e3])) : 0u;
+    }
+  }
+
+  float m[NQ], l[NQ], mg[NQ][GROUPS];
+  float acc[MT][4];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    m[q] = -INFINITY;
+    l[q] = 0.f;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) mg[q][k] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[i][k] = 0.f;
+  int ve = -100;  // exponent that the accumulated p s are scaled by: the largest value scale seen
+
+  for (int i = 0; i * KD_WARPS + warp < tiles; ++i) {
+    fetch(i + S::STAGES - 1);
+    cp_async_wait<S::STAGES - 1>();
+    __syncwarp();
+    const uint8_t* st = ws + (i % S::STAGES) * S::STAGE;
+    const __half2* kp = reinterpret_cast<const __half2*>(st + 2 * S::CODE_BYTES);
+    const __half2* vp = kp + KD_TILE * GROUPS;
+    const int j = j0 + (i * KD_WARPS + warp) * KD_TILE;
+
+    // ---- scores: C[key][column] = sum over the row's codes ----
+#pragma unroll
+    for (int mt = 0; mt < KD_TILE / 16; ++mt) {
+      float cs[GROUPS][4];
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) cs[k][0] = cs[k][1] = cs[k][2] = cs[k][3] = 0.f;
+      const uint8_t* ra = st + (mt * 16 + g) * (D / 2);
+      const uint8_t* rb = ra + 8 * (D / 2);
+      if constexpr (D >= 32) {
+        constexpr int WORDS = GS / 32;  // words of a group per lane
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+          uint32_t wa[WORDS], wb[WORDS];
+          if constexpr (WORDS == 2) {
+            const uint2 ua = *reinterpret_cast<const uint2*>(ra + k * 32 + t * 8);
+            const uint2 ub = *reinterpret_cast<const uint2*>(rb + k * 32 + t * 8);
+            wa[0] = ua.x; wa[1] = ua.y; wb[0] = ub.x; wb[1] = ub.y;
+          } else {
+            wa[0] = *reinterpret_cast<const uint32_t*>(ra + t * 4);
+            wb[0] = *reinterpret_cast<const uint32_t*>(rb + t * 4);
+          }
+#pragma unroll
+          for (int w = 0; w < WORDS; ++w) {
+            const int s = (k * WORDS + w) * 2;
+            mma_f16(cs[k], kd_top<0>(wa[w]), kd_top<0>(wb[w]), kd_top<1>(wa[w]), kd_top<1>(wb[w]), qb[s][0], qb[s][1]);
+            mma_f16(cs[k], kd_top<2>(wa[w]), kd_top<2>(wb[w]), kd_top<3>(wa[w]), kd_top<3>(wb[w]), qb[s + 1][0], qb[s + 1][1]);
+          }
+        }
+      } else {
+        // 4 codes per lane: byte 0 to the low half, byte 1 to the high half
+        const uint32_t xa = __byte_perm(*reinterpret_cast<const uint16_t*>(ra + t * 2), 0, 0x4140);
+        const uint32_t xb = __byte_perm(*reinterpret_cast<const uint16_t*>(rb + t * 2), 0, 0x4140);
+        mma_f16(cs[0], kd_top<0>(xa), kd_top<0>(xb), kd_top<1>(xa), kd_top<1>(xb), qb[0][0], qb[0][1]);
+      }
+      float r[4] = {cs[0][0], cs[0][1], cs[0][2], cs[0][3]};
+      if constexpr (GROUPS == 2) {  // the groups' scales belong to the key: rows g and g + 8
+        const float2 sa0 = __half22float2(kp[(mt * 16 + g) * 2]), sa1 = __half22float2(kp[(mt * 16 + g) * 2 + 1]);
+        const float2 sb0 = __half22float2(kp[(mt * 16 + g + 8) * 2]), sb1 = __half22float2(kp[(mt * 16 + g + 8) * 2 + 1]);
+        r[0] = sa0.x * cs[0][0] + sa1.x * cs[1][0];
+        r[1] = sa0.x * cs[0][1] + sa1.x * cs[1][1];
+        r[2] = sb0.x * cs[0][2] + sb1.x * cs[1][2];
+        r[3] = sb0.x * cs[0][3] + sb1.x * cs[1][3];
+      }
+      if constexpr (F32) {  // a query's two parts are one lane's two columns
+        if (t < NQ) {
+          sc[t * S::SC_LD + mt * 16 + g] = r[0] + r[1];
+          sc[t * S::SC_LD + mt * 16 + g + 8] = r[2] + r[3];
+        }
+      } else {
+        if (2 * t < NQ) {
+          sc[2 * t * S::SC_LD + mt * 16 + g] = r[0];
+          sc[2 * t * S::SC_LD + mt * 16 + g + 8] = r[2];
+        }
+        if (2 * t + 1 < NQ) {
+          sc[(2 * t + 1) * S::SC_LD + mt * 16 + g] = r[1];
+          sc[(2 * t + 1) * S::SC_LD + mt * 16 + g + 8] = r[3];
+        }
+      }
+    }
+    __syncwarp();
+
+    // ---- softmax: keys lane and lane + 32 of the tile ----
+    float ks[2][GROUPS], km[2][GROUPS], vs[2][GROUPS], vm[2][GROUPS];
+    bool valid[2];
+    float vbig = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = u * 32 + lane;
+      valid[u] = j + key < j1;
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) {
+        const float2 a = __half22float2(kp[key * GROUPS + k]), v = __half22float2(vp[key * GROUPS + k]);
+        ks[u][k] = a.x; km[u][k] = a.y;
+        vs[u][k] = valid[u] ? v.x : 0.f;
+        vm[u][k] = valid[u] ? v.y : 0.f;
+        vbig = fmaxf(vbig, vs[u][k]);
+      }
+    }
+    float z[NQ][2];
+    bool grow = false;
+    float top[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const float f = sfac[q];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float raw = sc[q * S::SC_LD + u * 32 + lane] * f;
+        float s = GROUPS == 1 ? raw * ks[u][0] : raw;
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) s = fmaf(km[u][k], ssum[q * GROUPS + k], s);
+        z[q][u] = valid[u] ? s : -INFINITY;
+      }
+      top[q] = warp_max(fmaxf(z[q][0], z[q][1]));
+      grow = grow || top[q] > m[q] + 8.f;
+    }
+    vbig = warp_max(vbig);
+    const int be = max((int)((__float_as_uint(vbig) >> 23) & 255u) - 127, -100);
+    if (grow || be > ve) {  // (warp-uniform) move the maxima, the values' exponent, and what was summed
+      const int ne = max(ve, be);
+      float corr[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const float nm = top[q] > m[q] + 8.f ? top[q] : m[q];
+        corr[q] = m[q] == -INFINITY ? 0.f : ex2(m[q] - nm);
+        m[q] = nm;
+        l[q] *= corr[q];
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) mg[q][k] *= corr[q];
+      }
+      const float ve_corr = ex2((float)(ve - ne));
+      ve = ne;
+      float c0 = 1.f, c1 = 1.f;  // of this lane's columns
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        if constexpr (F32) {
+          if (t == q) c0 = c1 = corr[q];
+        } else {
+          if (2 * t == q) c0 = corr[q];
+          if (2 * t + 1 == q) c1 = corr[q];
+        }
+      }
+      c0 *= ve_corr;
+      c1 *= ve_corr;
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {
+        acc[k][0] *= c0; acc[k][1] *= c1; acc[k][2] *= c0; acc[k][3] *= c1;
+      }
+    }
+    // p <= 2^8 and s 2^-ve < 2, so p s 2^(6 - ve) stays below 2^15
+    const float vup = __uint_as_float((uint32_t)(127 + 6 - ve) << 23);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = u * 32 + lane;
+      // position of the key among its 16 in the B operand: lane t's four slots are keys t, t+4, t+8, t+12
+      const int at = (key & ~15) + (key & 3) * 4 + ((key >> 2) & 3);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const float e = valid[u] ? ex2(z[q][u] - m[q]) : 0.f;
+        l[q] += e;
+        if (p.scores && valid[u] && q < nq) p.scores[((int64_t)b * p.NH + h0 + q) * p.L + j + key] = z[q][u];
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+          mg[q][k] = fmaf(e, vm[u][k], mg[q][k]);
+          const float ps = e * (vs[u][k] * vup);
+          const __half hi = __float2half_rn(ps);
+          __half* col = sp + (k * S::COLS + (F32 ? 2 * q : q)) * S::P_LD;
+          col[at] = hi;
+          if constexpr (F32) col[S::P_LD + at] = __float2half_rn((ps - __half2float(hi)) * 2048.f);
+        }
+      }
+    }
+    __syncwarp();
+
+    // ---- values: acc[d][column] += sum over the keys of codes * p s ----
+    const uint8_t* vc = st + S::CODE_BYTES;
+#pragma unroll
+    for (int kk = 0; kk < KD_TILE / 16; ++kk) {
+      const uint8_t* r0 = vc + (kk * 16 + t) * (D / 2);  // keys t, t+4, t+8, t+12
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) {
+        uint32_t b0 = 0, b1 = 0;
+        if (g < S::COLS) {
+          const uint2 u = *reinterpret_cast<const uint2*>(sp + (k * S::COLS + g) * S::P_LD + kk * 16 + t * 4);
+          b0 = u.x;
+          b1 = u.y;
+        }
+        if constexpr (D >= 64) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(r0 + k * 32 + g * 4);
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(r0 + 4 * (D / 2) + k * 32 + g * 4);
+          const uint32_t w2 = *reinterpret_cast<const uint32_t*>(r0 + 8 * (D / 2) + k * 32 + g * 4);
+          const uint32_t w3 = *reinterpret_cast<const uint32_t*>(r0 + 12 * (D / 2) + k * 32 + g * 4);
+          uint32_t x = __byte_perm(w0, w1, 0x5410), y = __byte_perm(w2, w3, 0x5410);  // elements 0..3
+          kd_value_mma<F32, 0>(acc[k * 4 + 0], x, y, b0, b1);
+          kd_value_mma<F32, 1>(acc[k * 4 + 1], x, y, b0, b1);
+          x = __byte_perm(w0, w1, 0x7632); y = __byte_perm(w2, w3, 0x7632);  // elements 4..7
+          kd_value_mma<F32, 0>(acc[k * 4 + 2], x, y, b0, b1);
+          kd_value_mma<F32, 1>(acc[k * 4 + 3], x, y, b0, b1);
+        } else if constexpr (D == 32) {
+          auto half_word = [&](int key) { return (uint32_t)*reinterpret_cast<const uint16_t*>(r0 + key * (D / 2) + g * 2); };
+          const uint32_t x = half_word(0) | half_word(4) << 16, y = half_word(8) | half_word(12) << 16;
+          kd_value_mma<F32, 0>(acc[0], x, y, b0, b1);
+          kd_value_mma<F32, 1>(acc[1], x, y, b0, b1);
+        } else {
+          auto byte = [&](int key) { return (uint32_t)r0[key * (D / 2) + g]; };
+          const uint32_t x = byte(0) | byte(4) << 16, y = byte(8) | byte(12) << 16;
+          kd_value_mma<F32, 0>(acc[0], x, y, b0, b1);
+        }
+      }
+    }
+    __syncwarp();  // the stage and the p s tile may be written again
+  }
+  cp_async_wait<0>();
+
+  // ---- the warps' states: [warp][query][D + 2] over the stages ----
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    l[q] = warp_sum(l[q]);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) mg[q][k] = warp_sum(mg[q][k]);
+  }
+  __syncthreads();
+  float* merge = reinterpret_cast<float*>(smem) + warp * NQ * (D + 2);
+  // the codes' 2^-18 or 2^-24 (16 times that in the odd rows) and p s's scaling
+  const float down = __uint_as_float((uint32_t)(127 + (F32 ? 18 : 24) - 6 + ve) << 23), down_odd = F32 ? down : down * 0.0625f;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    if (lane == 0) {
+      merge[q * (D + 2)] = m[q];
+      merge[q * (D + 2) + 1] = l[q];
+    }
+    const bool mine = F32 ? t == q : t == q / 2;
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {
+        constexpr int PER = GS / 8;  // elements of a group per lane row g
+        const int gr = k * 2 / PER, d = gr * GS + g * PER + (k * 2) % PER;
+        const float lo = F32 ? fmaf(acc[k][1], 1.f / 2048.f, acc[k][0]) : (q & 1) ? acc[k][1] : acc[k][0];
+        const float hi = F32 ? fmaf(acc[k][3], 1.f / 2048.f, acc[k][2]) : (q & 1) ? acc[k][3] : acc[k][2];
+        merge[q * (D + 2) + 2 + d] = fmaf(lo, down, mg[q][gr]);
+        merge[q * (D + 2) + 3 + d] = fmaf(hi, down_odd, mg[q][gr]);
+      }
+    }
+  }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  for (int i = threadIdx.x; i < nq * D; i += KD_THREADS) {
+    const int q = i / D, d = i % D, h = h0 + q;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < KD_WARPS; ++w) mx = fmaxf(mx, all[(w * NQ + q) * (D + 2)]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < KD_WARPS; ++w) {
+      const float* a = all + (w * NQ + q) * (D + 2);
+      const float f = ex2(a[0] - ref);
+      if (a[0] != -INFINITY || a[1] != 0.f) {
+        sum = fmaf(a[1], f, sum);
+        o = fmaf(a[2 + d], f, o);
+      }
+    }
+    const int64_t bh = (int64_t)b * p.NH + h;
+    if (p.ns > 1) {
+      float* stt = p.states + (bh * p.ns + split) * (D + 2);
+      stt[2 + d] = o;
+      if (d == 0) {
+        stt[0] = mx;
+        stt[1] = sum;
+      }
+    } else {
+      Elem<T>::store((T*)p.o + b * p.o_sb + h * p.o_sh + d, sum > 0.f || sum != sum ? o / sum : 0.f);
+      if (d == 0 && p.lse) p.lse[bh] = kd_lse(mx, sum);
+    }
+  }
+  if (p.ns == 1 && p.scores && p.chunks == 1) {  // one split over all of a key head's queries: the weights too
+    float mx[NQ], inv[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      mx[q] = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < KD_WARPS; ++w) mx[q] = fmaxf(mx[q], all[(w * NQ + q) * (D + 2)]);
+      const float ref = mx[q] == -INFINITY ? 0.f : mx[q];
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < KD_WARPS; ++w) {
+        const float* a = all + (w * NQ + q) * (D + 2);
+        if (a[0] != -INFINITY || a[1] != 0.f) sum = fmaf(a[1], ex2(a[0] - ref), sum);
+      }
+      mx[q] = ref;
+      inv[q] = 1.f / sum;
+    }
+    for (int key = threadIdx.x; key < p.L; key += KD_THREADS) {
+      float w = 0.f;
+      if (key < n)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          if (q < nq) w += ex2(p.scores[((int64_t)b * p.NH + h0 + q) * p.L + key] - mx[q]) * inv[q];
+      const int64_t at = b * p.w_sb + kvh * p.w_sh + key;
+      p.w_out[at] = (p.w_in ? p.w_in[at] : 0.f) + w;
+    }
+  }
+}
 
 __device__ __forceinline__ float block_reduce(float v, float* red, bool is_max) {
 #pragma unroll
@@ -49,70 +593,13 @@ __device__ __forceinline__ float block_reduce(float v, float* red, bool is_max) 
   return v;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(KD_THREADS) kv4_decode_partial_kernel(const Kv4View c, const Kv4Decode p) {
-  constexpr int G = kv4_groups(D), GS = kv4_group(D);
-  __shared__ float sq[D], sp[KD_CHUNK], red[KD_THREADS / 32];
-  grid_dependency_wait();
-  grid_dependents_launch();
-  const int bh = blockIdx.x / p.ns, split = blockIdx.x % p.ns;
-  const int b = bh / p.NH, h = bh % p.NH, kvh = h / p.G;
-  const int n = seq_length(p.lengths, b, p.L);
-  const int l0 = split * KD_CHUNK, l1 = min(n, l0 + KD_CHUNK);
-  const T* q = (const T*)p.q + b * p.q_sb + h * p.q_sh;
-  for (int d = threadIdx.x; d < D; d += KD_THREADS) sq[d] = Elem<T>::load(q + d) * p.scale_log2;
-  __syncthreads();
-  const int64_t row0 = b * c.sb + kvh * c.sh;
-  float mx = -INFINITY;
-  for (int j = l0 + threadIdx.x; j < l1; j += KD_THREADS) {
-    const uint8_t* code = c.codes + (row0 + j) * (D / 2);
-    float s = 0.f;
-    for (int g = 0; g < G; ++g) {
-      float dot = 0.f, qs = 0.f;
-      for (int d = 0; d < GS; ++d) {
-        const float x = sq[g * GS + d];
-        dot += x * (float)((code[(g * GS + d) / 2] >> (4 * (d & 1))) & 15);
-        qs += x;
-      }
-      const float2 sm = __half22float2(c.params[(row0 + j) * G + g]);
-      s += sm.x * dot + sm.y * qs;
-    }
-    sp[j - l0] = s;
-    mx = fmaxf(mx, s);
-  }
-  mx = block_reduce(mx, red, true);
-  float sum = 0.f;
-  for (int j = l0 + threadIdx.x; j < l1; j += KD_THREADS) {
-    const float e = exp2f(sp[j - l0] - mx);
-    sp[j - l0] = e;
-    sum += e;
-    if (p.probs) p.probs[(int64_t)bh * p.L + j] = e;
-  }
-  sum = block_reduce(sum, red, false);
-  __syncthreads();
-  float* st = p.states + ((int64_t)bh * p.ns + split) * (D + 2);
-  for (int d = threadIdx.x; d < D; d += KD_THREADS) {
-    float acc = 0.f;
-    for (int j = l0; j < l1; ++j) {
-      const int64_t row = c.si + row0 + j;
-      const float2 sm = __half22float2(c.params[row * G + d / GS]);
-      acc += sp[j - l0] * fmaf((float)((c.codes[row * (D / 2) + d / 2] >> (4 * (d & 1))) & 15), sm.x, sm.y);
-    }
-    st[2 + d] = acc;
-  }
-  if (threadIdx.x == 0) {
-    st[0] = mx;
-    st[1] = sum;
-  }
-}
-
 // One CTA per (KD_WCHUNK keys, sequence, key head); the first of them also writes o and lse.
 template <typename T, int D>
 __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv4Decode p) {
   __shared__ float red[KD_THREADS / 32];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int wchunks = p.probs ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
+  const int wchunks = p.scores ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
   const int bk = blockIdx.x / wchunks, chunk = blockIdx.x % wchunks;
   const int b = bk / p.NKV, kvh = bk % p.NKV;
   const int n = seq_length(p.lengths, b, p.L);
@@ -122,34 +609,38 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
 #pragma unroll
   for (int i = 0; i < PER; ++i) w[i] = 0.f;
   for (int g = 0; g < p.G; ++g) {
-    const int h = kvh * p.G + g, bh = b * p.NH + h;
-    const float* st = p.states + (int64_t)bh * p.ns * (D + 2);
-    float mx = -INFINITY, sum = 0.f;
-    for (int i = threadIdx.x; i < p.ns; i += KD_THREADS) mx = fmaxf(mx, st[(int64_t)i * (D + 2)]);
-    mx = block_reduce(mx, red, true);
-    if (mx == -INFINITY) mx = 0.f;
-    for (int i = threadIdx.x; i < p.ns; i += KD_THREADS)
-      sum += st[(int64_t)i * (D + 2) + 1] * exp2f(st[(int64_t)i * (D + 2)] - mx);
-    sum = block_reduce(sum, red, false);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    if (chunk == 0) {
-      for (int d = threadIdx.x; d < D; d += KD_THREADS) {
-        float acc = 0.f;
-        for (int i = 0; i < p.ns; ++i) acc += st[(int64_t)i * (D + 2) + 2 + d] * exp2f(st[(int64_t)i * (D + 2)] - mx);
-        Elem<T>::store((T*)p.o + b * p.o_sb + h * p.o_sh + d, acc * inv);
+    const int h = kvh * p.G + g;
+    const int64_t bh = (int64_t)b * p.NH + h;
+    float mx, sum;
+    if (p.ns > 1) {
+      const float* st = p.states + bh * p.ns * (D + 2);
+      mx = -INFINITY;
+      sum = 0.f;
+      for (int i = threadIdx.x; i < p.ns; i += KD_THREADS) mx = fmaxf(mx, st[(int64_t)i * (D + 2)]);
+      mx = block_reduce(mx, red, true);
+      if (mx == -INFINITY) mx = 0.f;
+      for (int i = threadIdx.x; i < p.ns; i += KD_THREADS)
+        sum += st[(int64_t)i * (D + 2) + 1] * ex2(st[(int64_t)i * (D + 2)] - mx);
+      sum = block_reduce(sum, red, false);
+      if (chunk == 0) {
+        for (int d = threadIdx.x; d < D; d += KD_THREADS) {
+          float acc = 0.f;
+          for (int i = 0; i < p.ns; ++i) acc += st[(int64_t)i * (D + 2) + 2 + d] * ex2(st[(int64_t)i * (D + 2)] - mx);
+          Elem<T>::store((T*)p.o + b * p.o_sb + h * p.o_sh + d, sum > 0.f || sum != sum ? acc / sum : 0.f);
+        }
+        if (threadIdx.x == 0 && p.lse) p.lse[bh] = kd_lse(mx, sum);
       }
-      if (threadIdx.x == 0 && p.lse) p.lse[bh] = n > 0 ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
-    if (p.probs) {
+    if (p.scores) {
+      const float inv = 1.f / sum;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int j = j0 + i * KD_THREADS + threadIdx.x;
-        if (j < j1 && j < n)
-          w[i] += p.probs[(int64_t)bh * p.L + j] * exp2f(st[(int64_t)(j / KD_CHUNK) * (D + 2)] - mx) * inv;
+        if (j < j1 && j < n) w[i] += ex2(p.scores[bh * p.L + j] - mx) * inv;
       }
     }
   }
-  if (p.probs) {
+  if (p.scores) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int j = j0 + i * KD_THREADS + threadIdx.x;
@@ -161,24 +652,55 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
   }
 }
 
-template <typename T, int D>
-static int kv4_decode_d(const Kv4View& c, const Kv4Decode& p, int B, cudaStream_t s) {
-  cudaError_t e = launch_pdl(kv4_decode_partial_kernel<T, D>, dim3((unsigned)p.ns * B * p.NH), dim3(KD_THREADS), 0, s, c, p);
+template <typename T, int D, int NQ>
+static int kv4_decode_q(const Kv4View& c, Kv4Decode p, int B, int sms, cudaStream_t s) {
+  using S = KdTile<D, NQ, sizeof(T) == 4>;
+  static_assert(S::BYTES <= 227 * 1024, "shared memory");
+  p.chunks = (p.G + NQ - 1) / NQ;
+  // enough splits that every SM holds several CTAs, each with at least one round of its warps
+  const int64_t units = (int64_t)B * p.NKV * p.chunks;
+  const int64_t want = ((int64_t)sms * 8 + units - 1) / units;
+  const int most = p.L <= KD_SPLIT ? 1 : kd_most_splits(p.L);
+  const int ns = (int)(want < most ? want : most);
+  const int tiles = (p.L + KD_TILE - 1) / KD_TILE;
+  p.per = (tiles + ns - 1) / ns * KD_TILE;
+  p.ns = (p.L + p.per - 1) / p.per;
+  if (p.ns == 1 && p.scores && p.chunks > 1) {  // the weights need every query's sum: use the combine kernel
+    p.per = (tiles + 1) / 2 * KD_TILE;
+    p.ns = 2;
+  }
+  static CtxOnce attr;
+  if (!set_smem_limit_once(kv4_decode_kernel<T, D, NQ>, S::BYTES, attr)) return ATTN_ERR_CUDA;
+  if (units * p.ns >= (int64_t)1 << 31) {
+    set_error("attn_kv4_decode: B*NH*L is too large for one launch; split the batch into several calls");
+    return ATTN_ERR_UNSUPPORTED;
+  }
+  cudaError_t e = launch_pdl(kv4_decode_kernel<T, D, NQ>, dim3((unsigned)(units * p.ns)), dim3(KD_THREADS), S::BYTES, s, c, p);
   count_launch();
-  if (int rc = check_launch("kv4_decode_partial_kernel", e)) return rc;
-  const int wc = p.probs ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
+  if (int rc = check_launch("kv4_decode_kernel", e)) return rc;
+  if (p.ns == 1) return ATTN_OK;
+  const int wc = p.scores ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
   e = launch_pdl(kv4_decode_combine_kernel<T, D>, dim3((unsigned)wc * B * p.NKV), dim3(KD_THREADS), 0, s, p);
   count_launch();
   return check_launch("kv4_decode_combine_kernel", e);
 }
 
+template <typename T, int D>
+static int kv4_decode_d(const Kv4View& c, const Kv4Decode& p, int B, int sms, cudaStream_t s) {
+  // a product has eight columns: eight queries, or four float32 ones in two parts each
+  if (p.G == 1) return kv4_decode_q<T, D, 1>(c, p, B, sms, s);
+  if (p.G == 2) return kv4_decode_q<T, D, 2>(c, p, B, sms, s);
+  if (sizeof(T) == 4 || p.G <= 4) return kv4_decode_q<T, D, 4>(c, p, B, sms, s);
+  return kv4_decode_q<T, D, sizeof(T) == 4 ? 4 : 8>(c, p, B, sms, s);
+}
+
 template <typename T>
-static int kv4_decode_t(const Kv4View& c, const Kv4Decode& p, int B, int D, cudaStream_t s) {
+static int kv4_decode_t(const Kv4View& c, const Kv4Decode& p, int B, int D, int sms, cudaStream_t s) {
   switch (D) {
-    case 16: return kv4_decode_d<T, 16>(c, p, B, s);
-    case 32: return kv4_decode_d<T, 32>(c, p, B, s);
-    case 64: return kv4_decode_d<T, 64>(c, p, B, s);
-    case 128: return kv4_decode_d<T, 128>(c, p, B, s);
+    case 16: return kv4_decode_d<T, 16>(c, p, B, sms, s);
+    case 32: return kv4_decode_d<T, 32>(c, p, B, sms, s);
+    case 64: return kv4_decode_d<T, 64>(c, p, B, sms, s);
+    case 128: return kv4_decode_d<T, 128>(c, p, B, sms, s);
   }
   return ATTN_ERR_UNSUPPORTED;
 }
@@ -206,10 +728,6 @@ extern "C" int attn_kv4_decode(const void* q, const void* codes, const void* par
   ATTN_REQUIRE(L > 0 && L <= capacity, "attn_kv4_decode: length %d outside 1 .. capacity %d", L, capacity);
   ATTN_REQUIRE(q_sb >= 0 && q_sh >= 0 && o_sb >= 0 && o_sh >= 0 && w_sb >= 0 && w_sh >= 0, "attn_kv4_decode: strides must not be negative");
   ATTN_REQUIRE(!weights_in || weights_out, "attn_kv4_decode: weights_in needs weights_out");
-  if ((int64_t)B * NH * kd_splits(L) >= (int64_t)1 << 31) {
-    set_error("attn_kv4_decode: B*NH*L is too large for one launch; split the batch into several calls");
-    return ATTN_ERR_UNSUPPORTED;
-  }
   const size_t need = attn_kv4_decode_workspace_size(B, NH, L, D, weights_out != nullptr);
   if (!workspace || workspace_bytes < need) {
     set_error("attn_kv4_decode: workspace of %zu bytes required", need);
@@ -219,9 +737,12 @@ extern "C" int attn_kv4_decode(const void* q, const void* codes, const void* par
   Kv4Decode p = {};
   p.q = q; p.o = o; p.lse = lse; p.lengths = lengths; p.w_in = weights_in; p.w_out = weights_out;
   p.q_sb = q_sb; p.q_sh = q_sh; p.o_sb = o_sb; p.o_sh = o_sh; p.w_sb = w_sb; p.w_sh = w_sh;
-  p.NH = NH; p.NKV = NKV; p.G = NH / NKV; p.L = L; p.ns = kd_splits(L);
+  p.NH = NH; p.NKV = NKV; p.G = NH / NKV; p.L = L;
+  p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.states = (float*)workspace;
-  p.probs = weights_out ? p.states + kd_states((int64_t)B * NH, L, D) : nullptr;
-  return dtype == ATTN_BF16 ? kv4_decode_t<__nv_bfloat16>(c, p, B, D, as_stream(stream)) : kv4_decode_t<float>(c, p, B, D, as_stream(stream));
+  p.scores = weights_out ? p.states + kd_states((int64_t)B * NH, L, D) : nullptr;
+  const int sms = current_device_sms();
+  return dtype == ATTN_BF16 ? kv4_decode_t<__nv_bfloat16>(c, p, B, D, sms, as_stream(stream))
+                            : kv4_decode_t<float>(c, p, B, D, sms, as_stream(stream));
 }
