@@ -94,8 +94,8 @@ uint64_t attn_launch_count(void);
  * instead of hanging, so its outputs are incomplete).  Codes are grouped by kernel: 1xx the GEMM
  * (106: its dynamic shared memory did not start 1024-byte aligned, checked before any work),
  * 2xx the attention forward, 3xx the attention backward (300: its dynamic shared memory did not
- * start 1024-byte aligned, checked before any work), 4xx the barriers of attn_grad_allreduce, 900
- * the self-test below.  The word keeps the first code until it is cleared; a set word does not
+ * start 1024-byte aligned, checked before any work), 4xx the barriers of attn_grad_allreduce, 5xx
+ * attn_key_weights, 900 the self-test below.  The word keeps the first code until it is cleared; a set word does not
  * affect later launches (each launch only stops early for a wait of its own that gave up).
  * Synchronises with the device.
  * clear != 0 resets it to 0.  Has no counterpart in the reference, whose kernels cannot give up.
@@ -275,20 +275,25 @@ int attn_kv4_decode(const void* q, const void* codes, const void* params, void* 
                     int64_t w_sb, int64_t w_sh, float scale, int dtype,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* Bytes of workspace attn_key_weights needs (may be 0). */
+size_t attn_key_weights_workspace_size(int B, int NKV, int T);
+
 /*
  * Accumulated attention weights of a causal prompt: weights_out[b, h, j] = weights_in[b, h, j] (NULL: 0;
  * may be the same array) + the sum over the NH / NKV query heads of key head h and the queries
  * i, max(j, first_query) <= i < lengths[b] (NULL: T), of exp(scale q_i . k_j - lse_i), with the lse
  * [B, NH, T] that attn_fwd wrote: the column sums of attn_probs' matrix without storing it.  Keys
  * from lengths[b] on get weights_in.  q: element (b, t, h, d) at q[b*q_sb + t*q_st + h*q_sh + d], k
- * likewise; element (b, h, j) of the weights at b*w_sb + h*w_sh + j.  head_dim up to 128.  ATTN_TF32:
- * q and k truncated to tf32, as attn_fwd's tf32 path reads them (head_dim <= 32).
+ * likewise; element (b, h, j) of the weights at b*w_sb + h*w_sh + j.  head_dim up to 128.  ATTN_BF16 with
+ * head_dim a multiple of 8 up to 64 and ATTN_TF32 with a multiple of 4 up to 32 (16-byte aligned, strides in
+ * 16-byte steps) run on the tensor cores, the rest on CUDA cores; ATTN_TF32 truncates q and k to tf32 either
+ * way, as attn_fwd's tf32 path reads them.
  */
 int attn_key_weights(const void* q, const void* k, const float* lse, const float* weights_in,
                      float* weights_out, int B, int NH, int NKV, int T, int D,
                      int64_t q_sb, int64_t q_st, int64_t q_sh, int64_t k_sb, int64_t k_st, int64_t k_sh,
                      int64_t w_sb, int64_t w_sh, int first_query, const int* lengths,
-                     float scale, int dtype, void* stream);
+                     float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace attn_kv4_evict needs. */
 size_t attn_kv4_evict_workspace_size(int B, int NH, int L, int keep);

@@ -4,10 +4,18 @@
 // the column sums of the causal softmax whose row statistics attn_fwd left in lse.  The T x T matrix
 // (attn_probs, the reference's cache_attn_weights) is never stored.
 //
-// A thread takes one key and a CTA 128 of them; queries pass through shared memory in tiles of 32 and
-// a thread forms 8 scores at a time, so that each value of its key is read once for 8 products.
+// bfloat16 (head_dim to 64) and tf32 (to 32) run on the tensor cores: a CTA takes 128 keys and streams
+// the queries past them in tiles of 128, S^T = K Q^T by tcgen05.mma into TMEM with the keys on the lanes, so
+// that a thread owns one key and its sum needs no other thread.  Per score there is one multiply-add, one ex2
+// and one addition: at 16 ex2 per clock and SM a 128 x 128 tile takes 1,024 cycles there, four times its
+// MMA, so the special-function unit bounds it.  Two CTAs share an SM (256 TMEM columns each, two score
+// tiles), so that one's loads and hand-overs hide behind the other's exponentials.
+//
+// Other shapes and float32 run on CUDA cores: a thread takes one key and a CTA 128 of them; queries pass
+// through shared memory in tiles of 32 and a thread forms 8 scores at a time, so that each value of its key is
+// read once for 8 products.
+#include "attn_tc_common.cuh"
 #include "kv4.cuh"
-#include "tc_common.cuh"
 #include <math.h>
 
 namespace attn {
@@ -94,14 +102,328 @@ static int key_weights_simt(const KeyWeights& p, int B, int dtype, cudaStream_t 
   return check_launch("key_weights_simt_kernel", e);
 }
 
+
+// ---- tensor cores ------------------------------------------------------------------------------
+constexpr int KT_STAGES = 3;                 // query tiles in flight
+constexpr int KT_THREADS = 192;              // 4 warps of sums, a TMA warp, an MMA warp
+constexpr int KT_TMEM = 256;                 // two 128-column score tiles
+constexpr int KT_SMEM = 1024 + (2 + KT_STAGES) * AT_TILE_BYTES + 4 * 2 * AT_TILE * 4 + 256;
+
+struct KwMaps {
+  TileMap q, k;
+};
+
+struct KwTc {
+  KeyWeights p;
+  int nt, parts, BK, units;  // key tiles, parts of a key tile's queries, B*NKV
+  float* partial;            // [parts][B*NKV][T] when parts > 1
+  int* err;
+};
+
+struct KwBars {
+  uint64_t k_full[2], k_empty[2], q_full[KT_STAGES], q_empty[KT_STAGES], s_full[2], s_free[2];
+  uint32_t tmem;
+};
+
+// One unit of work: key tile jt of (b, kvh), query tiles [lo, nt) of each of the G query heads in turn,
+// of which this part takes the steps [begin, end).
+struct KwUnit {
+  int b, kvh, jt, part, n, lo, span, begin, end;
+  __device__ __forceinline__ void set(const KwTc& a, int u) {
+    const int bk = u % a.BK, level = u / a.BK;  // the longest key tiles (the first) come first
+    part = level % a.parts;
+    jt = level / a.parts;
+    b = bk / a.p.NKV;
+    kvh = bk - b * a.p.NKV;
+    n = seq_length(a.p.lengths, b, a.p.T);
+    lo = max(jt, a.p.first / AT_TILE);
+    span = max((n + AT_TILE - 1) / AT_TILE - lo, 0);
+    const int total = span * a.p.G;
+    begin = (int)((int64_t)total * part / a.parts);
+    end = (int)((int64_t)total * (part + 1) / a.parts);
+  }
+};
+
+// Wait for a load that is known to be in flight, after a wait elsewhere gave up: at most 0.1 s.
+__device__ __forceinline__ void drain_load(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait_sleep(bar, parity, 200000u))
+    if (globaltimer_ns() - t0 > 100000000ull) return;
+}
+
+template <bool TF32>
+__global__ void __launch_bounds__(KT_THREADS, 2)
+key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwTc a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;                                   // [2]
+  uint8_t* sQ = sK + 2 * AT_TILE_BYTES;                 // [KT_STAGES]
+  float* sL = reinterpret_cast<float*>(sQ + KT_STAGES * AT_TILE_BYTES);  // [4 warps][2][128]
+  KwBars* bars = reinterpret_cast<KwBars*>(sL + 4 * 2 * AT_TILE);
+  const WaitErr werr = wait_err(a.err);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->k_full[i], 1);
+      mbar_init(&bars->k_empty[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->s_free[i], 4);
+    }
+    for (int i = 0; i < KT_STAGES; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_empty[i], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(&bars->tmem, KT_TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  grid_dependency_wait();
+  grid_dependents_launch();
+
+  if (warp == 4) {
+    // ---------------- TMA ----------------
+    if (lane == 0) {
+      int ku = 0, qn = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+        KwUnit w;
+        w.set(a, u);
+        if (w.begin >= w.end) continue;
+        const int ks = ku & 1;
+        if (!mbar_wait(&bars->k_empty[ks], ((ku >> 1) & 1) ^ 1, werr, 501)) { ok = false; break; }
+        mbar_arrive_expect_tx(&bars->k_full[ks], AT_TILE_BYTES);
+        load_tile(sK + ks * AT_TILE_BYTES, maps.k, &bars->k_full[ks], w.b, w.kvh, w.jt * AT_TILE);
+        ++ku;
+        for (int i = w.begin; i < w.end; ++i, ++qn) {
+          const int qs = qn % KT_STAGES;
+          if (!mbar_wait(&bars->q_empty[qs], ((qn / KT_STAGES) & 1) ^ 1, werr, 502)) { ok = false; break; }
+          mbar_arrive_expect_tx(&bars->q_full[qs], AT_TILE_BYTES);
+          load_tile(sQ + qs * AT_TILE_BYTES, maps.q, &bars->q_full[qs], w.b, w.kvh * a.p.G + i / w.span,
+                    (w.lo + i % w.span) * AT_TILE);
+        }
+      }
+      if (!ok) {  // leave no load of this CTA's behind
+        for (int i = max(0, ku - 2); i < ku; ++i) drain_load(&bars->k_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, qn - KT_STAGES); i < qn; ++i) drain_load(&bars->q_full[i % KT_STAGES], (i / KT_STAGES) & 1);
+      }
+    }
+  } else if (warp == 5) {
+    // ---------------- MMA ----------------
+    if (lane == 0) {
+      const uint32_t idesc = TF32 ? idesc_tf32_f32(128, 128, 0, 0) : idesc_bf16_f32(128, 128, 0, 0);
+      int ku = 0, qn = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+        KwUnit w;
+        w.set(a, u);
+        if (w.begin >= w.end) continue;
+        const int ks = ku & 1;
+        if (!mbar_wait(&bars->k_full[ks], (ku >> 1) & 1, werr, 503)) break;
+        const uint64_t k_desc = smem_desc_sw128(smem_u32(sK + ks * AT_TILE_BYTES), 16, 1024);
+        for (int i = w.begin; i < w.end; ++i, ++qn) {
+          const int qs = qn % KT_STAGES, buf = qn & 1;
+          if (!mbar_wait(&bars->q_full[qs], (qn / KT_STAGES) & 1, werr, 504) ||
+              !mbar_wait(&bars->s_free[buf], ((qn >> 1) & 1) ^ 1, werr, 505)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ + qs * AT_TILE_BYTES), 16, 1024);
+#pragma unroll
+          for (int k = 0; k < AT_D / 16; ++k) {
+            if constexpr (TF32)
+              umma_ss_tf32(tmem + buf * 128, desc_step(k_desc, k * 32), desc_step(q_desc, k * 32), idesc, k > 0 ? 1u : 0u);
+            else
+              umma_ss(tmem + buf * 128, desc_step(k_desc, k * 32), desc_step(q_desc, k * 32), idesc, k > 0 ? 1u : 0u);
+          }
+          umma_commit(&bars->s_full[buf]);
+          umma_commit(&bars->q_empty[qs]);
+          if (i + 1 == w.end) umma_commit(&bars->k_empty[ks]);
+        }
+        ++ku;
+      }
+    }
+  } else {
+    // ---------------- sums: thread = key ----------------
+    float* sl = sL + warp * 2 * AT_TILE;
+    const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16);
+    const float c = a.p.scale_log2;
+    int qn = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+      KwUnit w;
+      w.set(a, u);
+      const int row = warp * 32 + lane, j = w.jt * AT_TILE + row;
+      float total = 0.f;
+      // -lse in log2 units of the next tile's queries, four per lane, fetched a tile ahead
+      float next[4];
+      auto fetch = [&](int i) {
+        const int h = w.kvh * a.p.G + i / w.span, i0 = (w.lo + i % w.span) * AT_TILE;
+        const float* src = a.p.lse + ((int64_t)w.b * a.p.NH + h) * a.p.T + i0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) next[k] = i0 + k * 32 + lane < w.n ? src[k * 32 + lane] * -LOG2E : 0.f;
+      };
+      if (w.begin < w.end) fetch(w.begin);
+      for (int i = w.begin; i < w.end; ++i, ++qn) {
+        const int buf = qn & 1, i0 = (w.lo + i % w.span) * AT_TILE;
+        float* lb = sl + buf * AT_TILE;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) lb[k * 32 + lane] = next[k];
+        __syncwarp();
+        if (i + 1 < w.end) fetch(i + 1);
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[buf], (qn >> 1) & 1, werr, 506))) { ok = false; break; }
+        tc_fence_after();
+        // columns of this tile that count for this key: queries from max(j, first) to n - 1
+        const int c0 = max(j, a.p.first) - i0, c1 = w.n - i0;
+        const bool whole = i0 >= w.jt * AT_TILE + AT_TILE && i0 >= a.p.first && c1 >= AT_TILE;
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t sr[32];
+          tmem_ld32(tS + buf * 128 + cc * 32, sr);
+          tmem_wait_ld();
+          if (cc == 3) {  // the scores are in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->s_free[buf]);
+          }
+          const float4* l4 = reinterpret_cast<const float4*>(lb + cc * 32);
+          if (whole) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 l = l4[k];
+              s0 += ex2_approx(fmaf(__uint_as_float(sr[4 * k]), c, l.x));
+              s1 += ex2_approx(fmaf(__uint_as_float(sr[4 * k + 1]), c, l.y));
+              s2 += ex2_approx(fmaf(__uint_as_float(sr[4 * k + 2]), c, l.z));
+              s3 += ex2_approx(fmaf(__uint_as_float(sr[4 * k + 3]), c, l.w));
+            }
+          } else if (cc * 32 + 31 >= __reduce_min_sync(0xffffffffu, c0)) {
+            // (a chunk before every lane's first query is skipped.)  Unused scores may be anything, NaN
+            // too: they are replaced, not multiplied
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 l = l4[k];
+              const int col = cc * 32 + 4 * k;
+              const float e0 = ex2_approx(fmaf(__uint_as_float(sr[4 * k]), c, l.x));
+              const float e1 = ex2_approx(fmaf(__uint_as_float(sr[4 * k + 1]), c, l.y));
+              const float e2 = ex2_approx(fmaf(__uint_as_float(sr[4 * k + 2]), c, l.z));
+              const float e3 = ex2_approx(fmaf(__uint_as_float(sr[4 * k + 3]), c, l.w));
+              s0 += col >= c0 && col < c1 ? e0 : 0.f;
+              s1 += col + 1 >= c0 && col + 1 < c1 ? e1 : 0.f;
+              s2 += col + 2 >= c0 && col + 2 < c1 ? e2 : 0.f;
+              s3 += col + 3 >= c0 && col + 3 < c1 ? e3 : 0.f;
+            }
+          }
+        }
+        total += (s0 + s1) + (s2 + s3);
+      }
+      if (!ok) break;
+      if (j < a.p.T) {
+        const float sum = j < w.n ? total : 0.f;
+        if (a.parts > 1) {
+          a.partial[((int64_t)w.part * a.BK + (int64_t)w.b * a.p.NKV + w.kvh) * a.p.T + j] = sum;
+        } else {
+          const int64_t at = w.b * a.p.w_sb + w.kvh * a.p.w_sh + j;
+          a.p.w_out[at] = (a.p.w_in ? a.p.w_in[at] : 0.f) + sum;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, KT_TMEM);
+  }
+}
+
+__global__ void __launch_bounds__(256) key_weights_join_kernel(const KwTc a) {
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.BK * a.p.T) return;
+  const int bk = (int)(i / a.p.T), j = (int)(i - (int64_t)bk * a.p.T);
+  float sum = 0.f;
+  for (int k = 0; k < a.parts; ++k) sum += a.partial[((int64_t)k * a.BK + bk) * a.p.T + j];
+  const int64_t at = bk / a.p.NKV * a.p.w_sb + bk % a.p.NKV * a.p.w_sh + j;
+  a.p.w_out[at] = (a.p.w_in ? a.p.w_in[at] : 0.f) + sum;
+}
+
+// Parts that a key tile's queries are cut into: one while there are four units for every CTA.
+static int key_weights_parts(int B, int NKV, int T) {
+  const int64_t units = (int64_t)B * NKV * ((T + AT_TILE - 1) / AT_TILE);
+  const int64_t want = 4 * 2 * 148;
+  if (units >= want / 2) return 1;
+  const int64_t parts = (want + units - 1) / units, most = (T + AT_TILE - 1) / AT_TILE;
+  return (int)(parts < most ? parts : most);
+}
+
+static bool key_weights_tc_ok(const KeyWeights& p, int dtype) {
+  const int64_t q[3] = {p.q_sb, p.q_st, p.q_sh}, k[3] = {p.k_sb, p.k_st, p.k_sh};
+  if (!aligned(p.q, 16) || !aligned(p.k, 16)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (q[i] <= 0 || k[i] <= 0) return false;  // broadcast axes have no tensor map
+  if (dtype == ATTN_TF32)
+    return tc_head_dim_ok_tf32(p.D) && head_strides_ok_f32(q[0], q[1], q[2], p.D) && head_strides_ok_f32(k[0], k[1], k[2], p.D);
+  return dtype == ATTN_BF16 && tc_head_dim_ok(p.D) && head_strides_ok(q[0], q[1], q[2], p.D) &&
+         head_strides_ok(k[0], k[1], k[2], p.D);
+}
+
+static int key_weights_tc(const KeyWeights& p, int B, int tf32, float* partial, cudaStream_t s) {
+  KwMaps maps;
+  if (tf32) {
+    if (!make_head_map_f32(&maps.q, p.q, B, p.NH, p.T, p.D, p.q_sb, p.q_st, p.q_sh, 128) ||
+        !make_head_map_f32(&maps.k, p.k, B, p.NKV, p.T, p.D, p.k_sb, p.k_st, p.k_sh, 128))
+      return ATTN_ERR_CUDA;
+  } else if (!make_head_map(&maps.q, p.q, B, p.NH, p.T, p.D, p.q_sb, p.q_st, p.q_sh) ||
+             !make_head_map(&maps.k, p.k, B, p.NKV, p.T, p.D, p.k_sb, p.k_st, p.k_sh)) {
+    return ATTN_ERR_CUDA;
+  }
+  KwTc a;
+  a.p = p;
+  a.nt = (p.T + AT_TILE - 1) / AT_TILE;
+  a.parts = key_weights_parts(B, p.NKV, p.T);
+  a.BK = B * p.NKV;
+  const int64_t units = (int64_t)a.BK * a.nt * a.parts;
+  a.units = (int)units;
+  a.partial = partial;
+  a.err = dev_error_ptr();
+  if (!a.err) return ATTN_ERR_CUDA;
+  const int64_t ctas = 2 * (int64_t)current_device_sms();
+  const unsigned grid = (unsigned)(units < ctas ? units : ctas);
+  static CtxOnce attr[2];
+  if (!(tf32 ? set_smem_limit_once(key_weights_tc_kernel<true>, KT_SMEM, attr[1])
+             : set_smem_limit_once(key_weights_tc_kernel<false>, KT_SMEM, attr[0])))
+    return ATTN_ERR_CUDA;
+  cudaError_t e = tf32 ? launch_pdl(key_weights_tc_kernel<true>, dim3(grid), dim3(KT_THREADS), KT_SMEM, s, maps, a)
+                       : launch_pdl(key_weights_tc_kernel<false>, dim3(grid), dim3(KT_THREADS), KT_SMEM, s, maps, a);
+  count_launch();
+  if (int rc = check_launch("key_weights_tc_kernel", e)) return rc;
+  if (a.parts == 1) return ATTN_OK;
+  const int64_t n = (int64_t)a.BK * p.T;
+  e = launch_pdl(key_weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+  count_launch();
+  return check_launch("key_weights_join_kernel", e);
+}
+
 }  // namespace attn
 
 using namespace attn;
 
+extern "C" size_t attn_key_weights_workspace_size(int B, int NKV, int T) {
+  if (B <= 0 || NKV <= 0 || T <= 0) return 0;
+  const int parts = key_weights_parts(B, NKV, T);
+  return parts > 1 ? (size_t)parts * B * NKV * T * sizeof(float) : 0;
+}
+
 extern "C" int attn_key_weights(const void* q, const void* k, const float* lse, const float* weights_in,
                                 float* weights_out, int B, int NH, int NKV, int T, int D, int64_t q_sb, int64_t q_st,
                                 int64_t q_sh, int64_t k_sb, int64_t k_st, int64_t k_sh, int64_t w_sb, int64_t w_sh,
-                                int first_query, const int* lengths, float scale, int dtype, void* stream) {
+                                int first_query, const int* lengths, float scale, int dtype, void* workspace,
+                                size_t workspace_bytes, void* stream) {
   clear_error();
   ATTN_REQUIRE(q && k && lse && weights_out, "attn_key_weights: null pointer argument");
   ATTN_REQUIRE(dtype == ATTN_F32 || dtype == ATTN_BF16 || dtype == ATTN_TF32, "attn_key_weights: bad dtype");
@@ -116,11 +438,18 @@ extern "C" int attn_key_weights(const void* q, const void* k, const float* lse, 
     set_error("attn_key_weights: head_dim %d not supported (up to 128)", D);
     return ATTN_ERR_UNSUPPORTED;
   }
-  if ((int64_t)B * NKV * ((T + KW_KEYS - 1) / KW_KEYS) >= (int64_t)1 << 31) {
+  if ((int64_t)B * NKV * ((T + KW_KEYS - 1) / KW_KEYS) >= (int64_t)1 << 30) {
     set_error("attn_key_weights: too many key tiles for one launch; split the batch into several calls");
     return ATTN_ERR_UNSUPPORTED;
   }
   const KeyWeights p = {q, k, lse, weights_in, weights_out, q_sb, q_st, q_sh, k_sb, k_st, k_sh, w_sb, w_sh,
                         NH, NKV, NH / NKV, T, D, first_query, lengths, scale * 1.4426950408889634f};
+  const size_t need = attn_key_weights_workspace_size(B, NKV, T);
+  if (need && (!workspace || workspace_bytes < need)) {
+    set_error("attn_key_weights: workspace of %zu bytes required", need);
+    return ATTN_ERR_WORKSPACE;
+  }
+  ATTN_REQUIRE(aligned(workspace, 4), "attn_key_weights: misaligned workspace");
+  if (key_weights_tc_ok(p, dtype)) return key_weights_tc(p, B, dtype == ATTN_TF32, (float*)workspace, as_stream(stream));
   return key_weights_simt(p, B, dtype, as_stream(stream));
 }

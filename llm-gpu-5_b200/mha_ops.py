@@ -313,7 +313,7 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
 
 def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: float | None = None, first_query: int = 0,
                 lengths=None, weights: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                dtype=None) -> torch.Tensor:
+                dtype=None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Accumulated attention weights of a causal prompt, without its T x T matrix: [B, NKV, T] float32.
 
     q [B, T, NH, D], k [B, T, NKV, D] (NH / NKV query heads to a key head), lse [B, NH, T] from
@@ -338,9 +338,13 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
         if (isb, ish) != (wsb, wsh):
             raise ValueError("key_weights: weights and out must have the same strides")
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    need = lib.attn_key_weights_workspace_size(B, NKV, T)
+    if need or workspace is not None:
+        workspace = _scratch(workspace, need, dev)
     _call_on(dev, "attn_key_weights", q.data_ptr(), k.data_ptr(), lse.data_ptr(), w_in, w_out, B, NH, NKV, T, D,
              qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, int(first_query), lengths_p,
-             1.0 / math.sqrt(D) if scale is None else float(scale), dtype_code(q.dtype if dtype is None else dtype))
+             1.0 / math.sqrt(D) if scale is None else float(scale), dtype_code(q.dtype if dtype is None else dtype),
+             None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel() * workspace.element_size())
     return out
 
 

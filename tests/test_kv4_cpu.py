@@ -41,7 +41,7 @@ def _decode(**kw):
 
 def _weights(**kw):
     a = dict(q=FAKE, k=FAKE, lse=FAKE, w_in=None, w_out=FAKE, B=1, NH=4, NKV=2, T=8, D=64, q_sb=2048, q_st=256, q_sh=64,
-             k_sb=1024, k_st=128, k_sh=64, w_sb=16, w_sh=8, first=0, lengths=None, scale=0.125, dtype=0, stream=None)
+             k_sb=1024, k_st=128, k_sh=64, w_sb=16, w_sh=8, first=0, lengths=None, scale=0.125, dtype=0, ws=FAKE, ws_bytes=1 << 30, stream=None)
     a.update(kw)
     return _lib().attn_key_weights(*a.values())
 
@@ -88,7 +88,7 @@ def test_bad_caches_are_refused(call, bad, code, text):
     (_decode, dict(ws=FAKE + 4), ARG, "aligned"),
     (_weights, dict(q=None), ARG, "null"), (_weights, dict(w_out=None), ARG, "null"), (_weights, dict(dtype=5), ARG, "dtype"),
     (_weights, dict(NH=3), ARG, "multiple"), (_weights, dict(first=-1), ARG, "first_query"), (_weights, dict(T=0), ARG, "positive"),
-    (_weights, dict(D=160), UNSUPPORTED, "head_dim"), (_weights, dict(k_st=-1), ARG, "negative"),
+    (_weights, dict(D=160), UNSUPPORTED, "head_dim"), (_weights, dict(T=256, ws_bytes=4), WORKSPACE, "workspace"), (_weights, dict(k_st=-1), ARG, "negative"),
     (_evict, dict(weights=None), ARG, "null"), (_evict, dict(slots=None), ARG, "null"), (_evict, dict(L=17), ARG, "length"),
     (_evict, dict(L=0), ARG, "length"), (_evict, dict(keep=0), ARG, "keep"), (_evict, dict(keep=17), ARG, "keep"),
     (_evict, dict(recent=5), ARG, "recent"), (_evict, dict(recent=-1), ARG, "recent"), (_evict, dict(ws=None), WORKSPACE, "workspace"),
