@@ -113,9 +113,23 @@ struct KwMaps {
   TileMap q, k;
 };
 
+// n / d for 0 <= n < 2^31 as a multiplication by m = ceil(2^(31 + k) / d), k = ceil(log2 d): n m / 2^(31 + k)
+// exceeds n / d by less than n / 2^31 / d < 1 / d.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __host__ void set(uint32_t divisor) {
+    d = divisor;
+    shift = 0;
+    while ((1u << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> (31 + shift)); }
+};
+
 struct KwTc {
   KeyWeights p;
   int nt, parts, BK, units;  // key tiles, parts of a key tile's queries, B*NKV
+  FastDiv by_bk, by_nkv, by_parts;
   float* partial;            // [parts][B*NKV][T] when parts > 1
   int* err;
 };
@@ -125,24 +139,91 @@ struct KwBars {
   uint32_t tmem;
 };
 
-// One unit of work: key tile jt of (b, kvh), query tiles [lo, nt) of each of the G query heads in turn,
-// of which this part takes the steps [begin, end).
+// One unit of work: key tile jt of (b, kvh), query tiles [lo, lo + span) of each of the G query heads in
+// turn, of which this part takes the steps [begin, end).  Units are ordered longest first (the first
+// key tiles) and dealt to the CTAs forth and back, which evens out their totals: 32 x 8 heads of 8 tiles
+// come to 30 .. 33 tiles a CTA, dealt round and round to 27 .. 35.
 struct KwUnit {
   int b, kvh, jt, part, n, lo, span, begin, end;
-  __device__ __forceinline__ void set(const KwTc& a, int u) {
-    const int bk = u % a.BK, level = u / a.BK;  // the longest key tiles (the first) come first
-    part = level % a.parts;
-    jt = level / a.parts;
-    b = bk / a.p.NKV;
+  __device__ __forceinline__ bool set(const KwTc& a, int round) {
+    const int u = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if (u >= a.units) {
+      begin = end = 0;
+      return false;
+    }
+    const uint32_t level = a.by_bk.div(u), bk = u - level * a.BK;
+    jt = a.by_parts.div(level);
+    part = level - jt * a.parts;
+    b = a.by_nkv.div(bk);
     kvh = bk - b * a.p.NKV;
     n = seq_length(a.p.lengths, b, a.p.T);
     lo = max(jt, a.p.first / AT_TILE);
     span = max((n + AT_TILE - 1) / AT_TILE - lo, 0);
     const int total = span * a.p.G;
-    begin = (int)((int64_t)total * part / a.parts);
-    end = (int)((int64_t)total * (part + 1) / a.parts);
+    begin = 0;
+    end = total;
+    if (a.parts > 1) {
+      begin = (int)((int64_t)total * part / a.parts);
+      end = (int)((int64_t)total * (part + 1) / a.parts);
+    }
+    return true;
   }
 };
+
+// The query tiles of a unit in order: query head g of the key head, tile it.
+struct KwSteps {
+  int g, it;
+  __device__ __forceinline__ void start(const KwUnit& w) {
+    g = w.begin ? w.begin / max(w.span, 1) : 0;
+    it = w.lo + w.begin - g * w.span;
+  }
+  __device__ __forceinline__ void next(const KwUnit& w) {
+    if (++it == w.lo + w.span) {
+      it = w.lo;
+      ++g;
+    }
+  }
+};
+
+// All query tiles of a CTA's units in order.
+struct KwTiles {
+  KwUnit w;
+  KwSteps st;
+  int i, round;
+  bool more;
+  __device__ __forceinline__ void open(const KwTc& a) {  // the first tile of the next unit that has one
+    do more = w.set(a, round++);
+    while (more && w.begin >= w.end);
+    i = w.begin;
+    if (more) st.start(w);
+  }
+  __device__ __forceinline__ void start(const KwTc& a) {
+    round = 0;
+    open(a);
+  }
+  __device__ __forceinline__ void next(const KwTc& a) {
+    st.next(w);
+    if (++i == w.end) open(a);
+  }
+};
+
+// Two float32 in one register pair: sm_100's packed multiply-add and addition halve the issue slots.
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ void add2(uint64_t& a, uint64_t b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(b));
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+  return pair(__float_as_uint(ex2_approx(__uint_as_float((uint32_t)x))),
+              __float_as_uint(ex2_approx(__uint_as_float((uint32_t)(x >> 32)))));
+}
+__device__ __forceinline__ float pair_sum(uint64_t x) {
+  return __uint_as_float((uint32_t)x) + __uint_as_float((uint32_t)(x >> 32));
+}
 
 // Wait for a load that is known to be in flight, after a wait elsewhere gave up: at most 0.1 s.
 __device__ __forceinline__ void drain_load(uint64_t* bar, uint32_t parity) {
@@ -191,21 +272,22 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwTc a) {
     if (lane == 0) {
       int ku = 0, qn = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-        KwUnit w;
-        w.set(a, u);
+      KwUnit w;
+      for (int round = 0; ok && w.set(a, round); ++round) {
         if (w.begin >= w.end) continue;
         const int ks = ku & 1;
         if (!mbar_wait(&bars->k_empty[ks], ((ku >> 1) & 1) ^ 1, werr, 501)) { ok = false; break; }
         mbar_arrive_expect_tx(&bars->k_full[ks], AT_TILE_BYTES);
         load_tile(sK + ks * AT_TILE_BYTES, maps.k, &bars->k_full[ks], w.b, w.kvh, w.jt * AT_TILE);
         ++ku;
-        for (int i = w.begin; i < w.end; ++i, ++qn) {
+        KwSteps st;
+        st.start(w);
+        for (int i = w.begin; i < w.end; ++i, ++qn, st.next(w)) {
           const int qs = qn % KT_STAGES;
           if (!mbar_wait(&bars->q_empty[qs], ((qn / KT_STAGES) & 1) ^ 1, werr, 502)) { ok = false; break; }
           mbar_arrive_expect_tx(&bars->q_full[qs], AT_TILE_BYTES);
-          load_tile(sQ + qs * AT_TILE_BYTES, maps.q, &bars->q_full[qs], w.b, w.kvh * a.p.G + i / w.span,
-                    (w.lo + i % w.span) * AT_TILE);
+          load_tile(sQ + qs * AT_TILE_BYTES, maps.q, &bars->q_full[qs], w.b, w.kvh * a.p.G + st.g,
+                    st.it * AT_TILE);
         }
       }
       if (!ok) {  // leave no load of this CTA's behind
@@ -219,17 +301,17 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwTc a) {
       const uint32_t idesc = TF32 ? idesc_tf32_f32(128, 128, 0, 0) : idesc_bf16_f32(128, 128, 0, 0);
       int ku = 0, qn = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-        KwUnit w;
-        w.set(a, u);
+      KwUnit w;
+      for (int round = 0; ok && w.set(a, round); ++round) {
         if (w.begin >= w.end) continue;
         const int ks = ku & 1;
         if (!mbar_wait(&bars->k_full[ks], (ku >> 1) & 1, werr, 503)) break;
         const uint64_t k_desc = smem_desc_sw128(smem_u32(sK + ks * AT_TILE_BYTES), 16, 1024);
-        for (int i = w.begin; i < w.end; ++i, ++qn) {
-          const int qs = qn % KT_STAGES, buf = qn & 1;
-          if (!mbar_wait(&bars->q_full[qs], (qn / KT_STAGES) & 1, werr, 504) ||
-              !mbar_wait(&bars->s_free[buf], ((qn >> 1) & 1) ^ 1, werr, 505)) { ok = false; break; }
+        const int last = qn + w.end - w.begin;
+        for (int t = qn; t < last; ++t) {
+          const int qs = t % KT_STAGES, buf = t & 1;
+          if (!mbar_wait(&bars->q_full[qs], (t / KT_STAGES) & 1, werr, 504) ||
+              !mbar_wait(&bars->s_free[buf], ((t >> 1) & 1) ^ 1, werr, 505)) { ok = false; break; }
           tc_fence_after();
           const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ + qs * AT_TILE_BYTES), 16, 1024);
 #pragma unroll
@@ -241,94 +323,99 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwTc a) {
           }
           umma_commit(&bars->s_full[buf]);
           umma_commit(&bars->q_empty[qs]);
-          if (i + 1 == w.end) umma_commit(&bars->k_empty[ks]);
         }
+        if (ok) umma_commit(&bars->k_empty[ks]);
+        qn = last;
         ++ku;
       }
     }
   } else {
     // ---------------- sums: thread = key ----------------
+    // The four 32-column chunks of every tile go through two register buffers: while one is summed the
+    // next is on its way from TMEM, across tiles and units too (the next tile's scores are waited for, and
+    // its first chunk asked for, before this tile's last chunk is summed).
     float* sl = sL + warp * 2 * AT_TILE;
     const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16);
-    const float c = a.p.scale_log2;
-    int qn = 0;
+    const uint64_t cpair = pair(__float_as_uint(a.p.scale_log2), __float_as_uint(a.p.scale_log2));
+    const int row = warp * 32 + lane;
     bool ok = true;
-    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
-      KwUnit w;
-      w.set(a, u);
-      const int row = warp * 32 + lane, j = w.jt * AT_TILE + row;
+    KwTiles ahead;          // the tile whose lse is in `next`
+    float next[4];
+    ahead.start(a);
+    auto fetch = [&]() {
+      if (!ahead.more) return;
+      const int i0 = ahead.st.it * AT_TILE + lane;
+      const float* src = a.p.lse + ((int64_t)ahead.w.b * a.p.NH + ahead.w.kvh * a.p.G + ahead.st.g) * a.p.T + i0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) next[k] = i0 + k * 32 < ahead.w.n ? src[k * 32] : 0.f;
+    };
+    fetch();
+    int qn = 0;             // tiles summed
+    uint32_t sr[2][32];
+    // tile qn: -lse in log2 units for this warp, its scores complete, its first chunk on its way
+    auto prime = [&](int t) -> bool {
+      float* lb = sl + (t & 1) * AT_TILE;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) lb[k * 32 + lane] = next[k] * -LOG2E;
+      ahead.next(a);
+      fetch();
+      const bool full = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t & 1], (t >> 1) & 1, werr, 506));
+      __syncwarp();  // lb is written
+      tc_fence_after();
+      tmem_ld32(tS + (t & 1) * 128, sr[0]);
+      return full;
+    };
+    if (ahead.more) ok = prime(0);
+    KwUnit w;
+    for (int round = 0; ok && w.set(a, round); ++round) {
+      const int j = w.jt * AT_TILE + row;
+      const int64_t at = w.b * a.p.w_sb + w.kvh * a.p.w_sh + j;
+      const float have = a.parts == 1 && a.p.w_in && j < a.p.T ? a.p.w_in[at] : 0.f;
       float total = 0.f;
-      // -lse in log2 units of the next tile's queries, four per lane, fetched a tile ahead
-      float next[4];
-      auto fetch = [&](int i) {
-        const int h = w.kvh * a.p.G + i / w.span, i0 = (w.lo + i % w.span) * AT_TILE;
-        const float* src = a.p.lse + ((int64_t)w.b * a.p.NH + h) * a.p.T + i0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) next[k] = i0 + k * 32 + lane < w.n ? src[k * 32 + lane] * -LOG2E : 0.f;
-      };
-      if (w.begin < w.end) fetch(w.begin);
-      for (int i = w.begin; i < w.end; ++i, ++qn) {
-        const int buf = qn & 1, i0 = (w.lo + i % w.span) * AT_TILE;
-        float* lb = sl + buf * AT_TILE;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) lb[k * 32 + lane] = next[k];
-        __syncwarp();
-        if (i + 1 < w.end) fetch(i + 1);
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[buf], (qn >> 1) & 1, werr, 506))) { ok = false; break; }
-        tc_fence_after();
-        // columns of this tile that count for this key: queries from max(j, first) to n - 1
+      KwSteps st;
+      st.start(w);
+      for (int i = w.begin; i < w.end; ++i, ++qn, st.next(w)) {
+        const int buf = qn & 1, i0 = st.it * AT_TILE;
+        const float* lb = sl + buf * AT_TILE;
+        // columns that count for this key: queries from max(j, first) to n - 1; the warp's bounds
         const int c0 = max(j, a.p.first) - i0, c1 = w.n - i0;
-        const bool whole = i0 >= w.jt * AT_TILE + AT_TILE && i0 >= a.p.first && c1 >= AT_TILE;
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        const int c0_any = max(j - lane, a.p.first) - i0, c0_all = max(j - lane + 31, a.p.first) - i0;
+        uint64_t sum[2] = {0, 0};  // four running sums of the tile as two packed pairs
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
-          uint32_t sr[32];
-          tmem_ld32(tS + buf * 128 + cc * 32, sr);
           tmem_wait_ld();
-          if (cc == 3) {  // the scores are in registers
+          if (cc < 3) {
+            tmem_ld32(tS + buf * 128 + (cc + 1) * 32, sr[(cc + 1) & 1]);
+          } else {  // the scores are in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->s_free[buf]);
+            if (ahead.more) ok = prime(qn + 1);
           }
-          const float4* l4 = reinterpret_cast<const float4*>(lb + cc * 32);
-          if (whole) {
+          uint32_t(&x)[32] = sr[cc & 1];
+          if (cc * 32 + 32 <= c0_any) continue;  // before every lane's first query
+          if (cc * 32 < c0_all || cc * 32 + 32 > c1) {
+            // unused scores may be anything, NaN too: they are replaced, not multiplied
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 l = l4[k];
-              s0 += ex2_approx(fmaf(__uint_as_float(sr[4 * k]), c, l.x));
-              s1 += ex2_approx(fmaf(__uint_as_float(sr[4 * k + 1]), c, l.y));
-              s2 += ex2_approx(fmaf(__uint_as_float(sr[4 * k + 2]), c, l.z));
-              s3 += ex2_approx(fmaf(__uint_as_float(sr[4 * k + 3]), c, l.w));
-            }
-          } else if (cc * 32 + 31 >= __reduce_min_sync(0xffffffffu, c0)) {
-            // (a chunk before every lane's first query is skipped.)  Unused scores may be anything, NaN
-            // too: they are replaced, not multiplied
+            for (int k = 0; k < 32; ++k)
+              if (k < c0 - cc * 32 || k >= c1 - cc * 32) x[k] = 0xff800000u;  // -inf, its exponential 0
+          }
+          const ulonglong2* l2 = reinterpret_cast<const ulonglong2*>(lb + cc * 32);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 l = l4[k];
-              const int col = cc * 32 + 4 * k;
-              const float e0 = ex2_approx(fmaf(__uint_as_float(sr[4 * k]), c, l.x));
-              const float e1 = ex2_approx(fmaf(__uint_as_float(sr[4 * k + 1]), c, l.y));
-              const float e2 = ex2_approx(fmaf(__uint_as_float(sr[4 * k + 2]), c, l.z));
-              const float e3 = ex2_approx(fmaf(__uint_as_float(sr[4 * k + 3]), c, l.w));
-              s0 += col >= c0 && col < c1 ? e0 : 0.f;
-              s1 += col + 1 >= c0 && col + 1 < c1 ? e1 : 0.f;
-              s2 += col + 2 >= c0 && col + 2 < c1 ? e2 : 0.f;
-              s3 += col + 3 >= c0 && col + 3 < c1 ? e3 : 0.f;
-            }
+          for (int k = 0; k < 8; ++k) {
+            const ulonglong2 l = l2[k];
+            add2(sum[0], ex2_pair(fma2(pair(x[4 * k], x[4 * k + 1]), cpair, l.x)));
+            add2(sum[1], ex2_pair(fma2(pair(x[4 * k + 2], x[4 * k + 3]), cpair, l.y)));
           }
         }
-        total += (s0 + s1) + (s2 + s3);
+        total += pair_sum(sum[0]) + pair_sum(sum[1]);
+        if (!ok) break;
       }
       if (!ok) break;
       if (j < a.p.T) {
         const float sum = j < w.n ? total : 0.f;
-        if (a.parts > 1) {
-          a.partial[((int64_t)w.part * a.BK + (int64_t)w.b * a.p.NKV + w.kvh) * a.p.T + j] = sum;
-        } else {
-          const int64_t at = w.b * a.p.w_sb + w.kvh * a.p.w_sh + j;
-          a.p.w_out[at] = (a.p.w_in ? a.p.w_in[at] : 0.f) + sum;
-        }
+        if (a.parts > 1) a.partial[((int64_t)w.part * a.BK + (int64_t)w.b * a.p.NKV + w.kvh) * a.p.T + j] = sum;
+        else a.p.w_out[at] = have + sum;
       }
     }
   }
@@ -390,6 +477,9 @@ static int key_weights_tc(const KeyWeights& p, int B, int tf32, float* partial, 
   const int64_t units = (int64_t)a.BK * a.nt * a.parts;
   a.units = (int)units;
   a.partial = partial;
+  a.by_bk.set(a.BK);
+  a.by_nkv.set(p.NKV);
+  a.by_parts.set(a.parts);
   a.err = dev_error_ptr();
   if (!a.err) return ATTN_ERR_CUDA;
   const int64_t ctas = 2 * (int64_t)current_device_sms();
