@@ -113,19 +113,6 @@ struct KwMaps {
   TileMap q, k;
 };
 
-// n / d for 0 <= n < 2^31 as a multiplication by m = ceil(2^(31 + k) / d), k = ceil(log2 d): n m / 2^(31 + k)
-// exceeds n / d by less than n / 2^31 / d < 1 / d.
-struct FastDiv {
-  uint32_t d, mul, shift;
-  __host__ void set(uint32_t divisor) {
-    d = divisor;
-    shift = 0;
-    while ((1u << shift) < d) ++shift;
-    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> (31 + shift)); }
-};
-
 struct KwTc {
   KeyWeights p;
   int nt, parts, BK, units;  // key tiles, parts of a key tile's queries, B*NKV

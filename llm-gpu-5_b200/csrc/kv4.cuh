@@ -42,12 +42,24 @@ __device__ __forceinline__ int seq_length(const int* lengths, int b, int most) {
   return lengths ? min(max(lengths[b], 0), most) : most;
 }
 
+// n / d for 0 <= n < 2^31 as a multiplication by m = ceil(2^(31 + k) / d), k = ceil(log2 d): n m / 2^(31 + k)
+// exceeds n / d by less than n / 2^31 / d < 1 / d.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __host__ void set(uint32_t divisor) {
+    d = divisor;
+    shift = 0;
+    while ((1u << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> (31 + shift)); }
+};
+
 // The code of x in a group (s, m): the n in 0..15 nearest to (x - m) / s, ties to even, decided in
 // exact arithmetic.  x - m is split into its float32 rounding d and the rounding's error e (Knuth's
 // two-sum), and the borders (n +- 1/2) s are exact in float32 (5 + 11 bits); a division can only
 // place a value near a border on the wrong side of it, which the comparisons put right.
-__device__ __forceinline__ uint32_t kv4_code(float x, float s, float m, float inv) {
-  if (!(s > 0.f)) return 0;
+static __device__ __noinline__ uint32_t kv4_code_exact(float x, float s, float m, float inv) {
   const float d = __fsub_rn(x, m);
   const float bb = __fsub_rn(d, x);
   const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(d, bb)), -__fadd_rn(m, bb));
@@ -57,6 +69,28 @@ __device__ __forceinline__ uint32_t kv4_code(float x, float s, float m, float in
   if (d > hi || (d == hi && (e > 0.f || (e == 0.f && odd)))) n += 1.f;
   else if (d < lo || (d == lo && (e < 0.f || (e == 0.f && odd)))) n -= 1.f;
   return (uint32_t)fminf(fmaxf(n, 0.f), 15.f);
+}
+
+// The codes of eight values as one word.  t = (x - m) * (1 / s) in float32 is within 3 * 2^-24 * 15.5 <
+// 3e-6 of the exact quotient (clamped to 0..15, which decides alike), so its nearest integer is the code
+// unless t lies within 1e-5 of a border; then the word is formed again exactly.
+__device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], float s, float m, float inv) {
+  constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits, half to even
+  uint32_t w = 0;
+  float far = 0.f;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], m), inv), 0.f), 15.f);
+    const float r = __fadd_rn(t, MAGIC);
+    far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(r, MAGIC))));
+    w = w << 4 | (__float_as_uint(r) & 15u);
+  }
+  if (far > 0.49999f) {
+    w = 0;
+#pragma unroll 1
+    for (int i = 7; i >= 0; --i) w = w << 4 | kv4_code_exact(x[i], s, m, inv);
+  }
+  return s > 0.f ? w : 0u;
 }
 
 }  // namespace attn

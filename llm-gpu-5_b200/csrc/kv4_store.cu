@@ -6,9 +6,10 @@
 // prompt's store and launch latency a single token's.
 //
 // A row is taken by D / 8 lanes of 8 values each (16 bytes of bf16 per lane); a group's minimum and
-// maximum come from shuffles among its 2, 4 or 8 lanes.  Rows are walked with the position fastest, so
-// that a warp's codes (and scale pairs) of consecutive positions are one contiguous write while its
-// reads are whole rows of the token layout.
+// maximum come from shuffles among its 2, 4 or 8 lanes.  Rows are walked in runs of up to 32 positions of
+// one head, all heads of those positions in turn: a warp's codes (and scale pairs) of consecutive
+// positions are one contiguous write, its reads whole rows of the token layout, and the heads that share
+// a token's DRAM page are read at about the same time.
 #include "kv4.cuh"
 #include <math.h>
 
@@ -34,7 +35,31 @@ int kv4_check(const char* fn, const Kv4View& c, int B, int NH, int D) {
 struct Kv4Rows {
   const void *k, *v;
   int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
-  uint32_t T, NH, rows;  // rows = B * NH * T
+  uint32_t T, NH;
+  uint32_t rows, run;  // row = ((b * runs + position / run) * NH + h) * run + position % run; rows with padding
+  FastDiv by_run, by_nh, by_runs;
+};
+
+// Positions per run, and the number of rows with the last run of every sequence filled up.
+static inline int64_t kv4_set_rows(Kv4Rows* r, int B) {
+  r->run = r->T < 32 ? r->T : 32;
+  const uint32_t runs = (r->T + r->run - 1) / r->run;
+  const int64_t rows = (int64_t)B * runs * r->NH * r->run;
+  r->rows = (uint32_t)rows;
+  r->by_run.set(r->run);
+  r->by_nh.set(r->NH);
+  r->by_runs.set(runs);
+  return rows;
+}
+
+struct Kv4Row {
+  uint32_t b, h, t;
+  __device__ __forceinline__ Kv4Row(const Kv4Rows& a, uint32_t row) {
+    const uint32_t q = a.by_run.div(row), u = a.by_nh.div(q);
+    h = q - u * a.NH;
+    b = a.by_runs.div(u);
+    t = (u - b * a.by_runs.d) * a.run + row - q * a.run;
+  }
 };
 
 struct Kv4Slots {
@@ -53,7 +78,15 @@ struct Kv4Marks {
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, float* x) {
-  if constexpr (VEC) {
+  if constexpr (VEC && sizeof(T) == 2) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else if constexpr (VEC) {
     const float4 a = load4(p), b = load4(p + 4);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
@@ -73,11 +106,10 @@ kv4_store_kernel(const Kv4Rows in, const Kv4View c, const Kv4Slots sl, const Kv4
   const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
   const int sub = threadIdx.x % LPR;
   const bool value = blockIdx.y != 0;
-  const uint32_t r = min(row, in.rows - 1);
-  const uint32_t bh = r / in.T, t = r - bh * in.T;
-  const uint32_t b = bh / in.NH, h = bh - b * in.NH;
+  const Kv4Row at(in, min(row, in.rows - 1));
+  const uint32_t b = at.b, h = at.h, t = at.t;
   const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
-  const bool put = row < in.rows && slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : in.T);
+  const bool put = row < in.rows && t < in.T && slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : in.T);
   float x[8];
   if (put) {
     const T* src = value ? (const T*)in.v + b * in.v_sb + t * in.v_st + h * in.v_sh
@@ -109,16 +141,14 @@ kv4_store_kernel(const Kv4Rows in, const Kv4View c, const Kv4Slots sl, const Kv4
   const __half m = __float2half_rn(fin ? fminf(fmaxf(lo, -65504.f), 65504.f) : NAN);
   const float sf = __half2float(s), mf = __half2float(m);
   const float inv = sf > 0.f ? __fdiv_rn(1.f, sf) : 0.f;
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w |= kv4_code(x[i], sf, mf, inv) << (4 * i);
+  const uint32_t w = kv4_word(x, sf, mf, inv);
   const int64_t dst = (value ? c.si : 0) + b * c.sb + h * c.sh + slot;
   *reinterpret_cast<uint32_t*>(c.codes + dst * (D / 2) + sub * 4) = w;
   if (sub % LPG == 0) c.params[dst * kv4_groups(D) + sub / LPG] = __halves2half2(s, m);
   if (!value && sub == 0) {
-    const int64_t at = b * mk.sb + h * mk.sh + slot;
-    if (mk.weights) mk.weights[at] = 0.f;
-    if (mk.positions) mk.positions[at] = (int)(seq_value(mk.seen, b, mk.seen0) + t);
+    const int64_t mark = b * mk.sb + h * mk.sh + slot;
+    if (mk.weights) mk.weights[mark] = 0.f;
+    if (mk.positions) mk.positions[mark] = (int)(seq_value(mk.seen, b, mk.seen0) + t);
   }
 }
 
@@ -133,8 +163,9 @@ kv4_load_kernel(const Kv4Rows out, const Kv4View c, const Kv4Slots sl) {
   if (row >= out.rows) return;
   const int sub = threadIdx.x % LPR;
   const bool value = blockIdx.y != 0;
-  const uint32_t bh = row / out.T, t = row - bh * out.T;
-  const uint32_t b = bh / out.NH, h = bh - b * out.NH;
+  const Kv4Row at(out, row);
+  const uint32_t b = at.b, h = at.h, t = at.t;
+  if (t >= out.T) return;
   const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
   float x[8];
 #pragma unroll
@@ -150,7 +181,15 @@ kv4_load_kernel(const Kv4Rows out, const Kv4View c, const Kv4Slots sl) {
   T* dst = value ? (T*)out.v + b * out.v_sb + t * out.v_st + h * out.v_sh
                  : (T*)out.k + b * out.k_sb + t * out.k_st + h * out.k_sh;
   dst += sub * 8;
-  if constexpr (VEC) {
+  if constexpr (VEC && sizeof(T) == 2) {
+    uint32_t w2[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w2[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+  } else if constexpr (VEC) {
     store4(dst, make_float4(x[0], x[1], x[2], x[3]));
     store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
   } else {
@@ -171,9 +210,10 @@ static int kv4_rows_launch(const Kv4Rows& r, const Kv4View& c, const Kv4Slots& s
 
 template <typename T>
 static int kv4_rows_t(const Kv4Rows& r, int D, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
-  // vector accesses where every lane's first value is aligned for them (4 values: 8 bytes of bf16, 16 of float32)
-  const bool vec = aligned(r.k, 4 * sizeof(T)) && aligned(r.v, 4 * sizeof(T)) && r.k_sb % 4 == 0 && r.k_st % 4 == 0 &&
-                   r.k_sh % 4 == 0 && r.v_sb % 4 == 0 && r.v_st % 4 == 0 && r.v_sh % 4 == 0;
+  // 16-byte accesses where every lane's first value is aligned for them
+  constexpr int64_t V = 16 / sizeof(T);
+  const bool vec = aligned(r.k, 16) && aligned(r.v, 16) && r.k_sb % V == 0 && r.k_st % V == 0 && r.k_sh % V == 0 &&
+                   r.v_sb % V == 0 && r.v_st % V == 0 && r.v_sh % V == 0;
 #define KV4_ROWS(DD)                                                       \
   case DD:                                                                 \
     return vec ? kv4_rows_launch<T, DD, true>(r, c, sl, mk, s) : kv4_rows_launch<T, DD, false>(r, c, sl, mk, s);
@@ -182,7 +222,7 @@ static int kv4_rows_t(const Kv4Rows& r, int D, const Kv4View& c, const Kv4Slots&
   return ATTN_ERR_UNSUPPORTED;
 }
 
-static int kv4_rows(const char* fn, const Kv4Rows& r, int B, int D, int dtype, const Kv4View& c, const Kv4Slots& sl,
+static int kv4_rows(const char* fn, Kv4Rows r, int B, int D, int dtype, const Kv4View& c, const Kv4Slots& sl,
                     const Kv4Marks* mk, cudaStream_t s) {
   if (int rc = kv4_check(fn, c, B, (int)r.NH, D)) return rc;
   ATTN_REQUIRE(r.k && r.v, "%s: null pointer argument", fn);
@@ -192,6 +232,7 @@ static int kv4_rows(const char* fn, const Kv4Rows& r, int B, int D, int dtype, c
   for (int i = 0; i < 6; ++i) ATTN_REQUIRE(st[i] >= 0, "%s: strides must not be negative", fn);
   ATTN_REQUIRE(sl.starts || (sl.start >= 0 && (int64_t)sl.start + r.T <= c.cap),
                "%s: positions %d .. %lld exceed the capacity of %d", fn, sl.start, (long long)sl.start + r.T - 1, c.cap);
+  ATTN_REQUIRE(kv4_set_rows(&r, B) < (int64_t)1 << 31, "%s: B*NH*T must be below 2^31", fn);
   return dtype == ATTN_BF16 ? kv4_rows_t<__nv_bfloat16>(r, D, c, sl, mk, s) : kv4_rows_t<float>(r, D, c, sl, mk, s);
 }
 
@@ -208,7 +249,7 @@ extern "C" int attn_kv4_store(const void* k, const void* v, int dtype, int B, in
   ATTN_REQUIRE(B > 0 && T > 0 && NH > 0, "attn_kv4_store: sizes must be positive");
   ATTN_REQUIRE((int64_t)B * NH * T < (int64_t)1 << 31, "attn_kv4_store: B*NH*T must be below 2^31");
   ATTN_REQUIRE(!(weights || positions) || (w_sb >= 0 && w_sh >= 0), "attn_kv4_store: bad strides");
-  const Kv4Rows r = {k, v, k_sb, k_st, k_sh, v_sb, v_st, v_sh, (uint32_t)T, (uint32_t)NH, (uint32_t)(B * NH * T)};
+  const Kv4Rows r = {k, v, k_sb, k_st, k_sh, v_sb, v_st, v_sh, (uint32_t)T, (uint32_t)NH};
   const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
   ATTN_REQUIRE(c_si >= capacity && (B == 1 || c_sb >= capacity), "attn_kv4_store: cache rows must not overlap");
   const Kv4Marks mk = {weights, positions, w_sb, w_sh, seen, seen0};
@@ -221,7 +262,7 @@ extern "C" int attn_kv4_load(const void* codes, const void* params, int64_t c_si
   clear_error();
   ATTN_REQUIRE(B > 0 && T > 0 && NH > 0, "attn_kv4_load: sizes must be positive");
   ATTN_REQUIRE((int64_t)B * NH * T < (int64_t)1 << 31, "attn_kv4_load: B*NH*T must be below 2^31");
-  const Kv4Rows r = {k, v, o_sb, o_st, o_sh, o_sb, o_st, o_sh, (uint32_t)T, (uint32_t)NH, (uint32_t)(B * NH * T)};
+  const Kv4Rows r = {k, v, o_sb, o_st, o_sh, o_sb, o_st, o_sh, (uint32_t)T, (uint32_t)NH};
   const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
   return kv4_rows("attn_kv4_load", r, B, D, dtype, c, Kv4Slots{starts, start, counts}, nullptr, as_stream(stream));
 }

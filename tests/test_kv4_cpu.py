@@ -135,7 +135,7 @@ def test_cache_class_refuses_bad_sizes():
 
 
 def _code(x, s, m):
-    """kv4_code's float32 steps (csrc/kv4.cuh), in NumPy."""
+    """kv4_code_exact's float32 steps (csrc/kv4.cuh), in NumPy."""
     f = np.float32
     d = f(x - m)
     bb = f(d - x)
@@ -165,4 +165,9 @@ def test_code_steps_decide_exactly():
                 want = min(max(round(t), 0), 15)  # Fraction's round: half to even
                 assert _code(x, s, m) == want, (x, s, m, n)
                 checked += 1
+                # the quick way round is only taken where it decides alike
+                f = np.float32
+                q = f(min(max(f(f(x - m) * f(f(1) / s)), f(0)), f(15)))
+                if abs(f(q - np.rint(q))) <= f(0.49999):
+                    assert int(np.rint(q)) == want, (x, s, m, n)
     assert checked == 300 * 45
