@@ -71,26 +71,46 @@ static __device__ __noinline__ uint32_t kv4_code_exact(float x, float s, float m
   return (uint32_t)fminf(fmaxf(n, 0.f), 15.f);
 }
 
-// The codes of eight values as one word.  t = (x - m) * (1 / s) in float32 is within 3 * 2^-24 * 15.5 <
-// 3e-6 of the exact quotient (clamped to 0..15, which decides alike), so its nearest integer is the code
-// unless t lies within 1e-5 of a border; then the word is formed again exactly.
+// The codes of eight values as one word, inv = 1 / s to 2^-22.  t = 15 sat((x - m) inv / 15) + 0 in float32 is
+// within 15 * 5 * 2^-24 < 5e-6 of the exact quotient clamped to 0..15 (which decides alike), so its nearest
+// integer is the code unless t lies within 1e-5 of a border; then the word is formed again exactly.
+// The saturation, the rounding (adding 1.5 * 2^23 leaves the integer in the low bits) and the packing
+// (w * 16 + bits, the constant part taken off at the end) all run on the multiply-add pipe.
 __device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], float s, float m, float inv) {
-  constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits, half to even
+  constexpr float MAGIC = 12582912.f;
+  constexpr uint32_t MAGIC_BITS = 0x4b400000u;
+  const float inv15 = __fmul_rn(inv, 1.f / 15.f);
   uint32_t w = 0;
   float far = 0.f;
 #pragma unroll
   for (int i = 7; i >= 0; --i) {
-    const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], m), inv), 0.f), 15.f);
-    const float r = __fadd_rn(t, MAGIC);
-    far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(r, MAGIC))));
-    w = w << 4 | (__float_as_uint(r) & 15u);
+    const float t = __saturatef(__fmul_rn(__fsub_rn(x[i], m), inv15));
+    const float r = __fmaf_rn(t, 15.f, MAGIC);
+    far = fmaxf(far, fabsf(__fmaf_rn(t, 15.f, -__fsub_rn(r, MAGIC))));
+    w = w * 16u + __float_as_uint(r);
   }
+  w -= (uint32_t)(MAGIC_BITS * 0x11111111ull);
   if (far > 0.49999f) {
     w = 0;
 #pragma unroll 1
     for (int i = 7; i >= 0; --i) w = w << 4 | kv4_code_exact(x[i], s, m, inv);
   }
   return s > 0.f ? w : 0u;
+}
+
+// The numbers n s + m of a word's eight codes, each rounded once (n s is exact: 4 + 11 bits).  A code
+// is made a float32 where it stands: its bits in the mantissa of 2^23, which is then taken off; that leaves
+// n * 16^k, and s * 16^-k is exact.
+__device__ __forceinline__ void kv4_values(uint32_t w, float s, float m, float (&x)[8]) {
+  constexpr float BIG = 8388608.f;
+  float sk = s;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t mask = 15u << (4 * k);
+    x[k] = __fmaf_rn(__uint_as_float((w & mask) | 0x4b000000u) - BIG, sk, m);
+    x[k + 4] = __fmaf_rn(__uint_as_float(((w >> 16) & mask) | 0x4b000000u) - BIG, sk, m);
+    sk *= 0.0625f;
+  }
 }
 
 }  // namespace attn

@@ -9,7 +9,8 @@
 // maximum come from shuffles among its 2, 4 or 8 lanes.  Rows are walked in runs of up to 32 positions of
 // one head, all heads of those positions in turn: a warp's codes (and scale pairs) of consecutive
 // positions are one contiguous write, its reads whole rows of the token layout, and the heads that share
-// a token's DRAM page are read at about the same time.
+// a token's DRAM page are read at about the same time.  A thread takes the key and the value of its
+// place, so that the index arithmetic, as long as the quantisation itself, is shared by 16 values.
 #include "kv4.cuh"
 #include <math.h>
 
@@ -76,8 +77,9 @@ struct Kv4Marks {
   int seen0;
 };
 
+// Eight values, and their smallest and largest.  hi is +infinity where one of them is not finite.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float* x) {
+__device__ __forceinline__ void load8(const T* p, float (&x)[8], float& lo, float& hi) {
   if constexpr (VEC && sizeof(T) == 2) {
     const uint4 u = *reinterpret_cast<const uint4*>(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -86,14 +88,31 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
       x[2 * i] = __uint_as_float(w[i] << 16);
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-  } else if constexpr (VEC) {
-    const float4 a = load4(p), b = load4(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);  // two at a time
+    const __nv_bfloat162 mn = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+    const __nv_bfloat162 mx = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    lo = fminf(__low2float(mn), __high2float(mn));
+    hi = fmaxf(__low2float(mx), __high2float(mx));
   } else {
+    if constexpr (VEC) {
+      const float4 a = load4(p), b = load4(p + 4);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::load(p + i);
+      for (int i = 0; i < 8; ++i) x[i] = Elem<T>::load(p + i);
+    }
+    lo = hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+    }
   }
+  float zero = 0.f;  // stays 0 while everything is finite
+#pragma unroll
+  for (int i = 0; i < 8; ++i) zero = __fmaf_rn(x[i], 0.f, zero);
+  if (!(zero == 0.f)) hi = INFINITY;
 }
 
 template <typename T, int D, bool VEC>
@@ -105,47 +124,40 @@ kv4_store_kernel(const Kv4Rows in, const Kv4View c, const Kv4Slots sl, const Kv4
   grid_dependents_launch();
   const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
   const int sub = threadIdx.x % LPR;
-  const bool value = blockIdx.y != 0;
   const Kv4Row at(in, min(row, in.rows - 1));
   const uint32_t b = at.b, h = at.h, t = at.t;
   const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
   const bool put = row < in.rows && t < in.T && slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : in.T);
-  float x[8];
+  const int64_t dst0 = b * c.sb + h * c.sh + slot;
+  float x[2][8], lo[2] = {0.f, 0.f}, hi[2] = {0.f, 0.f};
   if (put) {
-    const T* src = value ? (const T*)in.v + b * in.v_sb + t * in.v_st + h * in.v_sh
-                         : (const T*)in.k + b * in.k_sb + t * in.k_st + h * in.k_sh;
-    load8<T, VEC>(src + sub * 8, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    load8<T, VEC>((const T*)in.k + b * in.k_sb + t * in.k_st + h * in.k_sh + sub * 8, x[0], lo[0], hi[0]);
+    load8<T, VEC>((const T*)in.v + b * in.v_sb + t * in.v_st + h * in.v_sh + sub * 8, x[1], lo[1], hi[1]);
   }
-  float lo = x[0], hi = x[0];
-  bool finite = true;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) <= 3.4028234664e38f;
-  }
-  int fin = finite;
+  for (int off = LPG / 2; off > 0; off >>= 1)
 #pragma unroll
-  for (int off = LPG / 2; off > 0; off >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    fin &= __shfl_xor_sync(0xffffffffu, fin, off);
-  }
+    for (int i = 0; i < 2; ++i) {
+      lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], off));
+      hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], off));
+    }
   if (!put) return;
-  // scale and minimum saturate at float16's largest value; a group holding an infinity or a NaN reads
-  // back as NaN
-  const __half s = __float2half_rn(fin ? fminf(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), 65504.f) : NAN);
-  const __half m = __float2half_rn(fin ? fminf(fmaxf(lo, -65504.f), 65504.f) : NAN);
-  const float sf = __half2float(s), mf = __half2float(m);
-  const float inv = sf > 0.f ? __fdiv_rn(1.f, sf) : 0.f;
-  const uint32_t w = kv4_word(x, sf, mf, inv);
-  const int64_t dst = (value ? c.si : 0) + b * c.sb + h * c.sh + slot;
-  *reinterpret_cast<uint32_t*>(c.codes + dst * (D / 2) + sub * 4) = w;
-  if (sub % LPG == 0) c.params[dst * kv4_groups(D) + sub / LPG] = __halves2half2(s, m);
-  if (!value && sub == 0) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // scale and minimum saturate at float16's largest value; a group holding an infinity or a NaN reads
+    // back as NaN
+    const bool fin = hi[i] < INFINITY;
+    const __half s = __float2half_rn(fin ? fminf(__fmul_rn(__fsub_rn(hi[i], lo[i]), 1.f / 15.f), 65504.f) : NAN);
+    const __half m = __float2half_rn(fin ? fminf(fmaxf(lo[i], -65504.f), 65504.f) : NAN);
+    const float sf = __half2float(s);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));  // (unused where s is 0 or NaN)
+    const uint32_t w = kv4_word(x[i], sf, __half2float(m), inv);
+    const int64_t dst = dst0 + i * c.si;
+    *reinterpret_cast<uint32_t*>(c.codes + dst * (D / 2) + sub * 4) = w;
+    if (sub % LPG == 0) c.params[dst * kv4_groups(D) + sub / LPG] = __halves2half2(s, m);
+  }
+  if (sub == 0 && (mk.weights || mk.positions)) {
     const int64_t mark = b * mk.sb + h * mk.sh + slot;
     if (mk.weights) mk.weights[mark] = 0.f;
     if (mk.positions) mk.positions[mark] = (int)(seq_value(mk.seen, b, mk.seen0) + t);
@@ -162,46 +174,47 @@ kv4_load_kernel(const Kv4Rows out, const Kv4View c, const Kv4Slots sl) {
   const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
   if (row >= out.rows) return;
   const int sub = threadIdx.x % LPR;
-  const bool value = blockIdx.y != 0;
   const Kv4Row at(out, row);
   const uint32_t b = at.b, h = at.h, t = at.t;
   if (t >= out.T) return;
   const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
-  float x[8];
+  const bool held = slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : out.T);
+  const int64_t src = b * c.sb + h * c.sh + slot, to = b * out.k_sb + t * out.k_st + h * out.k_sh + sub * 8;
+  uint32_t w[2] = {0, 0};
+  float2 p[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // reads as zeros
+  if (held)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : out.T)) {
-    const int64_t src = (value ? c.si : 0) + b * c.sb + h * c.sh + slot;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(c.codes + src * (D / 2) + sub * 4);
-    const float2 p = __half22float2(c.params[src * kv4_groups(D) + sub / LPG]);
-    // n*s is exact (4 + 11 bits), so the sum is rounded once
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w >> (4 * i)) & 15u), p.x, p.y);
-  }
-  T* dst = value ? (T*)out.v + b * out.v_sb + t * out.v_st + h * out.v_sh
-                 : (T*)out.k + b * out.k_sb + t * out.k_st + h * out.k_sh;
-  dst += sub * 8;
-  if constexpr (VEC && sizeof(T) == 2) {
-    uint32_t w2[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      w2[i] = *reinterpret_cast<const uint32_t*>(&v);
+    for (int i = 0; i < 2; ++i) {
+      w[i] = *reinterpret_cast<const uint32_t*>(c.codes + (src + i * c.si) * (D / 2) + sub * 4);
+      p[i] = __half22float2(c.params[(src + i * c.si) * kv4_groups(D) + sub / LPG]);
     }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
-  } else if constexpr (VEC) {
-    store4(dst, make_float4(x[0], x[1], x[2], x[3]));
-    store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) Elem<T>::store(dst + i, x[i]);
+  for (int i = 0; i < 2; ++i) {
+    float x[8];
+    kv4_values(w[i], p[i].x, p[i].y, x);
+    T* dst = (T*)(i ? out.v : out.k) + to;
+    if constexpr (VEC && sizeof(T) == 2) {
+      uint32_t w2[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+        w2[k] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+    } else if constexpr (VEC) {
+      store4(dst, make_float4(x[0], x[1], x[2], x[3]));
+      store4(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) Elem<T>::store(dst + k, x[k]);
+    }
   }
 }
 
 template <typename T, int D, bool VEC>
 static int kv4_rows_launch(const Kv4Rows& r, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
   constexpr uint32_t per = KV4_THREADS / (D / 8);
-  const dim3 grid((r.rows + per - 1) / per, 2);
+  const dim3 grid((r.rows + per - 1) / per);
   const cudaError_t e = mk ? launch_pdl(kv4_store_kernel<T, D, VEC>, grid, dim3(KV4_THREADS), 0, s, r, c, sl, *mk)
                            : launch_pdl(kv4_load_kernel<T, D, VEC>, grid, dim3(KV4_THREADS), 0, s, r, c, sl);
   count_launch();

@@ -167,7 +167,7 @@ def test_code_steps_decide_exactly():
                 checked += 1
                 # the quick way round is only taken where it decides alike
                 f = np.float32
-                q = f(min(max(f(f(x - m) * f(f(1) / s)), f(0)), f(15)))
+                q = f(min(max(f(f(x - m) * f(f(f(1) / s) * f(1 / 15))), f(0)), f(1))) * f(15)
                 if abs(f(q - np.rint(q))) <= f(0.49999):
                     assert int(np.rint(q)) == want, (x, s, m, n)
     assert checked == 300 * 45
