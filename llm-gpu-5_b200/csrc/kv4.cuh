@@ -59,7 +59,7 @@ struct FastDiv {
 // exact arithmetic.  x - m is split into its float32 rounding d and the rounding's error e (Knuth's
 // two-sum), and the borders (n +- 1/2) s are exact in float32 (5 + 11 bits); a division can only
 // place a value near a border on the wrong side of it, which the comparisons put right.
-static __device__ __noinline__ uint32_t kv4_code_exact(float x, float s, float m, float inv) {
+__device__ __forceinline__ uint32_t kv4_code_exact(float x, float s, float m, float inv) {
   const float d = __fsub_rn(x, m);
   const float bb = __fsub_rn(d, x);
   const float e = __fadd_rn(__fsub_rn(x, __fsub_rn(d, bb)), -__fadd_rn(m, bb));
@@ -73,7 +73,8 @@ static __device__ __noinline__ uint32_t kv4_code_exact(float x, float s, float m
 
 // The codes of eight values as one word, inv = 1 / s to 2^-22.  t = 15 sat((x - m) inv / 15) + 0 in float32 is
 // within 15 * 5 * 2^-24 < 5e-6 of the exact quotient clamped to 0..15 (which decides alike), so its nearest
-// integer is the code unless t lies within 1e-5 of a border; then the word is formed again exactly.
+// integer is the code unless t lies within 1e-5 of a border; such a value is decided again exactly
+// (bfloat16 values are so coarse that one in 1,250 lies on a border, and a third of the warps hold one).
 // The saturation, the rounding (adding 1.5 * 2^23 leaves the integer in the low bits) and the packing
 // (w * 16 + bits, the constant part taken off at the end) all run on the multiply-add pipe.
 __device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], float s, float m, float inv) {
@@ -82,18 +83,25 @@ __device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], float s, float
   const float inv15 = __fmul_rn(inv, 1.f / 15.f);
   uint32_t w = 0;
   float far = 0.f;
+  auto place = [&](float v, float& r) {  // distance from the nearest integer, which is left in r's low bits
+    const float t = __saturatef(__fmul_rn(__fsub_rn(v, m), inv15));
+    r = __fmaf_rn(t, 15.f, MAGIC);
+    return fabsf(__fmaf_rn(t, 15.f, -__fsub_rn(r, MAGIC)));
+  };
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float t = __saturatef(__fmul_rn(__fsub_rn(x[i], m), inv15));
-    const float r = __fmaf_rn(t, 15.f, MAGIC);
-    far = fmaxf(far, fabsf(__fmaf_rn(t, 15.f, -__fsub_rn(r, MAGIC))));
-    w = w * 16u + __float_as_uint(r);
+  for (int i = 7; i >= 0; i -= 2) {
+    float r0, r1;
+    const float f0 = place(x[i], r0), f1 = place(x[i - 1], r1);
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(far) : "f"(f0), "f"(f1));
+    w = (w * 16u + __float_as_uint(r0)) * 16u + __float_as_uint(r1);
   }
   w -= (uint32_t)(MAGIC_BITS * 0x11111111ull);
   if (far > 0.49999f) {
-    w = 0;
-#pragma unroll 1
-    for (int i = 7; i >= 0; --i) w = w << 4 | kv4_code_exact(x[i], s, m, inv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float r;
+      if (place(x[i], r) > 0.49999f) w = (w & ~(15u << (4 * i))) | kv4_code_exact(x[i], s, m, inv) << (4 * i);
+    }
   }
   return s > 0.f ? w : 0u;
 }

@@ -6,7 +6,7 @@
 // prompt's store and launch latency a single token's.
 //
 // A row is taken by D / 8 lanes of 8 values each (16 bytes of bf16 per lane); a group's minimum and
-// maximum come from shuffles among its 2, 4 or 8 lanes.  Rows are walked in runs of up to 32 positions of
+// maximum come from shuffles among its 2, 4 or 8 lanes.  Rows are walked in runs of up to a CTA's rows of
 // one head, all heads of those positions in turn: a warp's codes (and scale pairs) of consecutive
 // positions are one contiguous write, its reads whole rows of the token layout, and the heads that share
 // a token's DRAM page are read at about the same time.  A thread takes the key and the value of its
@@ -41,9 +41,10 @@ struct Kv4Rows {
   FastDiv by_run, by_nh, by_runs;
 };
 
-// Positions per run, and the number of rows with the last run of every sequence filled up.
-static inline int64_t kv4_set_rows(Kv4Rows* r, int B) {
-  r->run = r->T < 32 ? r->T : 32;
+// Positions per run (`most`: the rows of a CTA), and the number of rows with the last run of every
+// sequence filled up.
+static inline int64_t kv4_set_rows(Kv4Rows* r, int B, uint32_t most) {
+  r->run = r->T < most ? r->T : most;
   const uint32_t runs = (r->T + r->run - 1) / r->run;
   const int64_t rows = (int64_t)B * runs * r->NH * r->run;
   r->rows = (uint32_t)rows;
@@ -53,13 +54,29 @@ static inline int64_t kv4_set_rows(Kv4Rows* r, int B) {
   return rows;
 }
 
+// The row of a thread.  WHOLE: a CTA is one run, so all but the position is the same for its threads
+// and stays in uniform registers.
+template <int LPR, bool WHOLE>
 struct Kv4Row {
   uint32_t b, h, t;
-  __device__ __forceinline__ Kv4Row(const Kv4Rows& a, uint32_t row) {
-    const uint32_t q = a.by_run.div(row), u = a.by_nh.div(q);
+  bool in;
+  __device__ __forceinline__ explicit Kv4Row(const Kv4Rows& a) {
+    constexpr uint32_t PER = KV4_THREADS / LPR;
+    uint32_t q, place = threadIdx.x / LPR;
+    in = true;
+    if constexpr (WHOLE) {
+      q = blockIdx.x;
+    } else {
+      const uint32_t row = blockIdx.x * PER + place;
+      in = row < a.rows;
+      q = a.by_run.div(min(row, a.rows - 1));
+      place = min(row, a.rows - 1) - q * a.run;
+    }
+    const uint32_t u = a.by_nh.div(q);
     h = q - u * a.NH;
     b = a.by_runs.div(u);
-    t = (u - b * a.by_runs.d) * a.run + row - q * a.run;
+    t = (u - b * a.by_runs.d) * a.run + place;
+    in = in && t < a.T;
   }
 };
 
@@ -115,19 +132,18 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8], float& lo, floa
   if (!(zero == 0.f)) hi = INFINITY;
 }
 
-template <typename T, int D, bool VEC>
+template <typename T, int D, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_store_kernel(const Kv4Rows in, const Kv4View c, const Kv4Slots sl, const Kv4Marks mk) {
   constexpr int LPR = D / 8;             // lanes per row
   constexpr int LPG = kv4_group(D) / 8;  // lanes per group
   grid_dependency_wait();
   grid_dependents_launch();
-  const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
   const int sub = threadIdx.x % LPR;
-  const Kv4Row at(in, min(row, in.rows - 1));
+  const Kv4Row<LPR, WHOLE> at(in);
   const uint32_t b = at.b, h = at.h, t = at.t;
   const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
-  const bool put = row < in.rows && t < in.T && slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : in.T);
+  const bool put = at.in && slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : in.T);
   const int64_t dst0 = b * c.sb + h * c.sh + slot;
   float x[2][8], lo[2] = {0.f, 0.f}, hi[2] = {0.f, 0.f};
   if (put) {
@@ -164,19 +180,17 @@ kv4_store_kernel(const Kv4Rows in, const Kv4View c, const Kv4Slots sl, const Kv4
   }
 }
 
-template <typename T, int D, bool VEC>
+template <typename T, int D, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_load_kernel(const Kv4Rows out, const Kv4View c, const Kv4Slots sl) {
   constexpr int LPR = D / 8;
   constexpr int LPG = kv4_group(D) / 8;
   grid_dependency_wait();
   grid_dependents_launch();
-  const uint32_t row = blockIdx.x * (KV4_THREADS / LPR) + threadIdx.x / LPR;
-  if (row >= out.rows) return;
   const int sub = threadIdx.x % LPR;
-  const Kv4Row at(out, row);
+  const Kv4Row<LPR, WHOLE> at(out);
+  if (!at.in) return;
   const uint32_t b = at.b, h = at.h, t = at.t;
-  if (t >= out.T) return;
   const int64_t slot = seq_value(sl.starts, b, sl.start) + t;
   const bool held = slot >= 0 && slot < c.cap && (int64_t)t < seq_value(sl.counts, b, sl.counts ? 0 : out.T);
   const int64_t src = b * c.sb + h * c.sh + slot, to = b * out.k_sb + t * out.k_st + h * out.k_sh + sub * 8;
@@ -211,12 +225,19 @@ kv4_load_kernel(const Kv4Rows out, const Kv4View c, const Kv4Slots sl) {
   }
 }
 
-template <typename T, int D, bool VEC>
-static int kv4_rows_launch(const Kv4Rows& r, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
+template <typename T, int D, bool VEC, bool WHOLE>
+static cudaError_t kv4_rows_start(const Kv4Rows& r, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
   constexpr uint32_t per = KV4_THREADS / (D / 8);
   const dim3 grid((r.rows + per - 1) / per);
-  const cudaError_t e = mk ? launch_pdl(kv4_store_kernel<T, D, VEC>, grid, dim3(KV4_THREADS), 0, s, r, c, sl, *mk)
-                           : launch_pdl(kv4_load_kernel<T, D, VEC>, grid, dim3(KV4_THREADS), 0, s, r, c, sl);
+  return mk ? launch_pdl(kv4_store_kernel<T, D, VEC, WHOLE>, grid, dim3(KV4_THREADS), 0, s, r, c, sl, *mk)
+            : launch_pdl(kv4_load_kernel<T, D, VEC, WHOLE>, grid, dim3(KV4_THREADS), 0, s, r, c, sl);
+}
+
+template <typename T, int D, bool VEC>
+static int kv4_rows_launch(const Kv4Rows& r, const Kv4View& c, const Kv4Slots& sl, const Kv4Marks* mk, cudaStream_t s) {
+  // sequences of at least a CTA's rows take CTAs of their own; the rows of shorter ones share them
+  const cudaError_t e = r.run == KV4_THREADS / (D / 8) ? kv4_rows_start<T, D, VEC, true>(r, c, sl, mk, s)
+                                                      : kv4_rows_start<T, D, VEC, false>(r, c, sl, mk, s);
   count_launch();
   return check_launch(mk ? "kv4_store_kernel" : "kv4_load_kernel", e);
 }
@@ -245,7 +266,7 @@ static int kv4_rows(const char* fn, Kv4Rows r, int B, int D, int dtype, const Kv
   for (int i = 0; i < 6; ++i) ATTN_REQUIRE(st[i] >= 0, "%s: strides must not be negative", fn);
   ATTN_REQUIRE(sl.starts || (sl.start >= 0 && (int64_t)sl.start + r.T <= c.cap),
                "%s: positions %d .. %lld exceed the capacity of %d", fn, sl.start, (long long)sl.start + r.T - 1, c.cap);
-  ATTN_REQUIRE(kv4_set_rows(&r, B) < (int64_t)1 << 31, "%s: B*NH*T must be below 2^31", fn);
+  ATTN_REQUIRE(kv4_set_rows(&r, B, KV4_THREADS / (D / 8)) < (int64_t)1 << 31, "%s: B*NH*T must be below 2^31", fn);
   return dtype == ATTN_BF16 ? kv4_rows_t<__nv_bfloat16>(r, D, c, sl, mk, s) : kv4_rows_t<float>(r, D, c, sl, mk, s);
 }
 
