@@ -295,7 +295,7 @@ int attn_key_weights(const void* q, const void* k, const float* lse, const float
                      int64_t w_sb, int64_t w_sh, int first_query, const int* lengths,
                      float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace attn_kv4_evict needs. */
+/* Bytes of workspace attn_kv4_evict needs (0 up to 16,384 rows). */
 size_t attn_kv4_evict_workspace_size(int B, int NH, int L, int keep);
 
 /*

@@ -8,17 +8,24 @@
 // slot < keep, so the move can run in place with every row in parallel, and evicting one row of a full
 // cache moves one row.
 //
-// The select kernel finds the keep-th largest order key by radix (four passes of 8 bits over a
-// histogram in shared memory), numbers the ties, holes and spare rows with block scans in slot order,
-// and writes slots[i] = the row that slot i holds afterwards (-1 past the kept ones).  The move kernel
-// copies rows.
+// One CTA selects for one (sequence, head).  Up to 16,384 rows it holds every row's order key in registers,
+// consecutive rows to a thread, and finds the keep-th largest bit by bit from the top: 32 counts, each a
+// warp reduction, one barrier and a sum over the warps (no atomics, so the weights' skewed exponents cost
+// nothing).  Longer sequences take a radix search, four passes of 8 bits over a histogram in shared memory.
+// Ties, holes and spare rows are numbered with block scans in slot order, and slots[i] = the row that slot i
+// holds afterwards (-1 past the kept ones).  The rows are then copied, codes in 16-byte pieces: by the same
+// CTA when there are enough of them to fill the GPU or few rows to move (one launch), else by a second kernel.
+#include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
+#include <type_traits>
 
 namespace attn {
 
-constexpr int EV_THREADS = 1024;
+constexpr int EV_THREADS = 512;
+constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MOVE_THREADS = 256;
+constexpr int EV_MOST = 32;  // rows per thread of the register select
 
 struct Kv4Evict {
   Kv4View src, dst;
@@ -34,16 +41,19 @@ struct Kv4Evict {
   int* slots;  // [B*NH][keep]
   int* spare;  // workspace [B*NH][2][keep]: holes, then the rows that fill them
   int in_place;
+  int fused;   // the select kernel moves the rows too
 };
 
 // Order of a row: larger is kept longer.  Protected rows first; then the weight by value (NaN last).
-__device__ __forceinline__ uint32_t evict_key(const Kv4Evict& p, int64_t row_w, int j, int64_t protect_from) {
-  const int64_t at = p.pos ? (int64_t)p.pos[row_w + j] : j;
-  if (at >= protect_from) return 0xffffffffu;
-  const float w = p.w[row_w + j] + 0.f;  // -0 counts as 0
+__device__ __forceinline__ uint32_t evict_key(float weight, int64_t position, int64_t protect_from) {
+  if (position >= protect_from) return 0xffffffffu;
+  const float w = weight + 0.f;  // -0 counts as 0
   if (w != w) return 0u;
   const uint32_t u = __float_as_uint(w);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint32_t evict_key(const Kv4Evict& p, int64_t row_w, int j, int64_t protect_from) {
+  return evict_key(p.w[row_w + j], p.pos ? (int64_t)p.pos[row_w + j] : j, protect_from);
 }
 
 // Exclusive prefix of v over the block, and its total.
@@ -59,24 +69,81 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   if (lane == 31) red[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int y = red[lane];
+    int y = lane < EV_WARPS ? red[lane] : 0;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int z = __shfl_up_sync(0xffffffffu, y, off);
       if (lane >= off) y += z;
     }
-    red[lane] = y;
+    if (lane < EV_WARPS) red[lane] = y;
   }
   __syncthreads();
-  *total = red[31];
+  *total = red[EV_WARPS - 1];
   return x - v + (warp ? red[warp - 1] : 0);
 }
 
+// Sum over the block of a value that is already summed over each warp (lane 0's counts).
+__device__ __forceinline__ int block_total(int warp_total, int* red) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  if (lane == 0) red[warp] = warp_total;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, lane < EV_WARPS ? red[lane] : 0);
+}
+
+// Copy rows [first, first + count) of the kept ones of one (sequence, head): slot i gets row slots[i].
+template <int D>
+__device__ __forceinline__ void evict_move(const Kv4Evict& p, int b, int h, const int* slots, int first, int count) {
+  constexpr int GROUPS = kv4_groups(D);
+  using Unit = typename std::conditional<(D >= 32), uint4, uint2>::type;
+  constexpr int UNITS = D / 2 / sizeof(Unit);  // of a row's codes
+  constexpr int BATCH = 4;                     // loads in flight per thread
+  const int64_t s0 = b * p.src.sb + h * p.src.sh, d0 = b * p.dst.sb + h * p.dst.sh;
+  const int64_t ws = b * p.w_sb + h * p.w_sh, wd = b * p.dw_sb + h * p.dw_sh;
+  for (int i = first + threadIdx.x; i < first + count; i += blockDim.x) {
+    const int from = slots[i];
+    if (from < 0 || (p.in_place && from == i)) continue;
+    __half2 k[GROUPS], v[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      k[g] = p.src.params[(s0 + from) * GROUPS + g];
+      v[g] = p.src.params[(p.src.si + s0 + from) * GROUPS + g];
+    }
+    const float w = p.w[ws + from];
+    const int at = p.pos ? p.pos[ws + from] : from;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      p.dst.params[(d0 + i) * GROUPS + g] = k[g];
+      p.dst.params[(p.dst.si + d0 + i) * GROUPS + g] = v[g];
+    }
+    p.dw[wd + i] = w;
+    if (p.dpos) p.dpos[wd + i] = at;
+  }
+  for (int which = 0; which < 2; ++which) {
+    const Unit* src = reinterpret_cast<const Unit*>(p.src.codes) + (which * p.src.si + s0) * UNITS;
+    Unit* dst = reinterpret_cast<Unit*>(p.dst.codes) + (which * p.dst.si + d0) * UNITS;
+    for (int u0 = threadIdx.x; u0 < count * UNITS; u0 += blockDim.x * BATCH) {
+      Unit x[BATCH];
+      bool go[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int u = u0 + k * blockDim.x, i = first + u / UNITS;
+        const int from = u < count * UNITS ? slots[i] : -1;
+        go[k] = from >= 0 && !(p.in_place && from == i);
+        if (go[k]) x[k] = src[(int64_t)from * UNITS + u % UNITS];
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int u = u0 + k * blockDim.x;
+        if (go[k]) dst[(int64_t)first * UNITS + u] = x[k];
+      }
+    }
+  }
+}
+
+// PER rows per thread in registers; PER = 0: any number of rows, read again for every pass.
+template <int D, int PER>
 __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4Evict p) {
-  __shared__ uint32_t hist[256];
-  __shared__ int red[32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
+  __shared__ int red[2][EV_WARPS];
   grid_dependency_wait();
   grid_dependents_launch();
   const int bh = blockIdx.x, b = bh / p.NH, h = bh % p.NH;
@@ -84,87 +151,191 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
   int* slots = p.slots + (int64_t)bh * p.keep;
   if (n <= p.keep) {  // everything stays
     for (int i = threadIdx.x; i < p.keep; i += EV_THREADS) slots[i] = i < n ? i : -1;
-    return;
-  }
-  const int64_t row_w = b * p.w_sb + h * p.w_sh;
-  const int64_t protect_from = seq_value(p.seen, b, p.seen0) - p.recent;
-  // the keep-th largest key, digit by digit from the top; s_left = how many of the rows that match
-  // the prefix so far are still to be kept
-  if (threadIdx.x == 0) {
-    s_prefix = 0;
-    s_left = p.keep;
-  }
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-    __syncthreads();
-    const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int j = threadIdx.x; j < n; j += EV_THREADS) {
-      const uint32_t key = evict_key(p, row_w, j, protect_from);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+  } else {
+    const int64_t row_w = b * p.w_sb + h * p.w_sh;
+    const int64_t protect_from = seq_value(p.seen, b, p.seen0) - p.recent;
+    if constexpr (PER > 0) {
+      const int base = threadIdx.x * PER;
+      __shared__ uint16_t holes[EV_THREADS * PER / 2], spare[EV_THREADS * PER / 2];  // at most min(keep, n - keep)
+      uint32_t key[PER];
+      const bool wide = PER % 4 == 0 && row_w % 4 == 0 && (reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.pos)) % 16 == 0;
+      if (wide && base + PER <= n) {
+#pragma unroll
+        for (int k = 0; k < PER; k += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(p.w + row_w + base + k);
+          const int4 at = p.pos ? *reinterpret_cast<const int4*>(p.pos + row_w + base + k)
+                                : make_int4(base + k, base + k + 1, base + k + 2, base + k + 3);
+          key[k] = evict_key(w.x, at.x, protect_from);
+          if constexpr (PER % 4 == 0) {
+            key[k + 1] = evict_key(w.y, at.y, protect_from);
+            key[k + 2] = evict_key(w.z, at.z, protect_from);
+            key[k + 3] = evict_key(w.w, at.w, protect_from);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) key[k] = base + k < n ? evict_key(p, row_w, base + k, protect_from) : 0u;
+      }
+      // rows past the end have key 0 and would count for limit 0 alone, which ends the search as well
+      uint32_t limit = 0;
+      int round = 0;
+      for (uint32_t bit = 0x80000000u; bit; bit >>= 1, ++round) {
+        const uint32_t cand = limit | bit;
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) c += key[k] >= cand;
+        const int total = block_total(__reduce_add_sync(0xffffffffu, c), red[round & 1]);
+        if (total >= p.keep) limit = cand;
+        if (total == p.keep) break;  // these are the kept ones: no lower bit can change that
+      }
+      int above = 0, tie = 0;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        above += key[k] > limit;
+        tie += base + k < n && key[k] == limit;
+      }
+      __syncthreads();  // (either half of red may have been read last)
+      const int ties = p.keep - block_total(__reduce_add_sync(0xffffffffu, above), red[0]);
+      int total;
+      int rank = block_scan(tie, red[1], &total);
+      uint32_t kept = 0;
+      int count = 0;  // holes, and spare rows in the upper half
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int j = base + k;
+        const bool same = j < n && key[k] == limit;
+        const bool stay = j < n && (key[k] > limit || (same && rank < ties));
+        rank += same;
+        kept |= (uint32_t)stay << k;
+        if (j < n && j < p.keep && !stay) count += 1;
+        if (j >= p.keep && stay) count += 1 << 16;
+      }
+      int at = block_scan(count, red[0], &total);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int j = base + k;
+        const bool stay = (kept >> k & 1) != 0;
+        if (j < p.keep) {
+          if (stay) slots[j] = j;
+          else if (j < n) {
+            holes[at & 0xffff] = (uint16_t)j;
+            at += 1;
+          }
+        } else if (stay) {
+          spare[at >> 16] = (uint16_t)j;
+          at += 1 << 16;
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < (total & 0xffff); i += EV_THREADS) slots[holes[i]] = spare[i];
+    } else {
+      __shared__ uint32_t hist[256];
+      __shared__ uint32_t s_prefix;
+      __shared__ int s_left;
+      // the keep-th largest key, digit by digit from the top; s_left = how many of the rows that match
+      // the prefix so far are still to be kept
+      if (threadIdx.x == 0) {
+        s_prefix = 0;
+        s_left = p.keep;
+      }
+      for (int shift = 24; shift >= 0; shift -= 8) {
+        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+        __syncthreads();
+        const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+        for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
+          const int j = j0 + threadIdx.x;
+          const uint32_t key = j < n ? evict_key(p, row_w, j, protect_from) : 0u;
+          const uint32_t digit = j < n && (key & mask) == prefix ? (key >> shift) & 255u : 256u;
+          // lanes of one digit (weights share few exponents) add as one
+          const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+          if (digit < 256u && threadIdx.x % 32 == __ffs(peers) - 1) atomicAdd(&hist[digit], __popc(peers));
+        }
+        __syncthreads();
+        if (threadIdx.x < 32) {  // lane l: digits 255 - 8 l downwards
+          const int lane = threadIdx.x;
+          int c[8], sum = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum += c[k] = (int)hist[255 - 8 * lane - k];
+          int before = sum;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, off);
+            if (lane >= off) before += y;
+          }
+          before -= sum;
+          const int left = s_left;
+          __syncwarp();
+          if (before < left && before + sum >= left) {  // exactly one lane
+            int k = 0;
+            while (k < 7 && before + c[k] < left) before += c[k++];
+            s_left = left - before;
+            s_prefix = prefix | (uint32_t)(255 - 8 * lane - k) << shift;
+          }
+        }
+        __syncthreads();
+      }
+      const uint32_t limit = s_prefix;
+      const int ties = s_left;  // rows equal to the limit that are kept, the lowest slots first
+      int* holes = p.spare + (int64_t)bh * 2 * p.keep;
+      int* spare = holes + p.keep;
+      int tie0 = 0, hole0 = 0, spare0 = 0;
+      for (int base = 0; base < n; base += EV_THREADS) {
+        const int j = base + threadIdx.x;
+        const uint32_t key = j < n ? evict_key(p, row_w, j, protect_from) : 0u;
+        const bool tie = j < n && key == limit;
+        int total;
+        const int rank = tie0 + block_scan(tie, red[0], &total);
+        tie0 += total;
+        const bool kept = j < n && (key > limit || (tie && rank < ties));
+        const bool hole = j < p.keep && !kept, extra = j >= p.keep && kept;
+        const int both = block_scan(hole | (int)extra << 16, red[1], &total);
+        if (hole) holes[hole0 + (both & 0xffff)] = j;
+        if (extra) spare[spare0 + (both >> 16)] = j;
+        if (j < p.keep && kept) slots[j] = j;
+        hole0 += total & 0xffff;
+        spare0 += total >> 16;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < hole0; i += EV_THREADS) slots[holes[i]] = spare[i];
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int left = s_left, digit = 255;
-      while (digit > 0 && (int)hist[digit] < left) left -= (int)hist[digit--];
-      s_left = left;
-      s_prefix = prefix | (uint32_t)digit << shift;
-    }
-    __syncthreads();
   }
-  const uint32_t limit = s_prefix;
-  const int ties = s_left;  // rows equal to the limit that are kept, the lowest slots first
-  int* holes = p.spare + (int64_t)bh * 2 * p.keep;
-  int* spare = holes + p.keep;
-  int tie0 = 0, hole0 = 0, spare0 = 0;
-  for (int base = 0; base < n; base += EV_THREADS) {
-    const int j = base + threadIdx.x;
-    const uint32_t key = j < n ? evict_key(p, row_w, j, protect_from) : 0u;
-    const bool tie = j < n && key == limit;
-    int total;
-    const int rank = tie0 + block_scan(tie, red, &total);
-    tie0 += total;
-    const bool kept = j < n && (key > limit || (tie && rank < ties));
-    const bool hole = j < p.keep && !kept, extra = j >= p.keep && kept;
-    const int both = block_scan(hole | (int)extra << 16, red, &total);
-    if (hole) holes[hole0 + (both & 0xffff)] = j;
-    if (extra) spare[spare0 + (both >> 16)] = j;
-    if (j < p.keep && kept) slots[j] = j;
-    hole0 += total & 0xffff;
-    spare0 += total >> 16;
+  if (p.fused) {
+    __syncthreads();
+    evict_move<D>(p, b, h, slots, 0, min(n, p.keep));
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < hole0; i += EV_THREADS) slots[holes[i]] = spare[i];
 }
 
 template <int D>
 __global__ void __launch_bounds__(EV_MOVE_THREADS) kv4_evict_move_kernel(const Kv4Evict p) {
-  // a row's codes go in words of 4 bytes: D / 8 threads a row, K in grid.z = 0, V in 1
-  constexpr int LPR = D / 8, ROWS = EV_MOVE_THREADS / LPR;
   grid_dependency_wait();
   grid_dependents_launch();
-  const int chunks = (p.keep + ROWS - 1) / ROWS;
-  const int bh = blockIdx.x / chunks, i = (blockIdx.x % chunks) * ROWS + threadIdx.x / LPR, sub = threadIdx.x % LPR;
-  if (i >= p.keep) return;
-  const int from = p.slots[(int64_t)bh * p.keep + i];
-  if (from < 0 || (p.in_place && from == i)) return;
-  const int b = bh / p.NH, h = bh % p.NH;
-  const int64_t s = blockIdx.y * p.src.si + b * p.src.sb + h * p.src.sh + from;
-  const int64_t d = blockIdx.y * p.dst.si + b * p.dst.sb + h * p.dst.sh + i;
-  *reinterpret_cast<uint32_t*>(p.dst.codes + d * (D / 2) + sub * 4) =
-      *reinterpret_cast<const uint32_t*>(p.src.codes + s * (D / 2) + sub * 4);
-  if (sub < kv4_groups(D)) p.dst.params[d * kv4_groups(D) + sub] = p.src.params[s * kv4_groups(D) + sub];
-  if (blockIdx.y == 0 && sub == 0) {
-    const int64_t ws = b * p.w_sb + h * p.w_sh + from, wd = b * p.dw_sb + h * p.dw_sh + i;
-    p.dw[wd] = p.w[ws];
-    if (p.dpos) p.dpos[wd] = p.pos ? p.pos[ws] : from;
-  }
+  const int chunks = (p.keep + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
+  const int bh = blockIdx.x / chunks, first = (blockIdx.x - bh * chunks) * EV_MOVE_THREADS;
+  const int b = bh / p.NH, h = bh - b * p.NH;
+  evict_move<D>(p, b, h, p.slots + (int64_t)bh * p.keep, first, min(EV_MOVE_THREADS, p.keep - first));
 }
 
 template <int D>
-static cudaError_t kv4_evict_move(const Kv4Evict& p, int B, cudaStream_t s) {
-  constexpr int ROWS = EV_MOVE_THREADS / (D / 8);
-  const unsigned chunks = (p.keep + ROWS - 1) / ROWS;
-  return launch_pdl(kv4_evict_move_kernel<D>, dim3(chunks * B * p.NH, 2), dim3(EV_MOVE_THREADS), 0, s, p);
+static int kv4_evict_d(Kv4Evict& p, int B, cudaStream_t s) {
+  // one launch where there is little to move: a CTA moves a thousand rows in a few microseconds, while half of
+  // 32 x 8 heads of 8,192 rows took 90 us in one launch (a CTA's registers leave it alone on its SM) and 67 in two
+  const int rows = p.in_place ? (p.L - p.keep < p.keep ? p.L - p.keep : p.keep) : (p.L < p.keep ? p.L : p.keep);
+  const int64_t heads = (int64_t)B * p.NH;
+  p.fused = rows <= 1024;
+  const dim3 grid((unsigned)heads), block(EV_THREADS);
+  cudaError_t e;
+  if (p.L <= EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 1>, grid, block, 0, s, p);
+  else if (p.L <= 4 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 4>, grid, block, 0, s, p);
+  else if (p.L <= 16 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 16>, grid, block, 0, s, p);
+  else if (p.L <= EV_MOST * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, EV_MOST>, grid, block, 0, s, p);
+  else e = launch_pdl(kv4_evict_select_kernel<D, 0>, grid, block, 0, s, p);
+  count_launch();
+  if (int rc = check_launch("kv4_evict_select_kernel", e)) return rc;
+  if (p.fused) return ATTN_OK;
+  const unsigned chunks = (p.keep + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
+  e = launch_pdl(kv4_evict_move_kernel<D>, dim3(chunks * (unsigned)heads), dim3(EV_MOVE_THREADS), 0, s, p);
+  count_launch();
+  return check_launch("kv4_evict_move_kernel", e);
 }
 
 }  // namespace attn
@@ -173,7 +344,7 @@ using namespace attn;
 
 extern "C" size_t attn_kv4_evict_workspace_size(int B, int NH, int L, int keep) {
   if (B <= 0 || NH <= 0 || L <= 0 || keep <= 0) return 0;
-  return (size_t)B * NH * 2 * keep * sizeof(int);
+  return L <= attn::EV_MOST * attn::EV_THREADS ? 0 : (size_t)B * NH * 2 * keep * sizeof(int);
 }
 
 extern "C" int attn_kv4_evict(void* codes, void* params, float* weights, int* positions, int64_t c_si, int64_t c_sb,
@@ -199,7 +370,7 @@ extern "C" int attn_kv4_evict(void* codes, void* params, float* weights, int* po
   ATTN_REQUIRE(recent >= 0 && recent <= keep, "attn_kv4_evict: recent %d outside 0 .. keep %d", recent, keep);
   ATTN_REQUIRE(weights && slots && (in_place || dst_weights), "attn_kv4_evict: null pointer argument");
   const size_t need = attn_kv4_evict_workspace_size(B, NH, L, keep);
-  if (!workspace || workspace_bytes < need) {
+  if (need && (!workspace || workspace_bytes < need)) {
     set_error("attn_kv4_evict: workspace of %zu bytes required", need);
     return ATTN_ERR_WORKSPACE;
   }
@@ -215,15 +386,10 @@ extern "C" int attn_kv4_evict(void* codes, void* params, float* weights, int* po
   p.lengths = lengths; p.seen = seen; p.seen0 = seen0;
   p.slots = slots; p.spare = (int*)workspace; p.in_place = in_place;
   cudaStream_t s = as_stream(stream);
-  cudaError_t e = launch_pdl(kv4_evict_select_kernel, dim3(B * NH), dim3(EV_THREADS), 0, s, p);
-  count_launch();
-  if (int rc = check_launch("kv4_evict_select_kernel", e)) return rc;
   switch (D) {
-    case 16: e = kv4_evict_move<16>(p, B, s); break;
-    case 32: e = kv4_evict_move<32>(p, B, s); break;
-    case 64: e = kv4_evict_move<64>(p, B, s); break;
-    default: e = kv4_evict_move<128>(p, B, s); break;
+    case 16: return kv4_evict_d<16>(p, B, s);
+    case 32: return kv4_evict_d<32>(p, B, s);
+    case 64: return kv4_evict_d<64>(p, B, s);
+    default: return kv4_evict_d<128>(p, B, s);
   }
-  count_launch();
-  return check_launch("kv4_evict_move_kernel", e);
 }

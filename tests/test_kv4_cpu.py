@@ -91,8 +91,8 @@ def test_bad_caches_are_refused(call, bad, code, text):
     (_weights, dict(D=160), UNSUPPORTED, "head_dim"), (_weights, dict(T=256, ws_bytes=4), WORKSPACE, "workspace"), (_weights, dict(k_st=-1), ARG, "negative"),
     (_evict, dict(weights=None), ARG, "null"), (_evict, dict(slots=None), ARG, "null"), (_evict, dict(L=17), ARG, "length"),
     (_evict, dict(L=0), ARG, "length"), (_evict, dict(keep=0), ARG, "keep"), (_evict, dict(keep=17), ARG, "keep"),
-    (_evict, dict(recent=5), ARG, "recent"), (_evict, dict(recent=-1), ARG, "recent"), (_evict, dict(ws=None), WORKSPACE, "workspace"),
-    (_evict, dict(ws_bytes=4), WORKSPACE, "workspace"), (_evict, dict(c_sb=0), ARG, "overlap"),
+    (_evict, dict(recent=5), ARG, "recent"), (_evict, dict(recent=-1), ARG, "recent"), (_evict, dict(L=20000, cap=20000, c_sh=20000, c_sb=40000, c_si=80000, ws=None), WORKSPACE, "workspace"),
+    (_evict, dict(L=20000, cap=20000, c_sh=20000, c_sb=40000, c_si=80000, ws_bytes=4), WORKSPACE, "workspace"), (_evict, dict(c_sb=0), ARG, "overlap"),
     (_evict, dict(dc=FAKE, dp=2 * FAKE, dw=2 * FAKE, d_si=64, d_sb=32, d_sh=16, dcap=16), ARG, "another cache"),
     (_evict, dict(dc=2 * FAKE, dp=2 * FAKE, dw=None, d_si=64, d_sb=32, d_sh=16, dcap=16), ARG, "null"),
     (_evict, dict(dc=2 * FAKE, dp=2 * FAKE, dw=2 * FAKE, d_si=64, d_sb=32, d_sh=16, dcap=8), ARG, "multiples of 16"),
