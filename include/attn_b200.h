@@ -256,8 +256,9 @@ int attn_kv4_load(const void* codes, const void* params, int64_t c_si, int64_t c
                   const int* counts, void* k, void* v, int dtype,
                   int64_t o_sb, int64_t o_st, int64_t o_sh, void* stream);
 
-/* Bytes of workspace attn_kv4_decode needs (weights: whether weights_out is given). */
-size_t attn_kv4_decode_workspace_size(int B, int NH, int L, int D, int weights);
+/* Bytes of workspace attn_kv4_decode needs on the current device (weights: whether weights_out is given;
+ * may be 0). */
+size_t attn_kv4_decode_workspace_size(int B, int NH, int NKV, int L, int D, int dtype, int weights);
 
 /*
  * Single-query decode over a 4-bit cache: for each of the NH query heads of each sequence, attention

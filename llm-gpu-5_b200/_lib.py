@@ -52,7 +52,7 @@ SIGNATURES = {
                             _i64, _i, _p, _i, _p, _p, _p, _i64, _i64, _p, _i, _p]),
     "attn_kv4_load": (_i, [_p, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _i, _i64, _i64,
                            _i64, _p]),
-    "attn_kv4_decode_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "attn_kv4_decode_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "attn_kv4_decode": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i,
                              _p, _p, _p, _i64, _i64, _f, _i, _p, _sz, _p]),
     "attn_key_weights": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64,

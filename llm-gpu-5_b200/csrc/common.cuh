@@ -77,13 +77,13 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// The same for a kernel of CTA pairs: clusters of two consecutive CTAs along x (grid.x even).
+// The same for a kernel of clusters of `size` consecutive CTAs along x (grid.x a multiple of it).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pdl_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                                    Args&&... args) {
+inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), unsigned size, dim3 grid, dim3 block, size_t smem,
+                                      cudaStream_t s, Args&&... args) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = size;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -96,6 +96,13 @@ inline cudaError_t launch_pdl_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 bl
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Clusters of CTA pairs.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_pdl_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                    Args&&... args) {
+  return launch_pdl_cluster(kernel, 2, grid, block, smem, s, std::forward<Args>(args)...);
 }
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

@@ -24,11 +24,12 @@
 //     in two columns of the same product, and so does p s for a float32 output (its second part 2^11
 //     times too large, so that small weights keep it too), so their products are good to 2^-22.
 //
-// A warp takes tiles of 64 keys through a ring of its own of cp.async stages (no barrier between warps):
-// scores into shared memory, then one key per lane for the softmax, whose running maximum moves only
-// when it grows by more than 2^8 (the accumulators are rescaled then), then p s back as the B operand.
-// The length is split over CTAs; each writes an unnormalised partial state (m, l, o[D]) and the combine
-// kernel merges them and adds the weights.  A call with one split finishes in the first kernel.
+// A warp takes tiles of 64 keys (32 at head_dim 128) through a ring of its own of cp.async stages (no barrier
+// between warps): scores into shared memory, then one key per lane for the softmax, whose running maximum
+// moves only when it grows by more than 2^8 (the accumulators are rescaled then), then p s back as the B
+// operand.  The length is split over the CTAs of a cluster, up to eight, which merge their states (m, l, o[D])
+// through distributed shared memory and add the weights of their own keys: one launch.  Few heads over long
+// sequences need more CTAs than that: these write their states to the workspace for a combine kernel.
 #include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
@@ -37,9 +38,9 @@ namespace attn {
 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
-constexpr int KD_TILE = 64;      // keys per warp step
 constexpr int KD_WCHUNK = 1024;  // keys per combine CTA
-constexpr int KD_SPLIT = KD_TILE * KD_WARPS;  // keys a CTA takes in one round of its warps
+constexpr int KD_SPLIT = 64 * KD_WARPS;  // keys a CTA takes at least, where there are so many
+constexpr int KD_CLUSTER = 8;            // most CTAs of a cluster (the portable limit)
 
 struct Kv4Decode {
   const void* q;
@@ -50,21 +51,25 @@ struct Kv4Decode {
   float* w_out;
   int64_t q_sb, q_sh, o_sb, o_sh, w_sb, w_sh;
   int NH, NKV, G, L;
-  int ns, per;     // splits, keys per split (a multiple of KD_TILE)
+  int ns, per;     // splits, keys per split (a multiple of 64)
+  int cluster;     // the splits are a cluster's CTAs
   int nq, chunks;  // query heads per CTA, and CTAs' chunks of them per key head
-  float scale, scale_log2;
-  float* states;  // [B*NH][ns][D + 2]: max (log2 units), sum, unnormalised o; unused with one split
-  float* scores;  // [B*NH][L]: scores in log2 units; NULL without weights
+  float scale_log2;
+  int alone;       // this kernel finishes o and lse
+  float* states;  // [B*NH][ns][D + 2]: max (log2 units), sum, unnormalised o; alone, [B*NH][2]: max and sum
+  float* scores;  // [B*NH][L]: scores in log2 units, where they do not fit beside the CTA's other shared memory
+  int weights;    // whether weights are wanted
+  int zsmem;      // the scores of the CTA's keys stay in shared memory
 };
 
-// The most splits a call's keys are cut into: rounds of a CTA's warps, at least the two that a call
-// with weights and several chunks of query heads takes, and at most KD_MOST_SPLITS.
+// The most splits a call's keys are cut into: rounds of a CTA's warps, at most KD_MOST_SPLITS.
 constexpr int KD_MOST_SPLITS = 128;
 static int kd_most_splits(int L) {
   const int rounds = (L + KD_SPLIT - 1) / KD_SPLIT;
-  return rounds < 2 ? 2 : rounds < KD_MOST_SPLITS ? rounds : KD_MOST_SPLITS;
+  return rounds < KD_MOST_SPLITS ? rounds : KD_MOST_SPLITS;
 }
-static size_t kd_states(int64_t BH, int L, int D) { return ((size_t)BH * kd_most_splits(L) * (D + 2) + 3) / 4 * 4; }
+// Scores that a CTA keeps in shared memory for the weights (16 KB).
+constexpr int KD_ZFLOATS = 4096;
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
@@ -106,23 +111,27 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 
 // Codes in place: nibbles 0 and 1 of each half word (n * 2^-24 and 16 n * 2^-24 as float16).
 constexpr uint32_t KD_LOW = 0x000f000fu, KD_HIGH = 0x00f000f0u;
-// Nibble I of each half word at the top of a float16's mantissa: n * 2^-18.
-template <int I>
-__device__ __forceinline__ uint32_t kd_top(uint32_t w) {
-  constexpr int SHIFT = 6 - 4 * I;
-  return (SHIFT > 0 ? w << (SHIFT > 0 ? SHIFT : 0) : w >> (SHIFT > 0 ? 0 : -SHIFT)) & 0x03c003c0u;
-}
-// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs, in place or at the top.
+constexpr uint32_t KD_TOP = 0x03c003c0u;
+// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs: in place, or at the top of the
+// mantissa, n * 2^-18 (the left shifts as products, which run beside the ANDs on the multiply-add pipe).
 template <bool TOP, int PAIR>
 __device__ __forceinline__ void kd_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
+  const uint32_t x = PAIR ? w >> 8 : w;
   if constexpr (TOP) {
-    a = kd_top<2 * PAIR>(w);
-    b = kd_top<2 * PAIR + 1>(w);
+    a = (x * 64u) & KD_TOP;
+    b = (x * 4u) & KD_TOP;
   } else {
-    const uint32_t x = PAIR ? w >> 8 : w;
     a = x & KD_LOW;
     b = x & KD_HIGH;
   }
+}
+// c += (codes of two key rows) * (query): four codes a lane of each row.
+template <int PAIR>
+__device__ __forceinline__ void kd_score_mma(float (&c)[4], uint32_t wa, uint32_t wb, const uint32_t (&q)[2]) {
+  uint32_t a0, a1, a2, a3;
+  kd_pairs<true, PAIR>(wa, a0, a2);
+  kd_pairs<true, PAIR>(wb, a1, a3);
+  mma_f16(c, a0, a1, a2, a3, q[0], q[1]);
 }
 // acc += (codes of one value row pair) * (p s): x holds four elements of two keys, y of two more.
 template <bool TOP, int PAIR>
@@ -136,32 +145,49 @@ __device__ __forceinline__ void kd_value_mma(float (&acc)[4], uint32_t x, uint32
 // Sizes of a warp's shared memory for head_dim D and NQ queries.
 template <int D, int NQ, bool F32>
 struct KdTile {
+  static constexpr int TILE = D >= 128 ? 32 : 64;        // keys per warp step
   static constexpr int GROUPS = kv4_groups(D);
   static constexpr int COLS = F32 ? 2 * NQ : NQ;         // columns of the products
-  static constexpr int CODE_BYTES = KD_TILE * D / 2;     // one of K, V
-  static constexpr int PARAM_BYTES = KD_TILE * GROUPS * 4;
+  static constexpr int CODE_BYTES = TILE * D / 2;        // one of K, V
+  static constexpr int PARAM_BYTES = TILE * GROUPS * 4;
   static constexpr int STAGE = 2 * (CODE_BYTES + PARAM_BYTES);
-  static constexpr int STAGES = D >= 128 ? 2 : 3;
-  static constexpr int SC_LD = 68;                       // floats per query of the score tile (no bank conflicts)
-  static constexpr int P_LD = 80;                        // halves per column of the p s tile (likewise)
+  static constexpr int STAGES = D >= 64 ? 2 : 3;
+  static constexpr int SC_LD = TILE + 4;                 // floats per query of the score tile (no bank conflicts)
+  static constexpr int P_LD = TILE + 16;                 // halves per column of the p s tile (likewise)
   static constexpr int SC_BYTES = NQ * SC_LD * 4;
   static constexpr int P_BYTES = GROUPS * COLS * P_LD * 2;
   static constexpr int WARP = STAGES * STAGE + SC_BYTES + P_BYTES;
   static constexpr int Q_FLOATS = NQ * D + NQ * (1 + GROUPS);
-  static constexpr int MERGE = KD_WARPS * NQ * (D + 2) * 4;  // the warps' states, over the stages at the end
+  static constexpr int MERGE = (KD_WARPS + 1) * NQ * (D + 2) * 4;  // the warps' states and the CTA's, over the stages
   static constexpr int BYTES = KD_WARPS * WARP + Q_FLOATS * 4;
   static_assert(STAGE % 16 == 0 && SC_BYTES % 16 == 0 && P_BYTES % 16 == 0, "alignment");
   static_assert(MERGE <= KD_WARPS * WARP, "the merge reuses the stages");
 };
 
-// o, lse and the accumulated weights of one query head from its merged maximum and sum.
+__device__ __forceinline__ float kd_peer_load(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+// A float of CTA `rank` of the cluster, at the place of p in this CTA's shared memory.
+__device__ __forceinline__ float kd_peer(const float* p, uint32_t rank) {
+  return kd_peer_load(cluster_addr(p, rank));
+}
+
 __device__ __forceinline__ float kd_lse(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY; }
 
+// Every thread of the cluster's CTAs: earlier writes are visible to the others after it.  All CTAs of a
+// cluster are resident together and reach both of the kernel's syncs on every path.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c, const Kv4Decode p) {
+__global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4_decode_kernel(const Kv4View c, const Kv4Decode p) {
   constexpr bool F32 = sizeof(T) == 4;
   using S = KdTile<D, NQ, F32>;
-  constexpr int GROUPS = S::GROUPS, GS = kv4_group(D);
+  constexpr int GROUPS = S::GROUPS, GS = kv4_group(D), KD_TILE = S::TILE, PL = KD_TILE / 32;  // PL keys per lane
   constexpr int MT = D / 16;   // 16-row tiles of the value product
   constexpr int KS = D / 16;   // 16-deep steps of the score product
   extern __shared__ __align__(16) uint8_t smem[];
@@ -199,7 +225,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
         const uint8_t* src = c.codes + row * (D / 2);
         uint8_t* dst = st + which * S::CODE_BYTES;
 #pragma unroll
-        for (int k = 0; k < S::CODE_BYTES / 512; ++k)
+        for (int k = 0; k < (S::CODE_BYTES + 511) / 512; ++k)
           if ((k * 32 + lane) * 16 < rows * (D / 2)) cp_async16(dst + (k * 32 + lane) * 16, src + (k * 32 + lane) * 16);
         const uint8_t* psrc = reinterpret_cast<const uint8_t*>(c.params + row * GROUPS);
         uint8_t* pdst = st + 2 * S::CODE_BYTES + which * S::PARAM_BYTES;
@@ -272,6 +298,10 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
     }
   }
 
+  // scores kept for the weights: this CTA's keys in shared memory, or every key's in the workspace
+  float* zrow = p.zsmem ? reinterpret_cast<float*>(smem + S::BYTES) - j0 : p.scores + ((int64_t)b * p.NH + h0) * p.L;
+  const int64_t zld = p.zsmem ? p.per : p.L;
+
   float m[NQ], l[NQ], mg[NQ][GROUPS];
   float acc[MT][4];
 #pragma unroll
@@ -320,15 +350,15 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
 #pragma unroll
           for (int w = 0; w < WORDS; ++w) {
             const int s = (k * WORDS + w) * 2;
-            mma_f16(cs[k], kd_top<0>(wa[w]), kd_top<0>(wb[w]), kd_top<1>(wa[w]), kd_top<1>(wb[w]), qb[s][0], qb[s][1]);
-            mma_f16(cs[k], kd_top<2>(wa[w]), kd_top<2>(wb[w]), kd_top<3>(wa[w]), kd_top<3>(wb[w]), qb[s + 1][0], qb[s + 1][1]);
+            kd_score_mma<0>(cs[k], wa[w], wb[w], qb[s]);
+            kd_score_mma<1>(cs[k], wa[w], wb[w], qb[s + 1]);
           }
         }
       } else {
         // 4 codes per lane: byte 0 to the low half, byte 1 to the high half
         const uint32_t xa = __byte_perm(*reinterpret_cast<const uint16_t*>(ra + t * 2), 0, 0x4140);
         const uint32_t xb = __byte_perm(*reinterpret_cast<const uint16_t*>(rb + t * 2), 0, 0x4140);
-        mma_f16(cs[0], kd_top<0>(xa), kd_top<0>(xb), kd_top<1>(xa), kd_top<1>(xb), qb[0][0], qb[0][1]);
+        kd_score_mma<0>(cs[0], xa, xb, qb[0]);
       }
       float r[4] = {cs[0][0], cs[0][1], cs[0][2], cs[0][3]};
       if constexpr (GROUPS == 2) {  // the groups' scales belong to the key: rows g and g + 8
@@ -357,12 +387,12 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
     }
     __syncwarp();
 
-    // ---- softmax: keys lane and lane + 32 of the tile ----
-    float ks[2][GROUPS], km[2][GROUPS], vs[2][GROUPS], vm[2][GROUPS];
-    bool valid[2];
+    // ---- softmax: key lane of every 32 of the tile ----
+    float ks[PL][GROUPS], km[PL][GROUPS], vs[PL][GROUPS], vm[PL][GROUPS];
+    bool valid[PL];
     float vbig = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < PL; ++u) {
       const int key = u * 32 + lane;
       valid[u] = j + key < j1;
 #pragma unroll
@@ -374,21 +404,21 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
         vbig = fmaxf(vbig, vs[u][k]);
       }
     }
-    float z[NQ][2];
+    float z[NQ][PL];
     bool grow = false;
     float top[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       const float f = sfac[q];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < PL; ++u) {
         const float raw = sc[q * S::SC_LD + u * 32 + lane] * f;
         float s = GROUPS == 1 ? raw * ks[u][0] : raw;
 #pragma unroll
         for (int k = 0; k < GROUPS; ++k) s = fmaf(km[u][k], ssum[q * GROUPS + k], s);
         z[q][u] = valid[u] ? s : -INFINITY;
       }
-      top[q] = warp_max(fmaxf(z[q][0], z[q][1]));
+      top[q] = warp_max(fmaxf(z[q][0], z[q][PL - 1]));
       grow = grow || top[q] > m[q] + 8.f;
     }
     vbig = warp_max(vbig);
@@ -427,7 +457,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
     // p <= 2^8 and s 2^-ve < 2, so p s 2^(6 - ve) stays below 2^15
     const float vup = __uint_as_float((uint32_t)(127 + 6 - ve) << 23);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < PL; ++u) {
       const int key = u * 32 + lane;
       // position of the key among its 16 in the B operand: lane t's four slots are keys t, t+4, t+8, t+12
       const int at = (key & ~15) + (key & 3) * 4 + ((key >> 2) & 3);
@@ -435,7 +465,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
       for (int q = 0; q < NQ; ++q) {
         const float e = valid[u] ? ex2(z[q][u] - m[q]) : 0.f;
         l[q] += e;
-        if (p.scores && valid[u] && q < nq) p.scores[((int64_t)b * p.NH + h0 + q) * p.L + j + key] = z[q][u];
+        if (p.weights && valid[u] && q < nq) zrow[q * zld + j + key] = z[q][u];
 #pragma unroll
         for (int k = 0; k < GROUPS; ++k) {
           mg[q][k] = fmaf(e, vm[u][k], mg[q][k]);
@@ -520,9 +550,11 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
     }
   }
   __syncthreads();
+  // ---- the CTA's state: [query][D + 2] behind the warps' ----
   const float* all = reinterpret_cast<const float*>(smem);
+  float* own = reinterpret_cast<float*>(smem) + KD_WARPS * NQ * (D + 2);
   for (int i = threadIdx.x; i < nq * D; i += KD_THREADS) {
-    const int q = i / D, d = i % D, h = h0 + q;
+    const int q = i / D, d = i % D;
     float mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < KD_WARPS; ++w) mx = fmaxf(mx, all[(w * NQ + q) * (D + 2)]);
@@ -532,51 +564,62 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_kernel(const Kv4View c,
     for (int w = 0; w < KD_WARPS; ++w) {
       const float* a = all + (w * NQ + q) * (D + 2);
       const float f = ex2(a[0] - ref);
-      if (a[0] != -INFINITY || a[1] != 0.f) {
-        sum = fmaf(a[1], f, sum);
-        o = fmaf(a[2 + d], f, o);
-      }
+      sum = fmaf(a[1], f, sum);
+      o = fmaf(a[2 + d], f, o);
     }
-    const int64_t bh = (int64_t)b * p.NH + h;
-    if (p.ns > 1) {
-      float* stt = p.states + (bh * p.ns + split) * (D + 2);
-      stt[2 + d] = o;
-      if (d == 0) {
-        stt[0] = mx;
-        stt[1] = sum;
-      }
-    } else {
-      Elem<T>::store((T*)p.o + b * p.o_sb + h * p.o_sh + d, sum > 0.f || sum != sum ? o / sum : 0.f);
-      if (d == 0 && p.lse) p.lse[bh] = kd_lse(mx, sum);
+    float* to = !p.alone ? p.states + (((int64_t)b * p.NH + h0 + q) * p.ns + split) * (D + 2) : own + q * (D + 2);
+    to[2 + d] = o;
+    if (d == 0) {
+      to[0] = mx;
+      to[1] = sum;
     }
   }
-  if (p.ns == 1 && p.scores && p.chunks == 1) {  // one split over all of a key head's queries: the weights too
-    float mx[NQ], inv[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      mx[q] = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < KD_WARPS; ++w) mx[q] = fmaxf(mx[q], all[(w * NQ + q) * (D + 2)]);
-      const float ref = mx[q] == -INFINITY ? 0.f : mx[q];
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < KD_WARPS; ++w) {
-        const float* a = all + (w * NQ + q) * (D + 2);
-        if (a[0] != -INFINITY || a[1] != 0.f) sum = fmaf(a[1], ex2(a[0] - ref), sum);
-      }
-      mx[q] = ref;
-      inv[q] = 1.f / sum;
+  if (!p.alone) return;  // merged by the combine kernel
+
+  // ---- merge over the cluster (or this CTA alone) ----
+  if (p.cluster) cluster_sync();
+  else __syncthreads();
+  float* smx = sfac;  // [NQ] merged maxima, [NQ] reciprocal sums (the queries' factors are no longer needed)
+  float* sinv = sfac + NQ;
+  if (threadIdx.x < nq) {
+    const float* a = own + threadIdx.x * (D + 2);
+    float mx = -INFINITY, sum = 0.f;
+    for (int r = 0; r < p.ns; ++r) mx = fmaxf(mx, p.cluster ? kd_peer(a, r) : a[0]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    for (int r = 0; r < p.ns; ++r)
+      sum = fmaf(p.cluster ? kd_peer(a + 1, r) : a[1], ex2((p.cluster ? kd_peer(a, r) : a[0]) - ref), sum);
+    smx[threadIdx.x] = ref;
+    sinv[threadIdx.x] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int64_t bh = (int64_t)b * p.NH + h0 + threadIdx.x;
+    if (split == 0 && p.lse) p.lse[bh] = kd_lse(ref, sum);
+    if (split == 0 && p.weights && p.chunks > 1) {
+      p.states[bh * 2] = ref;
+      p.states[bh * 2 + 1] = sum;
     }
-    for (int key = threadIdx.x; key < p.L; key += KD_THREADS) {
-      float w = 0.f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x + split * KD_THREADS; i < nq * D; i += p.ns * KD_THREADS) {
+    const int q = i / D, d = i % D;
+    const float* a = own + q * (D + 2);
+    float o = 0.f;
+    for (int r = 0; r < p.ns; ++r)
+      o = fmaf(p.cluster ? kd_peer(a + 2 + d, r) : a[2 + d], ex2((p.cluster ? kd_peer(a, r) : a[0]) - smx[q]), o);
+    Elem<T>::store((T*)p.o + b * p.o_sb + (h0 + q) * p.o_sh + d, o * sinv[q]);
+  }
+  if (p.weights && p.chunks == 1) {  // all of a key head's queries are this CTA's: the weights of this CTA's keys
+    const int64_t w0 = b * p.w_sb + kvh * p.w_sh;
+    const int end = split + 1 == p.ns ? p.L : min(p.L, j0 + p.per);
+    for (int key = j0 + threadIdx.x; key < end; key += KD_THREADS) {
+      float w = p.w_in ? p.w_in[w0 + key] : 0.f;
+      float sum = 0.f;
       if (key < n)
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
-          if (q < nq) w += ex2(p.scores[((int64_t)b * p.NH + h0 + q) * p.L + key] - mx[q]) * inv[q];
-      const int64_t at = b * p.w_sb + kvh * p.w_sh + key;
-      p.w_out[at] = (p.w_in ? p.w_in[at] : 0.f) + w;
+          if (q < nq) sum = fmaf(ex2(zrow[q * zld + key] - smx[q]), sinv[q], sum);
+      p.w_out[w0 + key] = w + sum;
     }
   }
+  if (p.cluster) cluster_sync();  // the others may still read this CTA's state
 }
 
 __device__ __forceinline__ float block_reduce(float v, float* red, bool is_max) {
@@ -599,7 +642,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
   __shared__ float red[KD_THREADS / 32];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int wchunks = p.scores ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
+  const int wchunks = p.weights ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
   const int bk = blockIdx.x / wchunks, chunk = blockIdx.x % wchunks;
   const int b = bk / p.NKV, kvh = bk % p.NKV;
   const int n = seq_length(p.lengths, b, p.L);
@@ -612,7 +655,10 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
     const int h = kvh * p.G + g;
     const int64_t bh = (int64_t)b * p.NH + h;
     float mx, sum;
-    if (p.ns > 1) {
+    if (p.alone) {
+      mx = p.states[bh * 2];
+      sum = p.states[bh * 2 + 1];
+    } else {
       const float* st = p.states + bh * p.ns * (D + 2);
       mx = -INFINITY;
       sum = 0.f;
@@ -631,7 +677,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
         if (threadIdx.x == 0 && p.lse) p.lse[bh] = kd_lse(mx, sum);
       }
     }
-    if (p.scores) {
+    if (p.weights) {
       const float inv = 1.f / sum;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -640,7 +686,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
       }
     }
   }
-  if (p.scores) {
+  if (p.weights) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int j = j0 + i * KD_THREADS + threadIdx.x;
@@ -652,55 +698,84 @@ __global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv
   }
 }
 
-template <typename T, int D, int NQ>
-static int kv4_decode_q(const Kv4View& c, Kv4Decode p, int B, int sms, cudaStream_t s) {
-  using S = KdTile<D, NQ, sizeof(T) == 4>;
-  static_assert(S::BYTES <= 227 * 1024, "shared memory");
-  p.chunks = (p.G + NQ - 1) / NQ;
-  // enough splits that every SM holds several CTAs, each with at least one round of its warps
-  const int64_t units = (int64_t)B * p.NKV * p.chunks;
-  const int64_t want = ((int64_t)sms * 8 + units - 1) / units;
-  const int most = p.L <= KD_SPLIT ? 1 : kd_most_splits(p.L);
-  const int ns = (int)(want < most ? want : most);
-  const int tiles = (p.L + KD_TILE - 1) / KD_TILE;
-  p.per = (tiles + ns - 1) / ns * KD_TILE;
-  p.ns = (p.L + p.per - 1) / p.per;
-  if (p.ns == 1 && p.scores && p.chunks > 1) {  // the weights need every query's sum: use the combine kernel
-    p.per = (tiles + 1) / 2 * KD_TILE;
-    p.ns = 2;
+// How a call is cut up.
+struct KdPlan {
+  int nq, chunks, ns, per, cluster, alone, zsmem;  // alone: the first kernel finishes o and lse
+  size_t states, scores;  // floats of workspace
+};
+
+static KdPlan kd_plan(int B, int NH, int NKV, int L, int D, int dtype, int weights) {
+  KdPlan k;
+  const int G = NH / NKV;
+  // a product has eight columns: eight queries, or four float32 ones in two parts each
+  const int most_q = dtype == ATTN_F32 ? 4 : 8;
+  k.nq = G == 1 ? 1 : G == 2 ? 2 : G <= 4 || most_q == 4 ? 4 : 8;
+  k.chunks = (G + k.nq - 1) / k.nq;
+  // enough splits that every SM holds several CTAs, none with less than a round of its warps.  Up to eight
+  // are a cluster (a power of two of them)
+  const int64_t units = (int64_t)B * NKV * k.chunks;
+  const int64_t want = ((int64_t)current_device_sms() * 6 + units - 1) / units;
+  const int most = L <= KD_SPLIT ? 1 : kd_most_splits(L);
+  int ns = (int)(want < most ? want : most);
+  k.cluster = ns > 1 && ns <= KD_CLUSTER;
+  if (k.cluster) {
+    int c = 2;
+    while (c < ns) c *= 2;
+    ns = c;
   }
+  const int tiles = (L + 63) / 64;
+  k.per = (tiles + ns - 1) / ns * 64;
+  k.ns = k.cluster ? ns : (L + k.per - 1) / k.per;
+  k.alone = k.cluster || k.ns == 1;
+  // where a key head's queries take more than one CTA (chunks), the combine kernel adds their weights
+  k.zsmem = weights && k.alone && k.chunks == 1 && k.nq * k.per <= KD_ZFLOATS;
+  k.states = k.alone ? (weights && k.chunks > 1 ? (size_t)B * NH * 2 : 0) : (size_t)B * NH * k.ns * (D + 2);
+  k.states = (k.states + 3) / 4 * 4;
+  k.scores = weights && !k.zsmem ? (size_t)B * NH * L : 0;
+  return k;
+}
+
+template <typename T, int D, int NQ>
+static int kv4_decode_q(const Kv4View& c, const Kv4Decode& p, int B, cudaStream_t s) {
+  using S = KdTile<D, NQ, sizeof(T) == 4>;
+  static_assert(S::BYTES + KD_ZFLOATS * 4 <= 227 * 1024, "shared memory");
   static CtxOnce attr;
-  if (!set_smem_limit_once(kv4_decode_kernel<T, D, NQ>, S::BYTES, attr)) return ATTN_ERR_CUDA;
+  if (!set_smem_limit_once(kv4_decode_kernel<T, D, NQ>, S::BYTES + KD_ZFLOATS * 4, attr)) return ATTN_ERR_CUDA;
+  const int64_t units = (int64_t)B * p.NKV * p.chunks;
   if (units * p.ns >= (int64_t)1 << 31) {
     set_error("attn_kv4_decode: B*NH*L is too large for one launch; split the batch into several calls");
     return ATTN_ERR_UNSUPPORTED;
   }
-  cudaError_t e = launch_pdl(kv4_decode_kernel<T, D, NQ>, dim3((unsigned)(units * p.ns)), dim3(KD_THREADS), S::BYTES, s, c, p);
+  const dim3 grid((unsigned)(units * p.ns)), block(KD_THREADS);
+  const size_t smem = S::BYTES + (p.zsmem ? (size_t)NQ * p.per * 4 : 0);
+  cudaError_t e = p.cluster ? launch_pdl_cluster(kv4_decode_kernel<T, D, NQ>, p.ns, grid, block, smem, s, c, p)
+                            : launch_pdl(kv4_decode_kernel<T, D, NQ>, grid, block, smem, s, c, p);
   count_launch();
   if (int rc = check_launch("kv4_decode_kernel", e)) return rc;
-  if (p.ns == 1) return ATTN_OK;
-  const int wc = p.scores ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
+  if (p.alone && !(p.weights && p.chunks > 1)) return ATTN_OK;
+  const int wc = p.weights ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
   e = launch_pdl(kv4_decode_combine_kernel<T, D>, dim3((unsigned)wc * B * p.NKV), dim3(KD_THREADS), 0, s, p);
   count_launch();
   return check_launch("kv4_decode_combine_kernel", e);
 }
 
 template <typename T, int D>
-static int kv4_decode_d(const Kv4View& c, const Kv4Decode& p, int B, int sms, cudaStream_t s) {
-  // a product has eight columns: eight queries, or four float32 ones in two parts each
-  if (p.G == 1) return kv4_decode_q<T, D, 1>(c, p, B, sms, s);
-  if (p.G == 2) return kv4_decode_q<T, D, 2>(c, p, B, sms, s);
-  if (sizeof(T) == 4 || p.G <= 4) return kv4_decode_q<T, D, 4>(c, p, B, sms, s);
-  return kv4_decode_q<T, D, sizeof(T) == 4 ? 4 : 8>(c, p, B, sms, s);
+static int kv4_decode_d(const Kv4View& c, const Kv4Decode& p, int B, cudaStream_t s) {
+  switch (p.nq) {
+    case 1: return kv4_decode_q<T, D, 1>(c, p, B, s);
+    case 2: return kv4_decode_q<T, D, 2>(c, p, B, s);
+    case 4: return kv4_decode_q<T, D, 4>(c, p, B, s);
+  }
+  return kv4_decode_q<T, D, sizeof(T) == 4 ? 4 : 8>(c, p, B, s);
 }
 
 template <typename T>
-static int kv4_decode_t(const Kv4View& c, const Kv4Decode& p, int B, int D, int sms, cudaStream_t s) {
+static int kv4_decode_t(const Kv4View& c, const Kv4Decode& p, int B, int D, cudaStream_t s) {
   switch (D) {
-    case 16: return kv4_decode_d<T, 16>(c, p, B, sms, s);
-    case 32: return kv4_decode_d<T, 32>(c, p, B, sms, s);
-    case 64: return kv4_decode_d<T, 64>(c, p, B, sms, s);
-    case 128: return kv4_decode_d<T, 128>(c, p, B, sms, s);
+    case 16: return kv4_decode_d<T, 16>(c, p, B, s);
+    case 32: return kv4_decode_d<T, 32>(c, p, B, s);
+    case 64: return kv4_decode_d<T, 64>(c, p, B, s);
+    case 128: return kv4_decode_d<T, 128>(c, p, B, s);
   }
   return ATTN_ERR_UNSUPPORTED;
 }
@@ -709,9 +784,10 @@ static int kv4_decode_t(const Kv4View& c, const Kv4Decode& p, int B, int D, int 
 
 using namespace attn;
 
-extern "C" size_t attn_kv4_decode_workspace_size(int B, int NH, int L, int D, int weights) {
-  if (B <= 0 || NH <= 0 || L <= 0 || D <= 0) return 0;
-  return (kd_states((int64_t)B * NH, L, D) + (weights ? (size_t)B * NH * L : 0)) * sizeof(float);
+extern "C" size_t attn_kv4_decode_workspace_size(int B, int NH, int NKV, int L, int D, int dtype, int weights) {
+  if (B <= 0 || NH <= 0 || NKV <= 0 || NH % NKV || L <= 0 || D <= 0) return 0;
+  const KdPlan k = kd_plan(B, NH, NKV, L, D, dtype, weights);
+  return (k.states + k.scores) * sizeof(float);
 }
 
 extern "C" int attn_kv4_decode(const void* q, const void* codes, const void* params, void* o, float* lse, int B, int NH,
@@ -728,8 +804,9 @@ extern "C" int attn_kv4_decode(const void* q, const void* codes, const void* par
   ATTN_REQUIRE(L > 0 && L <= capacity, "attn_kv4_decode: length %d outside 1 .. capacity %d", L, capacity);
   ATTN_REQUIRE(q_sb >= 0 && q_sh >= 0 && o_sb >= 0 && o_sh >= 0 && w_sb >= 0 && w_sh >= 0, "attn_kv4_decode: strides must not be negative");
   ATTN_REQUIRE(!weights_in || weights_out, "attn_kv4_decode: weights_in needs weights_out");
-  const size_t need = attn_kv4_decode_workspace_size(B, NH, L, D, weights_out != nullptr);
-  if (!workspace || workspace_bytes < need) {
+  const KdPlan k = kd_plan(B, NH, NKV, L, D, dtype, weights_out != nullptr);
+  const size_t need = (k.states + k.scores) * sizeof(float);
+  if (need && (!workspace || workspace_bytes < need)) {
     set_error("attn_kv4_decode: workspace of %zu bytes required", need);
     return ATTN_ERR_WORKSPACE;
   }
@@ -738,11 +815,11 @@ extern "C" int attn_kv4_decode(const void* q, const void* codes, const void* par
   p.q = q; p.o = o; p.lse = lse; p.lengths = lengths; p.w_in = weights_in; p.w_out = weights_out;
   p.q_sb = q_sb; p.q_sh = q_sh; p.o_sb = o_sb; p.o_sh = o_sh; p.w_sb = w_sb; p.w_sh = w_sh;
   p.NH = NH; p.NKV = NKV; p.G = NH / NKV; p.L = L;
-  p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.nq = k.nq; p.chunks = k.chunks; p.ns = k.ns; p.per = k.per; p.cluster = k.cluster; p.alone = k.alone; p.zsmem = k.zsmem;
+  p.weights = weights_out != nullptr;
   p.states = (float*)workspace;
-  p.scores = weights_out ? p.states + kd_states((int64_t)B * NH, L, D) : nullptr;
-  const int sms = current_device_sms();
-  return dtype == ATTN_BF16 ? kv4_decode_t<__nv_bfloat16>(c, p, B, D, sms, as_stream(stream))
-                            : kv4_decode_t<float>(c, p, B, D, sms, as_stream(stream));
+  p.scores = k.scores ? p.states + k.states : nullptr;
+  return dtype == ATTN_BF16 ? kv4_decode_t<__nv_bfloat16>(c, p, B, D, as_stream(stream))
+                            : kv4_decode_t<float>(c, p, B, D, as_stream(stream));
 }

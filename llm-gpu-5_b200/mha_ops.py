@@ -313,11 +313,13 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
             raise ValueError("kv4_decode: weights and weights_out must have the same strides")
         wsb, wsh = osb, osh
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
-    workspace, ws, ws_bytes = _scratch(workspace, lib.attn_kv4_decode_workspace_size(B, NH, length, D, w_out is not None), q)
+    code = dtype_code(q.dtype)
+    need = lib.attn_kv4_decode_workspace_size(B, NH, NKV, length, D, code, w_out is not None)
+    workspace, ws, ws_bytes = _scratch(workspace, need, q)
     _call_on(dev, "attn_kv4_decode", q.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(),
              lse.data_ptr() if lse is not None else None, B, NH, NKV, length, D, qs[0], qs[1], os_[0], os_[1], si, sb, sh,
              cap, lengths_p, w_in, w_out, wsb, wsh, 1.0 / math.sqrt(D) if scale is None else float(scale),
-             dtype_code(q.dtype), ws, ws_bytes)
+             code, ws, ws_bytes)
     return out
 
 

@@ -54,6 +54,9 @@ def _evict(**kw):
     return _lib().attn_kv4_evict(*a.values())
 
 
+# one head over many rows: more splits than a cluster holds
+LONG = dict(B=1, NH=1, NKV=1, L=32768, cap=32768, c_sh=32768, c_sb=32768, c_si=32768)
+
 CACHE = [
     (dict(codes=None), ARG, "null"), (dict(params=None), ARG, "null"), (dict(D=48), UNSUPPORTED, "head_dim"),
     (dict(D=8), UNSUPPORTED, "head_dim"), (dict(D=256), UNSUPPORTED, "head_dim"), (dict(cap=17), ARG, "multiples of 16"),
@@ -84,7 +87,7 @@ def test_bad_caches_are_refused(call, bad, code, text):
     (_decode, dict(q=None), ARG, "null"), (_decode, dict(o=None), ARG, "null"), (_decode, dict(dtype=2), ARG, "dtype"),
     (_decode, dict(NH=3), ARG, "multiple"), (_decode, dict(NKV=0), ARG, "multiple"), (_decode, dict(L=0), ARG, "length"),
     (_decode, dict(L=17), ARG, "length"), (_decode, dict(q_sb=-1), ARG, "negative"), (_decode, dict(w_in=FAKE), ARG, "weights_out"),
-    (_decode, dict(ws=None), WORKSPACE, "workspace"), (_decode, dict(ws_bytes=16), WORKSPACE, "workspace"),
+    (_decode, dict(ws=None, **LONG), WORKSPACE, "workspace"), (_decode, dict(ws_bytes=16, **LONG), WORKSPACE, "workspace"),
     (_decode, dict(ws=FAKE + 4), ARG, "aligned"),
     (_weights, dict(q=None), ARG, "null"), (_weights, dict(w_out=None), ARG, "null"), (_weights, dict(dtype=5), ARG, "dtype"),
     (_weights, dict(NH=3), ARG, "multiple"), (_weights, dict(first=-1), ARG, "first_query"), (_weights, dict(T=0), ARG, "positive"),
@@ -107,7 +110,8 @@ def test_bad_arguments_are_refused(call, bad, code, text):
 
 def test_workspace_sizes_of_nothing():
     L = _lib()
-    assert L.attn_kv4_decode_workspace_size(0, 8, 10, 64, 1) == 0
+    assert L.attn_kv4_decode_workspace_size(0, 8, 8, 10, 64, 1, 1) == 0
+    assert L.attn_kv4_decode_workspace_size(1, 8, 3, 10, 64, 1, 1) == 0
     assert L.attn_kv4_evict_workspace_size(1, 8, 10, 0) == 0
 
 
