@@ -622,78 +622,87 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   if (p.cluster) cluster_sync();  // the others may still read this CTA's state
 }
 
-__device__ __forceinline__ float block_reduce(float v, float* red, bool is_max) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float u = __shfl_xor_sync(0xffffffffu, v, off);
-    v = is_max ? fmaxf(v, u) : v + u;
-  }
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < KD_THREADS / 32; ++i) v = is_max ? fmaxf(v, red[i]) : v + red[i];
-  return v;
-}
-
-// One CTA per (KD_WCHUNK keys, sequence, key head); the first of them also writes o and lse.
+// Merge the splits' states and add the weights: a CTA takes KD_WCHUNK keys of one (sequence, key head), and
+// its share of the outputs.  A warp finds a head's maximum and sum, the splits on its lanes, so that a call
+// waits for memory three times, not once per head and split.
+constexpr int KC_THREADS = 256;
+constexpr int KC_HEADS = 32;  // query heads at a time
 template <typename T, int D>
-__global__ void __launch_bounds__(KD_THREADS) kv4_decode_combine_kernel(const Kv4Decode p) {
-  __shared__ float red[KD_THREADS / 32];
+__global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv4Decode p) {
+  __shared__ float smx[KC_HEADS], sinv[KC_HEADS];
   grid_dependency_wait();
   grid_dependents_launch();
   const int wchunks = p.weights ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
   const int bk = blockIdx.x / wchunks, chunk = blockIdx.x % wchunks;
   const int b = bk / p.NKV, kvh = bk % p.NKV;
   const int n = seq_length(p.lengths, b, p.L);
-  const int j0 = chunk * KD_WCHUNK, j1 = min(p.L, j0 + KD_WCHUNK);
-  constexpr int PER = KD_WCHUNK / KD_THREADS;
-  float w[PER];
+  const int j0 = chunk * KD_WCHUNK + threadIdx.x;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  constexpr int PER = KD_WCHUNK / KC_THREADS;
+  const int64_t bh0 = (int64_t)b * p.NH + kvh * p.G, w0 = b * p.w_sb + kvh * p.w_sh;
+  float w[PER], have[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) w[i] = 0.f;
-  for (int g = 0; g < p.G; ++g) {
-    const int h = kvh * p.G + g;
-    const int64_t bh = (int64_t)b * p.NH + h;
-    float mx, sum;
-    if (p.alone) {
-      mx = p.states[bh * 2];
-      sum = p.states[bh * 2 + 1];
-    } else {
-      const float* st = p.states + bh * p.ns * (D + 2);
-      mx = -INFINITY;
-      sum = 0.f;
-      for (int i = threadIdx.x; i < p.ns; i += KD_THREADS) mx = fmaxf(mx, st[(int64_t)i * (D + 2)]);
-      mx = block_reduce(mx, red, true);
-      if (mx == -INFINITY) mx = 0.f;
-      for (int i = threadIdx.x; i < p.ns; i += KD_THREADS)
-        sum += st[(int64_t)i * (D + 2) + 1] * ex2(st[(int64_t)i * (D + 2)] - mx);
-      sum = block_reduce(sum, red, false);
-      if (chunk == 0) {
-        for (int d = threadIdx.x; d < D; d += KD_THREADS) {
-          float acc = 0.f;
-          for (int i = 0; i < p.ns; ++i) acc += st[(int64_t)i * (D + 2) + 2 + d] * ex2(st[(int64_t)i * (D + 2)] - mx);
-          Elem<T>::store((T*)p.o + b * p.o_sb + h * p.o_sh + d, sum > 0.f || sum != sum ? acc / sum : 0.f);
+  for (int i = 0; i < PER; ++i) {
+    const int j = j0 + i * KC_THREADS;
+    w[i] = 0.f;
+    have[i] = p.weights && p.w_in && j < p.L ? p.w_in[w0 + j] : 0.f;
+  }
+  for (int g0 = 0; g0 < p.G; g0 += KC_HEADS) {
+    const int heads = min(KC_HEADS, p.G - g0);
+    __syncthreads();
+    for (int g = warp; g < heads; g += KC_THREADS / 32) {
+      const int64_t bh = bh0 + g0 + g;
+      float mx, sum;
+      if (p.alone) {
+        mx = p.states[bh * 2];
+        sum = p.states[bh * 2 + 1];
+      } else {
+        const float* st = p.states + bh * p.ns * (D + 2);
+        float m = -INFINITY, l = 0.f;  // of this lane's splits
+        for (int i = lane; i < p.ns; i += 32) {
+          const float a = st[(int64_t)i * (D + 2)], c = st[(int64_t)i * (D + 2) + 1];
+          const float nm = fmaxf(m, a), ref = nm == -INFINITY ? 0.f : nm;
+          l = fmaf(l, ex2(m - ref), c * ex2(a - ref));
+          m = nm;
         }
-        if (threadIdx.x == 0 && p.lse) p.lse[bh] = kd_lse(mx, sum);
+        mx = warp_max(m);
+        if (mx == -INFINITY) mx = 0.f;
+        sum = warp_sum(l * ex2(m - mx));
+      }
+      if (lane == 0) {
+        smx[g] = mx;
+        sinv[g] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        if (!p.alone && chunk == 0 && p.lse) p.lse[bh] = kd_lse(mx, sum);
+      }
+    }
+    __syncthreads();
+    if (!p.alone) {
+      for (int i = chunk * KC_THREADS + threadIdx.x; i < heads * D; i += wchunks * KC_THREADS) {
+        const int g = i / D, d = i % D;
+        const float* st = p.states + (bh0 + g0 + g) * p.ns * (D + 2);
+        float o = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < p.ns; ++k) o = fmaf(st[(int64_t)k * (D + 2) + 2 + d], ex2(st[(int64_t)k * (D + 2)] - smx[g]), o);
+        Elem<T>::store((T*)p.o + b * p.o_sb + (kvh * p.G + g0 + g) * p.o_sh + d, o * sinv[g]);
       }
     }
     if (p.weights) {
-      const float inv = 1.f / sum;
+      for (int g = 0; g < heads; ++g) {
+        const float* z = p.scores + (bh0 + g0 + g) * p.L;
+        const float mx = smx[g], inv = sinv[g];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int j = j0 + i * KD_THREADS + threadIdx.x;
-        if (j < j1 && j < n) w[i] += ex2(p.scores[bh * p.L + j] - mx) * inv;
+        for (int i = 0; i < PER; ++i) {
+          const int j = j0 + i * KC_THREADS;
+          if (j < n) w[i] = fmaf(ex2(z[j] - mx), inv, w[i]);
+        }
       }
     }
   }
   if (p.weights) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int j = j0 + i * KD_THREADS + threadIdx.x;
-      if (j < j1) {
-        const int64_t at = b * p.w_sb + kvh * p.w_sh + j;
-        p.w_out[at] = (p.w_in ? p.w_in[at] : 0.f) + w[i];
-      }
+      const int j = j0 + i * KC_THREADS;
+      if (j < p.L) p.w_out[w0 + j] = have[i] + w[i];
     }
   }
 }
@@ -711,18 +720,20 @@ static KdPlan kd_plan(int B, int NH, int NKV, int L, int D, int dtype, int weigh
   const int most_q = dtype == ATTN_F32 ? 4 : 8;
   k.nq = G == 1 ? 1 : G == 2 ? 2 : G <= 4 || most_q == 4 ? 4 : 8;
   k.chunks = (G + k.nq - 1) / k.nq;
-  // enough splits that every SM holds several CTAs, none with less than a round of its warps.  Up to eight
-  // are a cluster (a power of two of them)
+  // about seven CTAs for every SM, none with less than a round of its warps: measured for 384, 512 and 128 units,
+  // ns = 3, 2 and 8 took 117, 22 and 50 us, half as many 129, 25 and 59, twice as many 115, 24 and 59.  Where the
+  // GPU holds them all at once they form clusters, a power of two of CTAs up to eight, and the call is one
+  // launch (64 units of 4,099 keys: 18 us against 22); with more CTAs than that, clusters wait for room
+  // (384 units: 137 us against 117)
   const int64_t units = (int64_t)B * NKV * k.chunks;
-  const int64_t want = ((int64_t)current_device_sms() * 6 + units - 1) / units;
+  const int sms = current_device_sms();
+  const int64_t want = ((int64_t)sms * 7 + units - 1) / units;
   const int most = L <= KD_SPLIT ? 1 : kd_most_splits(L);
   int ns = (int)(want < most ? want : most);
-  k.cluster = ns > 1 && ns <= KD_CLUSTER;
-  if (k.cluster) {
-    int c = 2;
-    while (c < ns) c *= 2;
-    ns = c;
-  }
+  int c = 2;
+  while (c < ns && c < KD_CLUSTER) c *= 2;
+  k.cluster = ns > 1 && c * units <= 4 * sms && ns <= 2 * KD_CLUSTER;
+  if (k.cluster) ns = c;
   const int tiles = (L + 63) / 64;
   k.per = (tiles + ns - 1) / ns * 64;
   k.ns = k.cluster ? ns : (L + k.per - 1) / k.per;
@@ -754,7 +765,7 @@ static int kv4_decode_q(const Kv4View& c, const Kv4Decode& p, int B, cudaStream_
   if (int rc = check_launch("kv4_decode_kernel", e)) return rc;
   if (p.alone && !(p.weights && p.chunks > 1)) return ATTN_OK;
   const int wc = p.weights ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
-  e = launch_pdl(kv4_decode_combine_kernel<T, D>, dim3((unsigned)wc * B * p.NKV), dim3(KD_THREADS), 0, s, p);
+  e = launch_pdl(kv4_decode_combine_kernel<T, D>, dim3((unsigned)wc * B * p.NKV), dim3(KC_THREADS), 0, s, p);
   count_launch();
   return check_launch("kv4_decode_combine_kernel", e);
 }
