@@ -38,7 +38,7 @@ namespace attn {
 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
-constexpr int KD_WCHUNK = 1024;  // keys per combine CTA
+constexpr int KD_WCHUNK = 2048;  // keys per combine CTA
 constexpr int KD_SPLIT = 64 * KD_WARPS;  // keys a CTA takes at least, where there are so many
 constexpr int KD_CLUSTER = 8;            // most CTAs of a cluster (the portable limit)
 
@@ -640,12 +640,15 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   constexpr int PER = KD_WCHUNK / KC_THREADS;
   const int64_t bh0 = (int64_t)b * p.NH + kvh * p.G, w0 = b * p.w_sb + kvh * p.w_sh;
-  float w[PER], have[PER];
+  // what does not depend on the states is asked for first: the sums so far, and the first head's scores
+  float w[PER], have[PER], z[PER];
+  const float* zrow = p.scores + bh0 * p.L + j0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int j = j0 + i * KC_THREADS;
     w[i] = 0.f;
     have[i] = p.weights && p.w_in && j < p.L ? p.w_in[w0 + j] : 0.f;
+    z[i] = p.weights && j < n ? zrow[i * KC_THREADS] : -INFINITY;
   }
   for (int g0 = 0; g0 < p.G; g0 += KC_HEADS) {
     const int heads = min(KC_HEADS, p.G - g0);
@@ -688,12 +691,14 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv
     }
     if (p.weights) {
       for (int g = 0; g < heads; ++g) {
-        const float* z = p.scores + (bh0 + g0 + g) * p.L;
         const float mx = smx[g], inv = sinv[g];
+        zrow += p.L;
+        const bool more = g0 + g + 1 < p.G;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int j = j0 + i * KC_THREADS;
-          if (j < n) w[i] = fmaf(ex2(z[j] - mx), inv, w[i]);
+          const float x = z[i];
+          z[i] = more && j0 + i * KC_THREADS < n ? zrow[i * KC_THREADS] : -INFINITY;  // of the next head
+          w[i] = fmaf(ex2(x - mx), inv, w[i]);
         }
       }
     }
