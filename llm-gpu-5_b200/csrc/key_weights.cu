@@ -11,17 +11,18 @@
 // MMA, so the special-function unit bounds it.  Two CTAs share an SM (256 TMEM columns each, two score
 // tiles), so that one's loads and hand-overs hide behind the other's exponentials.
 //
-// Other shapes and float32 run on CUDA cores: a thread takes one key and a CTA 128 of them; queries pass
-// through shared memory in tiles of 32 and a thread forms 8 scores at a time, so that each value of its key is
-// read once for 8 products.
+// Other shapes and float32 run on CUDA cores: a CTA takes 64 keys and streams the queries past them in tiles of
+// 64, a thread forms 4 x 4 scores (two 16-byte shared-memory reads for 16 products), and the 16 threads of a
+// key add up their sums at the end.
 #include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
 
 namespace attn {
 
-constexpr int KW_KEYS = 128;
-constexpr int KW_QUERIES = 32;
+constexpr int KW_TILE = 64;       // keys, and queries, of a CUDA-core tile
+constexpr int KW_LD = KW_TILE + 4;
+constexpr int KW_THREADS = 256;
 
 struct KeyWeights {
   const void *q, *k;
@@ -35,95 +36,12 @@ struct KeyWeights {
 
 __device__ __forceinline__ float tf32_cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
-template <typename T, bool TF32>
-__global__ void __launch_bounds__(KW_KEYS) key_weights_simt_kernel(const KeyWeights p) {
-  extern __shared__ float sm[];
-  float* sk = sm;                       // [D][KW_KEYS]
-  float* sq = sk + p.D * KW_KEYS;       // [KW_QUERIES][D]
-  float* sl = sq + KW_QUERIES * p.D;    // [KW_QUERIES]
-  grid_dependency_wait();
-  grid_dependents_launch();
-  const int ntile = (p.T + KW_KEYS - 1) / KW_KEYS;
-  const int bh = blockIdx.x / ntile, j0 = (blockIdx.x % ntile) * KW_KEYS;
-  const int b = bh / p.NKV, kvh = bh % p.NKV;
-  const int n = seq_length(p.lengths, b, p.T);
-  const int j = j0 + threadIdx.x;
-  const T* kb = (const T*)p.k + b * p.k_sb + kvh * p.k_sh;
-  for (int i = threadIdx.x; i < KW_KEYS * p.D; i += KW_KEYS) {
-    const int r = i / p.D, d = i - r * p.D;
-    float x = j0 + r < n ? Elem<T>::load(kb + (int64_t)(j0 + r) * p.k_st + d) : 0.f;
-    sk[d * KW_KEYS + r] = TF32 ? tf32_cut(x) : x;
-  }
-  float total = 0.f;
-  for (int g = 0; g < p.G; ++g) {
-    const int h = kvh * p.G + g;
-    const T* qb = (const T*)p.q + b * p.q_sb + h * p.q_sh;
-    const float* lse = p.lse + ((int64_t)b * p.NH + h) * p.T;
-    for (int i0 = max(j0, p.first); i0 < n; i0 += KW_QUERIES) {
-      __syncthreads();
-      for (int e = threadIdx.x; e < KW_QUERIES * p.D; e += KW_KEYS) {
-        const int r = e / p.D, d = e - r * p.D;
-        float x = i0 + r < n ? Elem<T>::load(qb + (int64_t)(i0 + r) * p.q_st + d) : 0.f;
-        sq[e] = TF32 ? tf32_cut(x) : x;
-      }
-      if (threadIdx.x < KW_QUERIES) sl[threadIdx.x] = i0 + threadIdx.x < n ? lse[i0 + threadIdx.x] * 1.4426950408889634f : 0.f;
-      __syncthreads();
-      for (int r0 = 0; r0 < KW_QUERIES; r0 += 8) {
-        float acc[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) acc[r] = 0.f;
-        for (int d = 0; d < p.D; ++d) {
-          const float x = sk[d * KW_KEYS + threadIdx.x];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) acc[r] += x * sq[(r0 + r) * p.D + d];
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const int i = i0 + r0 + r;
-          if (i < n && i >= j) total += exp2f(fmaf(acc[r], p.scale_log2, -sl[r0 + r]));
-        }
-      }
-    }
-  }
-  if (j < p.T) {
-    const int64_t at = b * p.w_sb + kvh * p.w_sh + j;
-    p.w_out[at] = (p.w_in ? p.w_in[at] : 0.f) + (j < n ? total : 0.f);
-  }
-}
-
-static int key_weights_simt(const KeyWeights& p, int B, int dtype, cudaStream_t s) {
-  const size_t smem = ((size_t)p.D * (KW_KEYS + KW_QUERIES) + KW_QUERIES) * sizeof(float);
-  const int64_t grid = (int64_t)B * p.NKV * ((p.T + KW_KEYS - 1) / KW_KEYS);
-  auto kern = dtype == ATTN_BF16 ? key_weights_simt_kernel<__nv_bfloat16, false>
-              : dtype == ATTN_TF32 ? key_weights_simt_kernel<float, true> : key_weights_simt_kernel<float, false>;
-  ATTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const cudaError_t e = launch_pdl(kern, dim3((unsigned)grid), dim3(KW_KEYS), smem, s, p);
-  count_launch();
-  return check_launch("key_weights_simt_kernel", e);
-}
-
-
-// ---- tensor cores ------------------------------------------------------------------------------
-constexpr int KT_STAGES = 3;                 // query tiles in flight
-constexpr int KT_THREADS = 192;              // 4 warps of sums, a TMA warp, an MMA warp
-constexpr int KT_TMEM = 256;                 // two 128-column score tiles
-constexpr int KT_SMEM = 1024 + (2 + KT_STAGES) * AT_TILE_BYTES + 4 * 2 * AT_TILE * 4 + 256;
-
-struct KwMaps {
-  TileMap q, k;
-};
-
-struct KwTc {
+struct KwWork {
   KeyWeights p;
   int nt, parts, BK, units;  // key tiles, parts of a key tile's queries, B*NKV
   FastDiv by_bk, by_nkv, by_parts;
   float* partial;            // [parts][B*NKV][T] when parts > 1
   int* err;
-};
-
-struct KwBars {
-  uint64_t k_full[2], k_empty[2], q_full[KT_STAGES], q_empty[KT_STAGES], s_full[2], s_free[2];
-  uint32_t tmem;
 };
 
 // One unit of work: key tile jt of (b, kvh), query tiles [lo, lo + span) of each of the G query heads in
@@ -132,20 +50,24 @@ struct KwBars {
 // come to 30 .. 33 tiles a CTA, dealt round and round to 27 .. 35.
 struct KwUnit {
   int b, kvh, jt, part, n, lo, span, begin, end;
-  __device__ __forceinline__ bool set(const KwTc& a, int round) {
+  __device__ __forceinline__ bool set(const KwWork& a, int round) {
     const int u = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     if (u >= a.units) {
       begin = end = 0;
       return false;
     }
+    open(a, u, AT_TILE);
+    return true;
+  }
+  __device__ __forceinline__ void open(const KwWork& a, int u, int tile) {
     const uint32_t level = a.by_bk.div(u), bk = u - level * a.BK;
     jt = a.by_parts.div(level);
     part = level - jt * a.parts;
     b = a.by_nkv.div(bk);
     kvh = bk - b * a.p.NKV;
     n = seq_length(a.p.lengths, b, a.p.T);
-    lo = max(jt, a.p.first / AT_TILE);
-    span = max((n + AT_TILE - 1) / AT_TILE - lo, 0);
+    lo = max(jt, a.p.first / tile);
+    span = max((n + tile - 1) / tile - lo, 0);
     const int total = span * a.p.G;
     begin = 0;
     end = total;
@@ -153,7 +75,6 @@ struct KwUnit {
       begin = (int)((int64_t)total * part / a.parts);
       end = (int)((int64_t)total * (part + 1) / a.parts);
     }
-    return true;
   }
 };
 
@@ -172,23 +93,124 @@ struct KwSteps {
   }
 };
 
+// The sum of key j of a unit: an output, or a part of one.
+__device__ __forceinline__ void kw_write(const KwWork& a, const KwUnit& w, int j, float sum) {
+  if (a.parts > 1) {
+    a.partial[((int64_t)w.part * a.BK + (int64_t)w.b * a.p.NKV + w.kvh) * a.p.T + j] = sum;
+  } else {
+    const int64_t at = w.b * a.p.w_sb + w.kvh * a.p.w_sh + j;
+    a.p.w_out[at] = (a.p.w_in ? a.p.w_in[at] : 0.f) + sum;
+  }
+}
+
+// Rows [r0, r0 + 64) of a head, rows past `rows` as zeros, into sm[d][row]; four rows of one element group at a time.
+template <typename T, bool TF32>
+__device__ __forceinline__ void kw_load_tile(float* sm, const T* base, int64_t st, int r0, int rows, int D) {
+  for (int e = threadIdx.x; e < KW_TILE * D; e += KW_THREADS) {
+    const int r = e / D, d = e - r * D;  // consecutive threads read consecutive elements
+    const float x = r0 + r < rows ? Elem<T>::load(base + (int64_t)(r0 + r) * st + d) : 0.f;
+    sm[d * KW_LD + r] = TF32 ? tf32_cut(x) : x;
+  }
+}
+
+template <typename T, bool TF32>
+__global__ void __launch_bounds__(KW_THREADS) key_weights_simt_kernel(const KwWork a) {
+  const KeyWeights& p = a.p;
+  extern __shared__ __align__(16) float sm[];
+  float* sk = sm;                    // [D][KW_LD]
+  float* sq = sk + p.D * KW_LD;      // [D][KW_LD]
+  float* sl = sq + p.D * KW_LD;      // [KW_TILE] -lse in log2 units
+  grid_dependency_wait();
+  grid_dependents_launch();
+  KwUnit w;
+  w.open(a, blockIdx.x, KW_TILE);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // queries 4 tx.., keys 4 ty..
+  const int j0 = w.jt * KW_TILE;
+  if (w.begin < w.end)
+    kw_load_tile<T, TF32>(sk, (const T*)p.k + w.b * p.k_sb + w.kvh * p.k_sh, p.k_st, j0, w.n, p.D);
+  float total[4] = {0.f, 0.f, 0.f, 0.f};
+  KwSteps st;
+  st.start(w);
+  for (int i = w.begin; i < w.end; ++i, st.next(w)) {
+    const int h = w.kvh * p.G + st.g, i0 = st.it * KW_TILE;
+    __syncthreads();
+    kw_load_tile<T, TF32>(sq, (const T*)p.q + w.b * p.q_sb + h * p.q_sh, p.q_st, i0, w.n, p.D);
+    if (threadIdx.x < KW_TILE)
+      sl[threadIdx.x] = i0 + threadIdx.x < w.n ? p.lse[((int64_t)w.b * p.NH + h) * p.T + i0 + threadIdx.x] * -1.4426950408889634f : 0.f;
+    __syncthreads();
+    float acc[4][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[x][y] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < p.D; ++d) {
+      const float4 kv = *reinterpret_cast<const float4*>(sk + d * KW_LD + 4 * ty);
+      const float4 qv = *reinterpret_cast<const float4*>(sq + d * KW_LD + 4 * tx);
+      const float k4[4] = {kv.x, kv.y, kv.z, kv.w}, q4[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = fmaf(k4[x], q4[y], acc[x][y]);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      float sum = 0.f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int q = i0 + 4 * tx + y;
+        const bool use = q < w.n && q >= p.first && q >= j0 + 4 * ty + x;
+        const float e = exp2f(fmaf(acc[x][y], p.scale_log2, sl[4 * tx + y]));
+        sum += use ? e : 0.f;
+      }
+      total[x] += sum;
+    }
+  }
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) total[x] += __shfl_xor_sync(0xffffffffu, total[x], off);
+  if (tx < 4) {  // thread tx of a key group writes key tx
+    const int j = j0 + 4 * ty + tx;
+    if (j < p.T) {
+      const float mine = tx == 0 ? total[0] : tx == 1 ? total[1] : tx == 2 ? total[2] : total[3];
+      kw_write(a, w, j, j < w.n ? mine : 0.f);
+    }
+  }
+}
+
+// ---- tensor cores ------------------------------------------------------------------------------
+constexpr int KT_STAGES = 3;                 // query tiles in flight
+constexpr int KT_THREADS = 192;              // 4 warps of sums, a TMA warp, an MMA warp
+constexpr int KT_TMEM = 256;                 // two 128-column score tiles
+constexpr int KT_SMEM = 1024 + (2 + KT_STAGES) * AT_TILE_BYTES + 4 * 2 * AT_TILE * 4 + 256;
+
+struct KwMaps {
+  TileMap q, k;
+};
+
+struct KwBars {
+  uint64_t k_full[2], k_empty[2], q_full[KT_STAGES], q_empty[KT_STAGES], s_full[2], s_free[2];
+  uint32_t tmem;
+};
+
 // All query tiles of a CTA's units in order.
 struct KwTiles {
   KwUnit w;
   KwSteps st;
   int i, round;
   bool more;
-  __device__ __forceinline__ void open(const KwTc& a) {  // the first tile of the next unit that has one
+  __device__ __forceinline__ void open(const KwWork& a) {  // the first tile of the next unit that has one
     do more = w.set(a, round++);
     while (more && w.begin >= w.end);
     i = w.begin;
     if (more) st.start(w);
   }
-  __device__ __forceinline__ void start(const KwTc& a) {
+  __device__ __forceinline__ void start(const KwWork& a) {
     round = 0;
     open(a);
   }
-  __device__ __forceinline__ void next(const KwTc& a) {
+  __device__ __forceinline__ void next(const KwWork& a) {
     st.next(w);
     if (++i == w.end) open(a);
   }
@@ -221,7 +243,7 @@ __device__ __forceinline__ void drain_load(uint64_t* bar, uint32_t parity) {
 
 template <bool TF32>
 __global__ void __launch_bounds__(KT_THREADS, 2)
-key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwTc a) {
+key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = smem;                                   // [2]
@@ -414,7 +436,7 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwTc a) {
   }
 }
 
-__global__ void __launch_bounds__(256) key_weights_join_kernel(const KwTc a) {
+__global__ void __launch_bounds__(256) key_weights_join_kernel(const KwWork a) {
   grid_dependency_wait();
   grid_dependents_launch();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -426,13 +448,53 @@ __global__ void __launch_bounds__(256) key_weights_join_kernel(const KwTc a) {
   a.p.w_out[at] = (a.p.w_in ? a.p.w_in[at] : 0.f) + sum;
 }
 
-// Parts that a key tile's queries are cut into: one while there are four units for every CTA.
-static int key_weights_parts(int B, int NKV, int T) {
-  const int64_t units = (int64_t)B * NKV * ((T + AT_TILE - 1) / AT_TILE);
-  const int64_t want = 4 * 2 * 148;
+// Parts that a key tile's queries are cut into: one while there are about two units for every CTA the GPU holds,
+// and none of fewer than four query tiles (the parts cost a second launch, as long as a tile or two).
+static int key_weights_parts(int B, int NKV, int T, int tile, int ctas) {
+  const int64_t tiles = (T + tile - 1) / tile, units = (int64_t)B * NKV * tiles, want = 4ll * ctas;
   if (units >= want / 2) return 1;
-  const int64_t parts = (want + units - 1) / units, most = (T + AT_TILE - 1) / AT_TILE;
+  const int64_t parts = (want + units - 1) / units;
+  const int64_t most = tiles / 4 > 1 ? tiles / 4 : 1;
   return (int)(parts < most ? parts : most);
+}
+constexpr int KW_CTAS = 2 * 148;  // CTAs that share the work, of either kernel
+
+// What both kernels take beside the arguments.
+static KwWork kw_work(const KeyWeights& p, int B, int tile, float* partial) {
+  KwWork a;
+  a.p = p;
+  a.nt = (p.T + tile - 1) / tile;
+  a.parts = key_weights_parts(B, p.NKV, p.T, tile, KW_CTAS);
+  a.BK = B * p.NKV;
+  a.units = a.BK * a.nt * a.parts;
+  a.by_bk.set(a.BK);
+  a.by_nkv.set(p.NKV);
+  a.by_parts.set(a.parts);
+  a.partial = partial;
+  a.err = nullptr;
+  return a;
+}
+
+static int key_weights_join(const KwWork& a, cudaStream_t s) {
+  if (a.parts == 1) return ATTN_OK;
+  const int64_t n = (int64_t)a.BK * a.p.T;
+  const cudaError_t e = launch_pdl(key_weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+  count_launch();
+  return check_launch("key_weights_join_kernel", e);
+}
+
+static int key_weights_simt(const KeyWeights& p, int B, int dtype, float* partial, cudaStream_t s) {
+  const size_t smem = ((size_t)2 * p.D * KW_LD + KW_TILE) * sizeof(float);
+  static CtxOnce attr[3];
+  const int which = dtype == ATTN_BF16 ? 0 : dtype == ATTN_TF32 ? 1 : 2;
+  auto kern = which == 0 ? key_weights_simt_kernel<__nv_bfloat16, false>
+              : which == 1 ? key_weights_simt_kernel<float, true> : key_weights_simt_kernel<float, false>;
+  if (!set_smem_limit_once(kern, (2 * 128 * KW_LD + KW_TILE) * 4, attr[which])) return ATTN_ERR_CUDA;
+  const KwWork a = kw_work(p, B, KW_TILE, partial);
+  const cudaError_t e = launch_pdl(kern, dim3((unsigned)a.units), dim3(KW_THREADS), smem, s, a);
+  count_launch();
+  if (int rc = check_launch("key_weights_simt_kernel", e)) return rc;
+  return key_weights_join(a, s);
 }
 
 static bool key_weights_tc_ok(const KeyWeights& p, int dtype) {
@@ -456,21 +518,11 @@ static int key_weights_tc(const KeyWeights& p, int B, int tf32, float* partial, 
              !make_head_map(&maps.k, p.k, B, p.NKV, p.T, p.D, p.k_sb, p.k_st, p.k_sh)) {
     return ATTN_ERR_CUDA;
   }
-  KwTc a;
-  a.p = p;
-  a.nt = (p.T + AT_TILE - 1) / AT_TILE;
-  a.parts = key_weights_parts(B, p.NKV, p.T);
-  a.BK = B * p.NKV;
-  const int64_t units = (int64_t)a.BK * a.nt * a.parts;
-  a.units = (int)units;
-  a.partial = partial;
-  a.by_bk.set(a.BK);
-  a.by_nkv.set(p.NKV);
-  a.by_parts.set(a.parts);
+  KwWork a = kw_work(p, B, AT_TILE, partial);
   a.err = dev_error_ptr();
   if (!a.err) return ATTN_ERR_CUDA;
   const int64_t ctas = 2 * (int64_t)current_device_sms();
-  const unsigned grid = (unsigned)(units < ctas ? units : ctas);
+  const unsigned grid = (unsigned)(a.units < ctas ? a.units : ctas);
   static CtxOnce attr[2];
   if (!(tf32 ? set_smem_limit_once(key_weights_tc_kernel<true>, KT_SMEM, attr[1])
              : set_smem_limit_once(key_weights_tc_kernel<false>, KT_SMEM, attr[0])))
@@ -479,11 +531,7 @@ static int key_weights_tc(const KeyWeights& p, int B, int tf32, float* partial, 
                        : launch_pdl(key_weights_tc_kernel<false>, dim3(grid), dim3(KT_THREADS), KT_SMEM, s, maps, a);
   count_launch();
   if (int rc = check_launch("key_weights_tc_kernel", e)) return rc;
-  if (a.parts == 1) return ATTN_OK;
-  const int64_t n = (int64_t)a.BK * p.T;
-  e = launch_pdl(key_weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
-  count_launch();
-  return check_launch("key_weights_join_kernel", e);
+  return key_weights_join(a, s);
 }
 
 }  // namespace attn
@@ -492,7 +540,9 @@ using namespace attn;
 
 extern "C" size_t attn_key_weights_workspace_size(int B, int NKV, int T) {
   if (B <= 0 || NKV <= 0 || T <= 0) return 0;
-  const int parts = key_weights_parts(B, NKV, T);
+  // whichever kernel the tensors suit
+  const int tc = key_weights_parts(B, NKV, T, AT_TILE, KW_CTAS), simt = key_weights_parts(B, NKV, T, KW_TILE, KW_CTAS);
+  const int parts = tc > simt ? tc : simt;
   return parts > 1 ? (size_t)parts * B * NKV * T * sizeof(float) : 0;
 }
 
@@ -515,7 +565,7 @@ extern "C" int attn_key_weights(const void* q, const void* k, const float* lse, 
     set_error("attn_key_weights: head_dim %d not supported (up to 128)", D);
     return ATTN_ERR_UNSUPPORTED;
   }
-  if ((int64_t)B * NKV * ((T + KW_KEYS - 1) / KW_KEYS) >= (int64_t)1 << 30) {
+  if ((int64_t)B * NKV * ((T + KW_TILE - 1) / KW_TILE) >= (int64_t)1 << 30) {
     set_error("attn_key_weights: too many key tiles for one launch; split the batch into several calls");
     return ATTN_ERR_UNSUPPORTED;
   }
@@ -528,5 +578,5 @@ extern "C" int attn_key_weights(const void* q, const void* k, const float* lse, 
   }
   ATTN_REQUIRE(aligned(workspace, 4), "attn_key_weights: misaligned workspace");
   if (key_weights_tc_ok(p, dtype)) return key_weights_tc(p, B, dtype == ATTN_TF32, (float*)workspace, as_stream(stream));
-  return key_weights_simt(p, B, dtype, as_stream(stream));
+  return key_weights_simt(p, B, dtype, (float*)workspace, as_stream(stream));
 }

@@ -9,11 +9,12 @@ the kernels here choose their own tiling.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
-from ._lib import ATTN_ACT_GELU, ATTN_ACT_GELU_BWD, ATTN_ACT_NONE, ATTN_BF16, ATTN_F32, ATTN_TF32, call, lib  # noqa: F401
+from ._lib import ATTN_ACT_GELU, ATTN_ACT_GELU_BWD, ATTN_ACT_NONE, ATTN_BF16, ATTN_F32, ATTN_TF32, AttnError, call, last_error, lib  # noqa: F401
 
 THREADS_PER_BLOCK = 256
 SOFTMAX_BLOCK_THREADS = 64
@@ -151,39 +152,48 @@ def kv4_empty(B: int, NH: int, capacity: int, D: int, device="cuda"):
             torch.empty((2, B, NH, cap, kv4_groups(D), 2), dtype=torch.float16, device=device))
 
 
+# The checks below run once per call of operators whose kernels take a few microseconds for a token: they
+# unpack shapes and strides once and compare dtypes by identity.
+_U8, _F16, _F32, _I32 = torch.uint8, torch.float16, torch.float32, torch.int32
+
+
 def _kv4_view(codes: torch.Tensor, params: torch.Tensor):
     """(B, NH, cap, D, strides in rows) of a cache's two arrays, checked."""
-    if codes.dtype != torch.uint8 or params.dtype != torch.float16:
+    if codes.dtype is not _U8 or params.dtype is not _F16:
         raise TypeError(f"4-bit cache: codes must be uint8 and params float16, got {codes.dtype} and {params.dtype}")
-    if codes.dim() != 5 or params.dim() != 6 or params.device != codes.device or not codes.is_cuda:
+    shape = codes.shape
+    if len(shape) != 5 or params.device != codes.device or not codes.is_cuda:
         raise ValueError("4-bit cache: expected CUDA codes [2, B, NH, cap, D/2] and params [2, B, NH, cap, groups, 2]")
-    two, B, NH, cap, half = codes.shape
-    D = 2 * half
-    if D not in KV4_HEAD_DIMS:
-        raise ValueError(f"the 4-bit cache takes head_dim 16, 32, 64 or 128, got {D}")
-    G = kv4_groups(D)
+    two, B, NH, cap, half = shape
+    if half not in (8, 16, 32, 64):
+        raise ValueError(f"the 4-bit cache takes head_dim 16, 32, 64 or 128, got {2 * half}")
+    G = 2 if half == 64 else 1
     if two != 2 or params.shape != (2, B, NH, cap, G, 2):
-        raise ValueError(f"4-bit cache: codes {tuple(codes.shape)} and params {tuple(params.shape)} do not match")
-    cs, ps = codes.stride(), params.stride()
-    si, sb, sh = cs[0] // half, cs[1] // half if B > 1 else NH * cap, cs[2] // half if NH > 1 else cap
-    if cs[3:] != (half, 1) or ps[3:] != (2 * G, 2, 1) or cs[0] % half or ps[0] != si * 2 * G \
-            or (B > 1 and (cs[1] % half or ps[1] != sb * 2 * G)) or (NH > 1 and (cs[2] % half or ps[2] != sh * 2 * G)):
+        raise ValueError(f"4-bit cache: codes {tuple(shape)} and params {tuple(params.shape)} do not match")
+    c0, c1, c2, c3, c4 = codes.stride()
+    p0, p1, p2, p3, p4, p5 = params.stride()
+    sh = c2 // half if NH > 1 else cap
+    sb = c1 // half if B > 1 else NH * cap
+    si = c0 // half
+    if c3 != half or c4 != 1 or p3 != 2 * G or p4 != 2 and G > 1 or p5 != 1 or si * half != c0 or p0 != si * 2 * G \
+            or (B > 1 and (sb * half != c1 or p1 != sb * 2 * G)) or (NH > 1 and (sh * half != c2 or p2 != sh * 2 * G)):
         raise ValueError("4-bit cache: rows must be contiguous and both arrays the same view")
-    return B, NH, cap, D, si, sb, sh
+    return B, NH, cap, 2 * half, si, sb, sh
 
 
 def _kv4_marks(name, t, dtype, B, NH, rows, device):
     """(address, sequence stride, head stride) of a [B, NH, >= rows] array beside the cache."""
     if t is None:
         return None, 0, 0
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != NH or t.shape[2] < rows or t.device != device:
-        raise ValueError(f"{name}: expected [{B}, {NH}, >= {rows}] on {device}, got {tuple(t.shape)} on {t.device}")
-    st = t.stride()
-    if st[2] != 1 and t.shape[2] > 1:
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != B or shape[1] != NH or shape[2] < rows or t.device != device:
+        raise ValueError(f"{name}: expected [{B}, {NH}, >= {rows}] on {device}, got {tuple(shape)} on {t.device}")
+    sb, sh, sl = t.stride()
+    if sl != 1 and shape[2] > 1:
         raise ValueError(f"{name}: the last axis must be contiguous")
-    return t.data_ptr(), st[0], st[1]
+    return t.data_ptr(), sb, sh
 
 
 def _per_sequence(name, x, B, device):
@@ -202,14 +212,25 @@ def _per_sequence(name, x, B, device):
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _call_on(device, name, *args):
     """Call an entry point on the current stream of the tensors' device."""
     index = device.index
-    if index == torch.cuda.current_device():
-        call(name, *args, _raw_stream(index))
+    if index == _current_device():
+        rc = getattr(lib, name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, _raw_stream(index))
+            rc = getattr(lib, name)(*args, _raw_stream(index))
+    if rc:
+        raise AttnError(name, rc, last_error())
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name, *sizes):
+    """What a *_workspace_size function answers for these sizes (and current device)."""
+    return getattr(lib, name)(*sizes[1:])
 
 
 def _scratch(workspace, need: int, like):
@@ -226,8 +247,9 @@ def _scratch(workspace, need: int, like):
 
 def _token_rows(name, x, B, NH, D, device):
     """Strides of a [B, T, NH, D] operand with contiguous rows."""
-    if x.dim() != 4 or x.shape[0] != B or x.shape[2] != NH or x.shape[3] != D or x.device != device:
-        raise ValueError(f"{name}: expected [{B}, T, {NH}, {D}] on {device}, got {tuple(x.shape)} on {x.device}")
+    shape = x.shape
+    if len(shape) != 4 or shape[0] != B or shape[2] != NH or shape[3] != D or x.device != device:
+        raise ValueError(f"{name}: expected [{B}, T, {NH}, {D}] on {device}, got {tuple(shape)} on {x.device}")
     st = x.stride()
     if st[3] != 1:
         raise ValueError(f"{name}: head_dim must be contiguous")
@@ -292,11 +314,12 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
     weights are added to it, in place or into ``weights_out``; with ``weights_out`` alone they are set."""
     B, NKV, cap, D, si, sb, sh = _kv4_view(codes, params)
     dev = codes.device
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.device != dev:
-        raise ValueError(f"q: expected [{B}, NH, {D}] on {dev}, got {tuple(q.shape)} on {q.device}")
-    NH = q.shape[1]
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != D or q.device != dev:
+        raise ValueError(f"q: expected [{B}, NH, {D}] on {dev}, got {tuple(shape)} on {q.device}")
+    NH = shape[1]
     if out is None:
-        out = q.new_empty((B, NH, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
         raise ValueError("out: must have q's shape, dtype and device")
     if lse is not None and (lse.shape != (B, NH) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev):
@@ -314,7 +337,7 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
         wsb, wsh = osb, osh
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
     code = dtype_code(q.dtype)
-    need = lib.attn_kv4_decode_workspace_size(B, NH, NKV, length, D, code, w_out is not None)
+    need = _workspace_bytes("attn_kv4_decode_workspace_size", _current_device(), B, NH, NKV, length, D, code, w_out is not None)
     workspace, ws, ws_bytes = _scratch(workspace, need, q)
     _call_on(dev, "attn_kv4_decode", q.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(),
              lse.data_ptr() if lse is not None else None, B, NH, NKV, length, D, qs[0], qs[1], os_[0], os_[1], si, sb, sh,
@@ -350,7 +373,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
         if (isb, ish) != (wsb, wsh):
             raise ValueError("key_weights: weights and out must have the same strides")
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
-    workspace, ws, ws_bytes = _scratch(workspace, lib.attn_key_weights_workspace_size(B, NKV, T), q)
+    workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_key_weights_workspace_size", 0, B, NKV, T), q)
     _call_on(dev, "attn_key_weights", q.data_ptr(), k.data_ptr(), lse.data_ptr(), w_in, w_out, B, NH, NKV, T, D,
              qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, int(first_query), lengths_p,
              1.0 / math.sqrt(D) if scale is None else float(scale), dtype_code(q.dtype if dtype is None else dtype),
@@ -394,7 +417,7 @@ def kv4_evict(codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, 
     if seen is None and lengths is not None:
         seen_p, seen0 = _per_sequence("lengths", lengths, B, dev)
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
-    workspace, ws, ws_bytes = _scratch(workspace, lib.attn_kv4_evict_workspace_size(B, NH, length, keep), codes)
+    workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_kv4_evict_workspace_size", 0, B, NH, length, keep), codes)
     _call_on(dev, "attn_kv4_evict", codes.data_ptr(), params.data_ptr(), wp, pp, si, sb, sh, cap, wsb, wsh, *dst,
              B, NH, length, D, keep, recent, lengths_p, seen_p, seen0, slots.data_ptr(), ws, ws_bytes)
     return slots

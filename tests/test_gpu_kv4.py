@@ -394,6 +394,7 @@ PROMPTS = [
     (1, 1, 1, 1, 16, 0, None), (2, 4, 4, 17, 32, 0, None), (2, 2, 2, 128, 64, 0, None), (1, 3, 3, 129, 64, 40, None),
     (3, 4, 2, 200, 64, 0, [200, 0, 77]), (2, 6, 2, 300, 32, 150, [160, 300]), (1, 2, 1, 513, 16, 500, None),
     (2, 2, 2, 64, 48, 63, None), (1, 2, 2, 257, 64, 257, None), (1, 5, 5, 385, 8, 130, None),
+    (1, 1, 1, 2100, 64, 0, None), (1, 2, 1, 1300, 32, 100, [1290]), (1, 1, 1, 1100, 128, 0, None),  # queries in parts
 ]
 
 

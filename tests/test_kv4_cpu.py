@@ -91,7 +91,7 @@ def test_bad_caches_are_refused(call, bad, code, text):
     (_decode, dict(ws=FAKE + 4), ARG, "aligned"),
     (_weights, dict(q=None), ARG, "null"), (_weights, dict(w_out=None), ARG, "null"), (_weights, dict(dtype=5), ARG, "dtype"),
     (_weights, dict(NH=3), ARG, "multiple"), (_weights, dict(first=-1), ARG, "first_query"), (_weights, dict(T=0), ARG, "positive"),
-    (_weights, dict(D=160), UNSUPPORTED, "head_dim"), (_weights, dict(T=256, ws_bytes=4), WORKSPACE, "workspace"), (_weights, dict(k_st=-1), ARG, "negative"),
+    (_weights, dict(D=160), UNSUPPORTED, "head_dim"), (_weights, dict(T=4096, w_sh=4096, ws_bytes=4), WORKSPACE, "workspace"), (_weights, dict(k_st=-1), ARG, "negative"),
     (_evict, dict(weights=None), ARG, "null"), (_evict, dict(slots=None), ARG, "null"), (_evict, dict(L=17), ARG, "length"),
     (_evict, dict(L=0), ARG, "length"), (_evict, dict(keep=0), ARG, "keep"), (_evict, dict(keep=17), ARG, "keep"),
     (_evict, dict(recent=5), ARG, "recent"), (_evict, dict(recent=-1), ARG, "recent"), (_evict, dict(L=20000, cap=20000, c_sh=20000, c_sb=40000, c_si=80000, ws=None), WORKSPACE, "workspace"),
