@@ -13,10 +13,10 @@
 //   - n as a float16 costs no conversion: its four bits in the mantissa of a float16 with a zero exponent
 //     are a subnormal number, exactly n times a power of two.  The tensor core aligns products by their
 //     operands' exponents, -14 for any subnormal, and drops what lies 24 bits below the largest: codes
-//     at the top of the mantissa (n * 2^-18) keep float32's accuracy and take a shift and an AND per pair;
-//     codes left where they are (n * 2^-24, or 16 n * 2^-24 in the next nibble) take one AND, a shift for
-//     every other pair, and keep 2^-17.  Scores, and the value product of a float32 output, use the
-//     first; the value product of a bfloat16 output (2^-9 itself) the second.
+//     moved to the second nibble (n * 2^-20) keep 2^-22, for an AND and half a shift per pair; codes left where
+//     they are (n * 2^-24, or 16 n * 2^-24 in the second nibble) save the shift and keep 2^-17.  Scores, and
+//     the value product of a float32 output, use the first; the value product of a bfloat16 output (2^-9
+//     itself) the second.
 //   - which element sits in which k slot does not matter as long as the query agrees, so a lane takes
 //     consecutive codes of a key's row.
 //   - q is scaled by a power of two to below 2^12 and p s to below 2^15, which keeps float16's 11 bits at
@@ -38,7 +38,7 @@ namespace attn {
 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
-constexpr int KD_WCHUNK = 2048;  // keys per combine CTA
+constexpr int KD_WCHUNK = 4096;  // keys per combine CTA
 constexpr int KD_SPLIT = 64 * KD_WARPS;  // keys a CTA takes at least, where there are so many
 constexpr int KD_CLUSTER = 8;            // most CTAs of a cluster (the portable limit)
 
@@ -111,15 +111,14 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 
 // Codes in place: nibbles 0 and 1 of each half word (n * 2^-24 and 16 n * 2^-24 as float16).
 constexpr uint32_t KD_LOW = 0x000f000fu, KD_HIGH = 0x00f000f0u;
-constexpr uint32_t KD_TOP = 0x03c003c0u;
-// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs: in place, or at the top of the
-// mantissa, n * 2^-18 (the left shifts as products, which run beside the ANDs on the multiply-add pipe).
+// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs: in place, or both where the odd one
+// stands, n * 2^-20 (the shift as a product, which runs beside the ANDs on the multiply-add pipe).
 template <bool TOP, int PAIR>
 __device__ __forceinline__ void kd_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
   const uint32_t x = PAIR ? w >> 8 : w;
   if constexpr (TOP) {
-    a = (x * 64u) & KD_TOP;
-    b = (x * 4u) & KD_TOP;
+    a = (x * 16u) & KD_HIGH;
+    b = x & KD_HIGH;
   } else {
     a = x & KD_LOW;
     b = x & KD_HIGH;
@@ -234,6 +233,11 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     }
     cp_async_commit();
   };
+  if (tiles == 0 && !p.alone) {  // a split behind its sequence's end
+    for (int i = threadIdx.x; i < nq * (D + 2); i += KD_THREADS)
+      p.states[(((int64_t)b * p.NH + h0 + i / (D + 2)) * p.ns + split) * (D + 2) + i % (D + 2)] = i % (D + 2) ? 0.f : -INFINITY;
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
 
@@ -264,8 +268,8 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
       const float total = warp_sum(sum[k]);
       if (lane == 0) ssum[q * GROUPS + k] = total * p.scale_log2;
     }
-    // the product carries the codes' 2^-18 and the row's `up`
-    if (lane == 0) sfac[q] = p.scale_log2 * __uint_as_float((uint32_t)(127 + 7 + e) << 23);
+    // the product carries the codes' 2^-20 and the row's `up`
+    if (lane == 0) sfac[q] = p.scale_log2 * __uint_as_float((uint32_t)(127 + 9 + e) << 23);
   }
   __syncthreads();
 
@@ -528,8 +532,8 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   }
   __syncthreads();
   float* merge = reinterpret_cast<float*>(smem) + warp * NQ * (D + 2);
-  // the codes' 2^-18 or 2^-24 (16 times that in the odd rows) and p s's scaling
-  const float down = __uint_as_float((uint32_t)(127 + (F32 ? 18 : 24) - 6 + ve) << 23), down_odd = F32 ? down : down * 0.0625f;
+  // the codes' 2^-20 or 2^-24 (16 times that in the odd rows) and p s's scaling
+  const float down = __uint_as_float((uint32_t)(127 + (F32 ? 20 : 24) - 6 + ve) << 23), down_odd = F32 ? down : down * 0.0625f;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     if (lane == 0) {
@@ -732,7 +736,7 @@ static KdPlan kd_plan(int B, int NH, int NKV, int L, int D, int dtype, int weigh
   // (384 units: 137 us against 117)
   const int64_t units = (int64_t)B * NKV * k.chunks;
   const int sms = current_device_sms();
-  const int64_t want = ((int64_t)sms * 7 + units - 1) / units;
+  const int64_t want = ((int64_t)sms * 7 + units / 2) / units > 1 ? ((int64_t)sms * 7 + units / 2) / units : 1;
   const int most = L <= KD_SPLIT ? 1 : kd_most_splits(L);
   int ns = (int)(want < most ? want : most);
   int c = 2;

@@ -118,24 +118,24 @@ __device__ __forceinline__ void evict_move(const Kv4Evict& p, int b, int h, cons
     p.dw[wd + i] = w;
     if (p.dpos) p.dpos[wd + i] = at;
   }
-  for (int which = 0; which < 2; ++which) {
-    const Unit* src = reinterpret_cast<const Unit*>(p.src.codes) + (which * p.src.si + s0) * UNITS;
-    Unit* dst = reinterpret_cast<Unit*>(p.dst.codes) + (which * p.dst.si + d0) * UNITS;
-    for (int u0 = threadIdx.x; u0 < count * UNITS; u0 += blockDim.x * BATCH) {
-      Unit x[BATCH];
-      bool go[BATCH];
+  // keys' units, then values', in one sequence: a chunk of 256 rows is one batch for 256 threads
+  const Unit* src = reinterpret_cast<const Unit*>(p.src.codes) + s0 * UNITS;
+  Unit* dst = reinterpret_cast<Unit*>(p.dst.codes) + (d0 + first) * UNITS;
+  const int units = count * UNITS;
+  for (int u0 = threadIdx.x; u0 < 2 * units; u0 += blockDim.x * BATCH) {
+    Unit x[BATCH];
+    bool go[BATCH];
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const int u = u0 + k * blockDim.x, i = first + u / UNITS;
-        const int from = u < count * UNITS ? slots[i] : -1;
-        go[k] = from >= 0 && !(p.in_place && from == i);
-        if (go[k]) x[k] = src[(int64_t)from * UNITS + u % UNITS];
-      }
+    for (int k = 0; k < BATCH; ++k) {
+      const int v = u0 + k * blockDim.x, u = v < units ? v : v - units, i = first + u / UNITS;
+      const int from = v < 2 * units ? slots[i] : -1;
+      go[k] = from >= 0 && !(p.in_place && from == i);
+      if (go[k]) x[k] = src[((v < units ? 0 : p.src.si) + from) * UNITS + u % UNITS];
+    }
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const int u = u0 + k * blockDim.x;
-        if (go[k]) dst[(int64_t)first * UNITS + u] = x[k];
-      }
+    for (int k = 0; k < BATCH; ++k) {
+      const int v = u0 + k * blockDim.x, u = v < units ? v : v - units;
+      if (go[k]) dst[(v < units ? 0 : p.dst.si) * UNITS + u] = x[k];
     }
   }
 }
