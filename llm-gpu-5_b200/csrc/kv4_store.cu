@@ -28,6 +28,7 @@ int kv4_check(const char* fn, const Kv4View& c, int B, int NH, int D) {
   ATTN_REQUIRE(c.cap % KV4_ALIGN_ROWS == 0 && c.si % KV4_ALIGN_ROWS == 0 && c.sb % KV4_ALIGN_ROWS == 0 &&
                    c.sh % KV4_ALIGN_ROWS == 0,
                "%s: the cache's capacity and strides must be multiples of %d rows", fn, KV4_ALIGN_ROWS);
+  ATTN_REQUIRE(c.cap <= 1 << 30, "%s: capacity %d exceeds 2^30 rows", fn, c.cap);  // positions are ints with room to round up
   ATTN_REQUIRE(c.si >= 0 && c.sb >= 0 && c.sh >= c.cap, "%s: bad cache strides", fn);
   ATTN_REQUIRE(aligned(c.codes, 16) && aligned(c.params, 16), "%s: the cache must be 16-byte aligned", fn);
   return ATTN_OK;

@@ -230,6 +230,8 @@ DECODES = [
     (2, 8, 2, 64, 63, None), (2, 7, 1, 128, 65, [64, 65]), (1, 9, 1, 64, 300, None), (2, 24, 2, 32, 31, None),
     (4, 4, 4, 128, 1000, [0, 999, 16, 255]), (2, 5, 5, 64, 4100, [4097, 4100]), (1, 2, 1, 16, 2049, None),
     (2, 40, 2, 64, 640, [640, 3]), (3, 2, 2, 32, 17, [0, 0, 0]),
+    (40, 8, 8, 32, 600, [(37 * b) % 601 for b in range(40)]),  # more CTAs than the GPU holds, two splits each
+    (1, 33, 1, 16, 5000, None),                                # 33 query heads to a cached one
 ]
 
 
@@ -298,6 +300,21 @@ def test_decode_poisoned_rows_poison_only_their_sequence(ops):
     keep = torch.ones((3, 2), dtype=torch.bool)
     keep[1, 0] = False
     assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_not_finite_query_stays_in_its_head(ops, dtype):
+    """A NaN or an infinity in one query head of a shared group leaves the other heads' outputs alone."""
+    codes, params = make_cache(ops, 2, 1, 70, 64, seed=1)
+    q = torch.randn((2, 4, 64), generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    clean = ops.kv4_decode(q, codes, params, 70)
+    q[0, 1, 3] = float("nan")
+    q[1, 2, 5] = float("inf")
+    got = ops.kv4_decode(q, codes, params, 70)
+    bad = torch.zeros((2, 4), dtype=torch.bool)
+    bad[0, 1] = bad[1, 2] = True
+    assert bool(torch.isnan(got.cpu()[bad].float()).all())
+    assert torch.equal(got.cpu()[~bad], clean.cpu()[~bad])
 
 
 def test_decode_is_repeatable_and_order_free(ops):
@@ -443,6 +460,24 @@ def test_prompt_weights_match_plain(ops, kind, B, NH, NKV, T, D, first, lengths)
     ops.key_weights(q, k, lse, first_query=first, lengths=lens, weights=have[:, :, :T], dtype="tf32" if kind == "tf32" else None)
     within(have[:, :, :T], before[:, :, :T] + w, e + U * (before[:, :, :T] + w) * 2, "added")
     assert torch.equal(have.cpu().double()[:, :, T:], before[:, :, T:])
+
+
+@pytest.mark.parametrize("kind", ["fp32", "tf32", "bf16"])
+def test_prompt_weights_ignore_the_padding(ops, kind):
+    """Whatever lies behind a sequence's last token (queries, keys, lse: NaN and infinities here) reaches
+    no weight, and the weights there are 0."""
+    B, T, NH, D = 3, 300, 2, 32
+    dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+    how = dict(lengths=torch.tensor([300, 129, 5], dtype=torch.int32, device="cuda"), dtype="tf32" if kind == "tf32" else None)
+    gen = torch.Generator().manual_seed(4)
+    q, k = (torch.randn((B, T, NH, D), generator=gen).to(dtype).cuda() for _ in range(2))
+    lse = torch.full((B, NH, T), 4.0, device="cuda")
+    clean = ops.key_weights(q, k, lse, **how)
+    for b, n in enumerate((300, 129, 5)):
+        q[b, n:], k[b, n:], lse[b, :, n:] = float("nan"), float("inf"), float("-inf")
+    got = ops.key_weights(q, k, lse, **how)
+    assert torch.equal(got, clean)
+    assert not bool(got[1, :, 129:].any()) and not bool(got[2, :, 5:].any()) and bool(got[2, :, :5].all())
 
 
 @pytest.mark.parametrize("kind", ["fp32", "tf32", "bf16"])

@@ -63,6 +63,7 @@ CACHE = [
     (dict(c_sh=24), ARG, "multiples of 16"), (dict(c_sb=33), ARG, "multiples of 16"), (dict(c_si=65), ARG, "multiples of 16"),
     (dict(cap=32), ARG, "stride"), (dict(codes=FAKE + 8), ARG, "aligned"), (dict(params=FAKE + 4), ARG, "aligned"),
     (dict(B=0), ARG, "positive"), (dict(B=-1), ARG, "positive"),
+    (dict(cap=(1 << 30) + 16, c_sh=1 << 31, c_sb=1 << 32, c_si=1 << 33), ARG, "2^30"),
 ]
 
 
