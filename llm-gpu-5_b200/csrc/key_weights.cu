@@ -8,8 +8,13 @@
 // the queries past them in tiles of 128, S^T = K Q^T by tcgen05.mma into TMEM with the keys on the lanes, so
 // that a thread owns one key and its sum needs no other thread.  Per score there is one multiply-add, one ex2
 // and one addition: at 16 ex2 per clock and SM a 128 x 128 tile takes 1,024 cycles there, four times its
-// MMA, so the special-function unit bounds it.  Two CTAs share an SM (256 TMEM columns each, two score
-// tiles), so that one's loads and hand-overs hide behind the other's exponentials.
+// MMA, so the special-function unit is the bound: 9,216 tiles (32 x 8 heads of 1,024 tokens) are 34 us of
+// it.  Measured 59 us, the unit 55-60 % busy: a warp spends as long on waiting for scores, masks and moving on
+// to the next tile as in its exponentials, and other warps fill that time only in part.  Three CTAs of one
+// score tile each share an SM (59 us; two CTAs of two score tiles, the next tile's scores asked for before
+// the last ones are summed, 62-64; four CTAs, whose 80 registers spill, 62; eight warps of half the columns,
+// 61-69).  A polynomial exponential on the multiply-add pipe for an eighth to a half of the columns was
+// slower (66-81 against 64), as is every instruction added here.
 //
 // Other shapes and float32 run on CUDA cores: a CTA takes 64 keys and streams the queries past them in tiles of
 // 64, a thread forms 4 x 4 scores (two 16-byte shared-memory reads for 16 products), and the 16 threads of a
@@ -180,17 +185,20 @@ __global__ void __launch_bounds__(KW_THREADS) key_weights_simt_kernel(const KwWo
 }
 
 // ---- tensor cores ------------------------------------------------------------------------------
-constexpr int KT_STAGES = 3;                 // query tiles in flight
+constexpr int KT_CTAS = 3;                   // CTAs per SM
+constexpr int KT_STAGES = 2;                 // query tiles in flight
+constexpr int KT_KEYS = 2;                   // key tiles in flight
+constexpr int KT_BUFS = 1;                   // score tiles in TMEM
 constexpr int KT_THREADS = 192;              // 4 warps of sums, a TMA warp, an MMA warp
-constexpr int KT_TMEM = 256;                 // two 128-column score tiles
-constexpr int KT_SMEM = 1024 + (2 + KT_STAGES) * AT_TILE_BYTES + 4 * 2 * AT_TILE * 4 + 256;
+constexpr int KT_TMEM = KT_BUFS * AT_TILE;
+constexpr int KT_SMEM = 1024 + (KT_KEYS + KT_STAGES) * AT_TILE_BYTES + 4 * AT_TILE * 4 + 256;
 
 struct KwMaps {
   TileMap q, k;
 };
 
 struct KwBars {
-  uint64_t k_full[2], k_empty[2], q_full[KT_STAGES], q_empty[KT_STAGES], s_full[2], s_free[2];
+  uint64_t k_full[KT_KEYS], k_empty[KT_KEYS], q_full[KT_STAGES], q_empty[KT_STAGES], s_full[KT_BUFS], s_free[KT_BUFS];
   uint32_t tmem;
 };
 
@@ -242,20 +250,22 @@ __device__ __forceinline__ void drain_load(uint64_t* bar, uint32_t parity) {
 }
 
 template <bool TF32>
-__global__ void __launch_bounds__(KT_THREADS, 2)
+__global__ void __launch_bounds__(KT_THREADS, KT_CTAS)
 key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sK = smem;                                   // [2]
-  uint8_t* sQ = sK + 2 * AT_TILE_BYTES;                 // [KT_STAGES]
-  float* sL = reinterpret_cast<float*>(sQ + KT_STAGES * AT_TILE_BYTES);  // [4 warps][2][128]
-  KwBars* bars = reinterpret_cast<KwBars*>(sL + 4 * 2 * AT_TILE);
+  uint8_t* sK = smem;                                   // [KT_KEYS]
+  uint8_t* sQ = sK + KT_KEYS * AT_TILE_BYTES;           // [KT_STAGES]
+  float* sL = reinterpret_cast<float*>(sQ + KT_STAGES * AT_TILE_BYTES);  // [4 warps][128]
+  KwBars* bars = reinterpret_cast<KwBars*>(sL + 4 * AT_TILE);
   const WaitErr werr = wait_err(a.err);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < KT_KEYS; ++i) {
       mbar_init(&bars->k_full[i], 1);
       mbar_init(&bars->k_empty[i], 1);
+    }
+    for (int i = 0; i < KT_BUFS; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->s_free[i], 4);
     }
@@ -284,8 +294,8 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
       KwUnit w;
       for (int round = 0; ok && w.set(a, round); ++round) {
         if (w.begin >= w.end) continue;
-        const int ks = ku & 1;
-        if (!mbar_wait(&bars->k_empty[ks], ((ku >> 1) & 1) ^ 1, werr, 501)) { ok = false; break; }
+        const int ks = ku % KT_KEYS;
+        if (!mbar_wait(&bars->k_empty[ks], ((ku / KT_KEYS) & 1) ^ 1, werr, 501)) { ok = false; break; }
         mbar_arrive_expect_tx(&bars->k_full[ks], AT_TILE_BYTES);
         load_tile(sK + ks * AT_TILE_BYTES, maps.k, &bars->k_full[ks], w.b, w.kvh, w.jt * AT_TILE);
         ++ku;
@@ -300,7 +310,7 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
         }
       }
       if (!ok) {  // leave no load of this CTA's behind
-        for (int i = max(0, ku - 2); i < ku; ++i) drain_load(&bars->k_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, ku - KT_KEYS); i < ku; ++i) drain_load(&bars->k_full[i % KT_KEYS], (i / KT_KEYS) & 1);
         for (int i = max(0, qn - KT_STAGES); i < qn; ++i) drain_load(&bars->q_full[i % KT_STAGES], (i / KT_STAGES) & 1);
       }
     }
@@ -313,14 +323,14 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
       KwUnit w;
       for (int round = 0; ok && w.set(a, round); ++round) {
         if (w.begin >= w.end) continue;
-        const int ks = ku & 1;
-        if (!mbar_wait(&bars->k_full[ks], (ku >> 1) & 1, werr, 503)) break;
+        const int ks = ku % KT_KEYS;
+        if (!mbar_wait(&bars->k_full[ks], (ku / KT_KEYS) & 1, werr, 503)) break;
         const uint64_t k_desc = smem_desc_sw128(smem_u32(sK + ks * AT_TILE_BYTES), 16, 1024);
         const int last = qn + w.end - w.begin;
         for (int t = qn; t < last; ++t) {
-          const int qs = t % KT_STAGES, buf = t & 1;
+          const int qs = t % KT_STAGES, buf = t % KT_BUFS;
           if (!mbar_wait(&bars->q_full[qs], (t / KT_STAGES) & 1, werr, 504) ||
-              !mbar_wait(&bars->s_free[buf], ((t >> 1) & 1) ^ 1, werr, 505)) { ok = false; break; }
+              !mbar_wait(&bars->s_free[buf], ((t / KT_BUFS) & 1) ^ 1, werr, 505)) { ok = false; break; }
           tc_fence_after();
           const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ + qs * AT_TILE_BYTES), 16, 1024);
 #pragma unroll
@@ -340,10 +350,7 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
     }
   } else {
     // ---------------- sums: thread = key ----------------
-    // The four 32-column chunks of every tile go through two register buffers: while one is summed the
-    // next is on its way from TMEM, across tiles and units too (the next tile's scores are waited for, and
-    // its first chunk asked for, before this tile's last chunk is summed).
-    float* sl = sL + warp * 2 * AT_TILE;
+    float* lb = sL + warp * AT_TILE;
     const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16);
     const uint64_t cpair = pair(__float_as_uint(a.p.scale_log2), __float_as_uint(a.p.scale_log2));
     const int row = warp * 32 + lane;
@@ -360,21 +367,6 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
     };
     fetch();
     int qn = 0;             // tiles summed
-    uint32_t sr[2][32];
-    // tile qn: -lse in log2 units for this warp, its scores complete, its first chunk on its way
-    auto prime = [&](int t) -> bool {
-      float* lb = sl + (t & 1) * AT_TILE;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) lb[k * 32 + lane] = next[k] * -LOG2E;
-      ahead.next(a);
-      fetch();
-      const bool full = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t & 1], (t >> 1) & 1, werr, 506));
-      __syncwarp();  // lb is written
-      tc_fence_after();
-      tmem_ld32(tS + (t & 1) * 128, sr[0]);
-      return full;
-    };
-    if (ahead.more) ok = prime(0);
     KwUnit w;
     for (int round = 0; ok && w.set(a, round); ++round) {
       const int j = w.jt * AT_TILE + row;
@@ -384,24 +376,29 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
       KwSteps st;
       st.start(w);
       for (int i = w.begin; i < w.end; ++i, ++qn, st.next(w)) {
-        const int buf = qn & 1, i0 = st.it * AT_TILE;
-        const float* lb = sl + buf * AT_TILE;
+        const int buf = qn % KT_BUFS, i0 = st.it * AT_TILE;
+        // -lse in log2 units for this warp; the next tile's is on its way while this one is summed
+#pragma unroll
+        for (int k = 0; k < 4; ++k) lb[k * 32 + lane] = next[k] * -LOG2E;
+        ahead.next(a);
+        fetch();
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[buf], (qn / KT_BUFS) & 1, werr, 506))) { ok = false; break; }
+        tc_fence_after();
         // columns that count for this key: queries from max(j, first) to n - 1; the warp's bounds
         const int c0 = max(j, a.p.first) - i0, c1 = w.n - i0;
         const int c0_any = max(j - lane, a.p.first) - i0, c0_all = max(j - lane + 31, a.p.first) - i0;
         uint64_t sum[2] = {0, 0};  // four running sums of the tile as two packed pairs
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
+          uint32_t x[32];
+          tmem_ld32(tS + buf * 128 + cc * 32, x);
           tmem_wait_ld();
-          if (cc < 3) {
-            tmem_ld32(tS + buf * 128 + (cc + 1) * 32, sr[(cc + 1) & 1]);
-          } else {  // the scores are in registers
+          if (cc == 3) {  // the scores are in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->s_free[buf]);
-            if (ahead.more) ok = prime(qn + 1);
           }
-          uint32_t(&x)[32] = sr[cc & 1];
           if (cc * 32 + 32 <= c0_any) continue;  // before every lane's first query
           if (cc * 32 < c0_all || cc * 32 + 32 > c1) {
             // unused scores may be anything, NaN too: they are replaced, not multiplied
@@ -418,7 +415,7 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
           }
         }
         total += pair_sum(sum[0]) + pair_sum(sum[1]);
-        if (!ok) break;
+        __syncwarp();  // lb is written again for the next tile
       }
       if (!ok) break;
       if (j < a.p.T) {
@@ -521,7 +518,7 @@ static int key_weights_tc(const KeyWeights& p, int B, int tf32, float* partial, 
   KwWork a = kw_work(p, B, AT_TILE, partial);
   a.err = dev_error_ptr();
   if (!a.err) return ATTN_ERR_CUDA;
-  const int64_t ctas = 2 * (int64_t)current_device_sms();
+  const int64_t ctas = KT_CTAS * (int64_t)current_device_sms();
   const unsigned grid = (unsigned)(a.units < ctas ? a.units : ctas);
   static CtxOnce attr[2];
   if (!(tf32 ? set_smem_limit_once(key_weights_tc_kernel<true>, KT_SMEM, attr[1])
