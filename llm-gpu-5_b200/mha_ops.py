@@ -154,7 +154,8 @@ def kv4_empty(B: int, NH: int, capacity: int, D: int, device="cuda"):
 
 # The checks below run once per call of operators whose kernels take a few microseconds for a token: they
 # unpack shapes and strides once and compare dtypes by identity.
-_U8, _F16, _F32, _I32 = torch.uint8, torch.float16, torch.float32, torch.int32
+_U8, _F16 = torch.uint8, torch.float16
+_OF = {code: dtype for dtype, code in _DT.items()}
 
 
 def _kv4_view(codes: torch.Tensor, params: torch.Tensor):
@@ -215,16 +216,13 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
-def _call_on(device, name, *args):
-    """Call an entry point on the current stream of the tensors' device."""
-    index = device.index
-    if index == _current_device():
-        rc = getattr(lib, name)(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, _raw_stream(index))
-    if rc:
-        raise AttnError(name, rc, last_error())
+def _other_device(device):
+    """Make the tensors' device the current one where it is not; what was current, to go back to, or None."""
+    index = _current_device()
+    if device.index == index:
+        return None
+    torch.cuda.set_device(device)
+    return index
 
 
 @functools.lru_cache(maxsize=1024)
@@ -272,6 +270,7 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: tor
     T = k.shape[1]
     if T == 0 or B == 0:
         return
+    code = dtype_code(k.dtype)
     wp, wsb, wsh = _kv4_marks("weights", weights, torch.float32, B, NH, cap, dev)
     pp, psb, psh = _kv4_marks("positions", positions, torch.int32, B, NH, cap, dev)
     if wp is not None and pp is not None and (wsb, wsh) != (psb, psh):
@@ -281,9 +280,16 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: tor
     starts, start = _per_sequence("pos", pos, B, dev)
     seen_p, seen0 = _per_sequence("seen", pos if seen is None else seen, B, dev)
     counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
-    _call_on(dev, "attn_kv4_store", k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), B, T, NH, D, ks[0], ks[1], ks[2],
-             vs[0], vs[1], vs[2], codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, starts, start, counts_p, wp, pp,
-             wsb, wsh, seen_p, seen0)
+    before = _other_device(dev)
+    try:
+        rc = lib.attn_kv4_store(k.data_ptr(), v.data_ptr(), code, B, T, NH, D, ks[0], ks[1], ks[2],
+                                vs[0], vs[1], vs[2], codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, starts, start, counts_p, wp, pp,
+                                wsb, wsh, seen_p, seen0, _raw_stream(dev.index))
+    finally:
+        if before is not None:
+            torch.cuda.set_device(before)
+    if rc:
+        raise AttnError("attn_kv4_store", rc, last_error())
 
 
 def kv4_load(codes: torch.Tensor, params: torch.Tensor, pos, T: int, dtype: torch.dtype = torch.float32, counts=None):
@@ -291,14 +297,22 @@ def kv4_load(codes: torch.Tensor, params: torch.Tensor, pos, T: int, dtype: torc
     ``dtype``; zeros for the rows from ``counts`` on and for slots outside the cache."""
     B, NH, cap, D, si, sb, sh = _kv4_view(codes, params)
     dev = codes.device
+    code = dtype_code(dtype)
     k = codes.new_empty((B, T, NH, D), dtype=dtype)
     v = torch.empty_like(k)
     if k.numel() == 0:
         return k, v
     starts, start = _per_sequence("pos", pos, B, dev)
     counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
-    _call_on(dev, "attn_kv4_load", codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, B, T, NH, D, starts, start,
-             counts_p, k.data_ptr(), v.data_ptr(), dtype_code(dtype), T * NH * D, NH * D, D)
+    before = _other_device(dev)
+    try:
+        rc = lib.attn_kv4_load(codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, B, T, NH, D, starts, start,
+                               counts_p, k.data_ptr(), v.data_ptr(), code, T * NH * D, NH * D, D, _raw_stream(dev.index))
+    finally:
+        if before is not None:
+            torch.cuda.set_device(before)
+    if rc:
+        raise AttnError("attn_kv4_load", rc, last_error())
     return k, v
 
 
@@ -339,10 +353,17 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
     code = dtype_code(q.dtype)
     need = _workspace_bytes("attn_kv4_decode_workspace_size", _current_device(), B, NH, NKV, length, D, code, w_out is not None)
     workspace, ws, ws_bytes = _scratch(workspace, need, q)
-    _call_on(dev, "attn_kv4_decode", q.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(),
-             lse.data_ptr() if lse is not None else None, B, NH, NKV, length, D, qs[0], qs[1], os_[0], os_[1], si, sb, sh,
-             cap, lengths_p, w_in, w_out, wsb, wsh, 1.0 / math.sqrt(D) if scale is None else float(scale),
-             code, ws, ws_bytes)
+    before = _other_device(dev)
+    try:
+        rc = lib.attn_kv4_decode(q.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(),
+                                 lse.data_ptr() if lse is not None else None, B, NH, NKV, length, D, qs[0], qs[1], os_[0], os_[1], si, sb, sh,
+                                 cap, lengths_p, w_in, w_out, wsb, wsh, 1.0 / math.sqrt(D) if scale is None else float(scale),
+                                 code, ws, ws_bytes, _raw_stream(dev.index))
+    finally:
+        if before is not None:
+            torch.cuda.set_device(before)
+    if rc:
+        raise AttnError("attn_kv4_decode", rc, last_error())
     return out
 
 
@@ -360,6 +381,9 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
     B, T, NH, D = q.shape
     NKV, dev = k.shape[2], q.device
     qs, ks = _token_rows("q", q, B, NH, D, dev), _token_rows("k", k, B, NKV, D, dev)
+    code = dtype_code(q.dtype if dtype is None else dtype)
+    if q.dtype is not (torch.float32 if code == ATTN_TF32 else _OF[code]):
+        raise TypeError(f"key_weights: {dtype} does not go with operands of {q.dtype}")
     if k.shape[1] != T:
         raise ValueError(f"key_weights: q holds {T} tokens, k {k.shape[1]}")
     if lse.shape != (B, NH, T) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
@@ -374,10 +398,17 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
             raise ValueError("key_weights: weights and out must have the same strides")
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
     workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_key_weights_workspace_size", 0, B, NKV, T), q)
-    _call_on(dev, "attn_key_weights", q.data_ptr(), k.data_ptr(), lse.data_ptr(), w_in, w_out, B, NH, NKV, T, D,
-             qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, int(first_query), lengths_p,
-             1.0 / math.sqrt(D) if scale is None else float(scale), dtype_code(q.dtype if dtype is None else dtype),
-             ws, ws_bytes)
+    before = _other_device(dev)
+    try:
+        rc = lib.attn_key_weights(q.data_ptr(), k.data_ptr(), lse.data_ptr(), w_in, w_out, B, NH, NKV, T, D,
+                                  qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, int(first_query), lengths_p,
+                                  1.0 / math.sqrt(D) if scale is None else float(scale), code,
+                                  ws, ws_bytes, _raw_stream(dev.index))
+    finally:
+        if before is not None:
+            torch.cuda.set_device(before)
+    if rc:
+        raise AttnError("attn_key_weights", rc, last_error())
     return out
 
 
@@ -418,8 +449,15 @@ def kv4_evict(codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, 
         seen_p, seen0 = _per_sequence("lengths", lengths, B, dev)
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
     workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_kv4_evict_workspace_size", 0, B, NH, length, keep), codes)
-    _call_on(dev, "attn_kv4_evict", codes.data_ptr(), params.data_ptr(), wp, pp, si, sb, sh, cap, wsb, wsh, *dst,
-             B, NH, length, D, keep, recent, lengths_p, seen_p, seen0, slots.data_ptr(), ws, ws_bytes)
+    before = _other_device(dev)
+    try:
+        rc = lib.attn_kv4_evict(codes.data_ptr(), params.data_ptr(), wp, pp, si, sb, sh, cap, wsb, wsh, *dst,
+                                B, NH, length, D, keep, recent, lengths_p, seen_p, seen0, slots.data_ptr(), ws, ws_bytes, _raw_stream(dev.index))
+    finally:
+        if before is not None:
+            torch.cuda.set_device(before)
+    if rc:
+        raise AttnError("attn_kv4_evict", rc, last_error())
     return slots
 
 
