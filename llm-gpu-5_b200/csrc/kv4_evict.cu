@@ -210,14 +210,15 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
         if (j < n && j < p.keep && !stay) count += 1;
         if (j >= p.keep && stay) count += 1 << 16;
       }
+      // every slot keeps its row, in one coalesced sweep; the holes are written over below
+      for (int i = threadIdx.x; i < p.keep; i += EV_THREADS) slots[i] = i;
       int at = block_scan(count, red[0], &total);
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
         const int j = base + k;
         const bool stay = (kept >> k & 1) != 0;
         if (j < p.keep) {
-          if (stay) slots[j] = j;
-          else if (j < n) {
+          if (!stay && j < n) {
             holes[at & 0xffff] = (uint16_t)j;
             at += 1;
           }
