@@ -12,11 +12,11 @@
 // single query, which the idle tensor pipe does not mind), with the codes as the A operand:
 //   - n as a float16 costs no conversion: its four bits in the mantissa of a float16 with a zero exponent
 //     are a subnormal number, exactly n times a power of two.  The tensor core aligns products by their
-//     operands' exponents, -14 for any subnormal, and drops what lies 24 bits below the largest: codes
-//     moved to the second nibble (n * 2^-20) keep 2^-22, for an AND and half a shift per pair; codes left where
-//     they are (n * 2^-24, or 16 n * 2^-24 in the second nibble) save the shift and keep 2^-17.  Scores, and
-//     the value product of a float32 output, use the first; the value product of a bfloat16 output (2^-9
-//     itself) the second.
+//     operands' exponents, -14 for any subnormal, and drops what lies 24 bits below the largest: codes at
+//     the top of the mantissa (n * 2^-18) keep float32's accuracy, for a shift and an AND per pair; codes in the
+//     second nibble (n * 2^-20) keep 2^-22 and save half the shifts; codes left where they are (n * 2^-24, or
+//     16 n * 2^-24 in the second nibble) save them all and keep 2^-17.  float32 calls use the first, the scores
+//     of bfloat16 ones the second, and their value product (the output keeps 2^-9) the third.
 //   - which element sits in which k slot does not matter as long as the query agrees, so a lane takes
 //     consecutive codes of a key's row.
 //   - q is scaled by a power of two to below 2^12 and p s to below 2^15, which keeps float16's 11 bits at
@@ -28,8 +28,11 @@
 // between warps): scores into shared memory, then one key per lane for the softmax, whose running maximum
 // moves only when it grows by more than 2^8 (the accumulators are rescaled then), then p s back as the B
 // operand.  The length is split over the CTAs of a cluster, up to eight, which merge their states (m, l, o[D])
-// through distributed shared memory and add the weights of their own keys: one launch.  Few heads over long
-// sequences need more CTAs than that: these write their states to the workspace for a combine kernel.
+// through distributed shared memory and add the weights of their own keys: one launch, where the GPU holds all
+// clusters at once.  Otherwise (many heads, or few over long sequences) the splits write their states to the
+// workspace for a combine kernel.  Measured: 32 x 12 heads of 16,384 rows with weights 88 us for this kernel
+// (453 MB of cache and 25 of scores, 84 % of the copy rate) and 22 for the combine kernel; 64 x 8 heads of 2,048
+// rows 22-25 us; 8 x 8 float32 heads of 4,099 rows of 32 in one launch of clusters, 13 us with the host's part.
 #include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
@@ -109,14 +112,19 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// Codes in place: nibbles 0 and 1 of each half word (n * 2^-24 and 16 n * 2^-24 as float16).
-constexpr uint32_t KD_LOW = 0x000f000fu, KD_HIGH = 0x00f000f0u;
-// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs: in place, or both where the odd one
-// stands, n * 2^-20 (the shift as a product, which runs beside the ANDs on the multiply-add pipe).
-template <bool TOP, int PAIR>
+// Where a code's bits stand in its float16: n * 2^-24 and, in the second nibble, 16 n * 2^-24; the second nibble
+// for both, n * 2^-20; or the top of the mantissa, n * 2^-18.
+enum KdPlace { KD_INPLACE, KD_SECOND, KD_TOP };
+constexpr uint32_t KD_LOW = 0x000f000fu, KD_HIGH = 0x00f000f0u, KD_TOPMOST = 0x03c003c0u;
+// Nibbles 2*PAIR and 2*PAIR + 1 of each half word as two float16 pairs (left shifts as products, which run
+// beside the ANDs on the multiply-add pipe).
+template <int PLACE, int PAIR>
 __device__ __forceinline__ void kd_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
   const uint32_t x = PAIR ? w >> 8 : w;
-  if constexpr (TOP) {
+  if constexpr (PLACE == KD_TOP) {
+    a = (x * 64u) & KD_TOPMOST;
+    b = (x * 4u) & KD_TOPMOST;
+  } else if constexpr (PLACE == KD_SECOND) {
     a = (x * 16u) & KD_HIGH;
     b = x & KD_HIGH;
   } else {
@@ -125,19 +133,19 @@ __device__ __forceinline__ void kd_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
   }
 }
 // c += (codes of two key rows) * (query): four codes a lane of each row.
-template <int PAIR>
+template <int PLACE, int PAIR>
 __device__ __forceinline__ void kd_score_mma(float (&c)[4], uint32_t wa, uint32_t wb, const uint32_t (&q)[2]) {
   uint32_t a0, a1, a2, a3;
-  kd_pairs<true, PAIR>(wa, a0, a2);
-  kd_pairs<true, PAIR>(wb, a1, a3);
+  kd_pairs<PLACE, PAIR>(wa, a0, a2);
+  kd_pairs<PLACE, PAIR>(wb, a1, a3);
   mma_f16(c, a0, a1, a2, a3, q[0], q[1]);
 }
 // acc += (codes of one value row pair) * (p s): x holds four elements of two keys, y of two more.
-template <bool TOP, int PAIR>
+template <int PLACE, int PAIR>
 __device__ __forceinline__ void kd_value_mma(float (&acc)[4], uint32_t x, uint32_t y, uint32_t b0, uint32_t b1) {
   uint32_t xa, xb, ya, yb;
-  kd_pairs<TOP, PAIR>(x, xa, xb);
-  kd_pairs<TOP, PAIR>(y, ya, yb);
+  kd_pairs<PLACE, PAIR>(x, xa, xb);
+  kd_pairs<PLACE, PAIR>(y, ya, yb);
   mma_f16(acc, xa, xb, ya, yb, b0, b1);
 }
 
@@ -187,6 +195,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   constexpr bool F32 = sizeof(T) == 4;
   using S = KdTile<D, NQ, F32>;
   constexpr int GROUPS = S::GROUPS, GS = kv4_group(D), KD_TILE = S::TILE, PL = KD_TILE / 32;  // PL keys per lane
+  constexpr int KPLACE = F32 ? KD_TOP : KD_SECOND, VPLACE = F32 ? KD_TOP : KD_INPLACE;
   constexpr int MT = D / 16;   // 16-row tiles of the value product
   constexpr int KS = D / 16;   // 16-deep steps of the score product
   extern __shared__ __align__(16) uint8_t smem[];
@@ -256,9 +265,9 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     }
     big = warp_max(big);
     // 2^(11 - exponent of the largest), so that the scaled row is below 2^12; exponents are kept to
-    // where both powers are normal numbers
+    // where both powers are normal numbers (a row that reaches 2^122, whose scores float32 hardly holds, gives NaN)
     int e = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
-    e = min(max(e, -110), 113);
+    e = min(max(e, -110), 118);
     const float up = __uint_as_float((uint32_t)(127 + 11 - e) << 23);
 #pragma unroll
     for (int k = 0; k < (D + 31) / 32; ++k)
@@ -268,8 +277,8 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
       const float total = warp_sum(sum[k]);
       if (lane == 0) ssum[q * GROUPS + k] = total * p.scale_log2;
     }
-    // the product carries the codes' 2^-20 and the row's `up`
-    if (lane == 0) sfac[q] = p.scale_log2 * __uint_as_float((uint32_t)(127 + 9 + e) << 23);
+    // the product carries the codes' 2^-18 or 2^-20 and the row's `up`
+    if (lane == 0) sfac[q] = p.scale_log2 * __uint_as_float((uint32_t)(127 + (F32 ? 7 : 9) + e) << 23);
   }
   __syncthreads();
 
@@ -354,15 +363,15 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
 #pragma unroll
           for (int w = 0; w < WORDS; ++w) {
             const int s = (k * WORDS + w) * 2;
-            kd_score_mma<0>(cs[k], wa[w], wb[w], qb[s]);
-            kd_score_mma<1>(cs[k], wa[w], wb[w], qb[s + 1]);
+            kd_score_mma<KPLACE, 0>(cs[k], wa[w], wb[w], qb[s]);
+            kd_score_mma<KPLACE, 1>(cs[k], wa[w], wb[w], qb[s + 1]);
           }
         }
       } else {
         // 4 codes per lane: byte 0 to the low half, byte 1 to the high half
         const uint32_t xa = __byte_perm(*reinterpret_cast<const uint16_t*>(ra + t * 2), 0, 0x4140);
         const uint32_t xb = __byte_perm(*reinterpret_cast<const uint16_t*>(rb + t * 2), 0, 0x4140);
-        kd_score_mma<0>(cs[0], xa, xb, qb[0]);
+        kd_score_mma<KPLACE, 0>(cs[0], xa, xb, qb[0]);
       }
       float r[4] = {cs[0][0], cs[0][1], cs[0][2], cs[0][3]};
       if constexpr (GROUPS == 2) {  // the groups' scales belong to the key: rows g and g + 8
@@ -484,7 +493,14 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     __syncwarp();
 
     // ---- values: acc[d][column] += sum over the keys of codes * p s ----
+    // (the tensor core's additions round towards zero; a float32 output's tiles are added with rounding to nearest,
+    // so that the bias of long sums stays below the other errors)
     const uint8_t* vc = st + S::CODE_BYTES;
+    float tile_sum[F32 ? MT : 1][4];
+    if constexpr (F32)
+#pragma unroll
+      for (int k = 0; k < MT; ++k) tile_sum[k][0] = tile_sum[k][1] = tile_sum[k][2] = tile_sum[k][3] = 0.f;
+    float(*sum_v)[4] = F32 ? tile_sum : acc;
 #pragma unroll
     for (int kk = 0; kk < KD_TILE / 16; ++kk) {
       const uint8_t* r0 = vc + (kk * 16 + t) * (D / 2);  // keys t, t+4, t+8, t+12
@@ -502,23 +518,28 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
           const uint32_t w2 = *reinterpret_cast<const uint32_t*>(r0 + 8 * (D / 2) + k * 32 + g * 4);
           const uint32_t w3 = *reinterpret_cast<const uint32_t*>(r0 + 12 * (D / 2) + k * 32 + g * 4);
           uint32_t x = __byte_perm(w0, w1, 0x5410), y = __byte_perm(w2, w3, 0x5410);  // elements 0..3
-          kd_value_mma<F32, 0>(acc[k * 4 + 0], x, y, b0, b1);
-          kd_value_mma<F32, 1>(acc[k * 4 + 1], x, y, b0, b1);
+          kd_value_mma<VPLACE, 0>(sum_v[k * 4 + 0], x, y, b0, b1);
+          kd_value_mma<VPLACE, 1>(sum_v[k * 4 + 1], x, y, b0, b1);
           x = __byte_perm(w0, w1, 0x7632); y = __byte_perm(w2, w3, 0x7632);  // elements 4..7
-          kd_value_mma<F32, 0>(acc[k * 4 + 2], x, y, b0, b1);
-          kd_value_mma<F32, 1>(acc[k * 4 + 3], x, y, b0, b1);
+          kd_value_mma<VPLACE, 0>(sum_v[k * 4 + 2], x, y, b0, b1);
+          kd_value_mma<VPLACE, 1>(sum_v[k * 4 + 3], x, y, b0, b1);
         } else if constexpr (D == 32) {
           auto half_word = [&](int key) { return (uint32_t)*reinterpret_cast<const uint16_t*>(r0 + key * (D / 2) + g * 2); };
           const uint32_t x = half_word(0) | half_word(4) << 16, y = half_word(8) | half_word(12) << 16;
-          kd_value_mma<F32, 0>(acc[0], x, y, b0, b1);
-          kd_value_mma<F32, 1>(acc[1], x, y, b0, b1);
+          kd_value_mma<VPLACE, 0>(sum_v[0], x, y, b0, b1);
+          kd_value_mma<VPLACE, 1>(sum_v[1], x, y, b0, b1);
         } else {
           auto byte = [&](int key) { return (uint32_t)r0[key * (D / 2) + g]; };
           const uint32_t x = byte(0) | byte(4) << 16, y = byte(8) | byte(12) << 16;
-          kd_value_mma<F32, 0>(acc[0], x, y, b0, b1);
+          kd_value_mma<VPLACE, 0>(sum_v[0], x, y, b0, b1);
         }
       }
     }
+    if constexpr (F32)
+#pragma unroll
+      for (int k = 0; k < MT; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[k][r] += tile_sum[k][r];
     __syncwarp();  // the stage and the p s tile may be written again
   }
   cp_async_wait<0>();
@@ -532,8 +553,8 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   }
   __syncthreads();
   float* merge = reinterpret_cast<float*>(smem) + warp * NQ * (D + 2);
-  // the codes' 2^-20 or 2^-24 (16 times that in the odd rows) and p s's scaling
-  const float down = __uint_as_float((uint32_t)(127 + (F32 ? 20 : 24) - 6 + ve) << 23), down_odd = F32 ? down : down * 0.0625f;
+  // the codes' 2^-18 or 2^-24 (16 times that in the odd rows) and p s's scaling
+  const float down = __uint_as_float((uint32_t)(127 + (F32 ? 18 : 24) - 6 + ve) << 23), down_odd = F32 ? down : down * 0.0625f;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     if (lane == 0) {

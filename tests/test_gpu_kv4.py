@@ -394,6 +394,37 @@ def test_captured_decode_loop_grows_with_device_lengths(pkg, ops):
         assert torch.equal(loops[i].pos, eager[i].pos) and loops[i].lens.tolist() == [s + steps for s in start]
 
 
+@pytest.mark.parametrize("B,NH,L", [(1, 3, 2000), (1, 1, 9000), (70, 8, 600)])
+def test_captured_calls_of_every_plan(pkg, ops, B, NH, L):
+    """Decode as a cluster, and through the combine kernel, prompt weights in parts and an eviction, captured
+    and replayed on new queries: the same numbers as eager calls."""
+    D = 64
+    codes, params = make_cache(ops, B, NH, L, D, seed=L)
+    cap = codes.shape[3]
+    gen = torch.Generator().manual_seed(L)
+    q = torch.randn((B, NH, D), generator=gen).cuda()
+    w = torch.rand((B, NH, cap), generator=gen).cuda()
+    pos = torch.arange(cap, dtype=torch.int32, device="cuda").expand(B, NH, cap).contiguous()
+    T = 700 if B > 1 else 2100
+    qk = torch.randn((2, 1, T, 1, D), generator=gen).bfloat16().cuda()
+    lse = torch.full((1, 1, T), 5.0, device="cuda")
+
+    def step():
+        w2 = torch.empty_like(w)
+        o = ops.kv4_decode(q, codes, params, L, weights=w, weights_out=w2)
+        out = ops.kv4_empty(B, NH, 512, D) + (torch.zeros((B, NH, 512), device="cuda"), torch.zeros((B, NH, 512), dtype=torch.int32, device="cuda"))
+        slots = ops.kv4_evict(codes, params, w2, pos, L, 500, recent=7, out=out)
+        return (o, w2, ops.key_weights(qk[0], qk[1], lse), slots, out[2], out[3], out[0][:, :, :, :500].clone())
+
+    step()
+    graph = pkg.graphs.CapturedStep(step)
+    for i in range(3):
+        q.copy_(torch.randn((B, NH, D), generator=gen))
+        want = [t.clone() for t in step()]
+        for a, b in zip(graph.replay(), want):
+            assert torch.equal(a[..., :L], b[..., :L])
+
+
 def test_decode_of_many_sequence_heads(ops):
     """More sequences x heads than a grid's second axis holds."""
     B, NH, D, L = 8200, 8, 16, 3
