@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
         const uint32_t cand = limit | bit;
         int c = 0;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) c += key[k] >= cand;
+        for (int k = 0; k < PER; ++k)  // c += key >= cand, as the carry of key - cand: two instructions a key
+          asm("{\n\t.reg .u32 t;\n\tadd.cc.u32 t, %1, %2;\n\taddc.u32 %0, %0, 0;\n\t}" : "+r"(c) : "r"(key[k]), "r"(0u - cand));
         const int total = block_total(__reduce_add_sync(0xffffffffu, c), red[round & 1]);
         if (total >= p.keep) limit = cand;
         if (total == p.keep) break;  // these are the kept ones: no lower bit can change that
