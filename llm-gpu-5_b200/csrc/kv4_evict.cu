@@ -11,7 +11,8 @@
 // One CTA selects for one (sequence, head).  Up to 16,384 rows it holds every row's order key in registers,
 // consecutive rows to a thread, and finds the keep-th largest bit by bit from the top: 32 counts, each a
 // warp reduction, one barrier and a sum over the warps (no atomics, so the weights' skewed exponents cost
-// nothing).  Longer sequences take a radix search, four passes of 8 bits over a histogram in shared memory.
+// nothing).  After about nine of them the undecided keys are few enough for one to a thread, and a count is a
+// barrier (730 cycles a round before, 50 after).  Longer sequences take a radix search, four passes of 8 bits over a histogram in shared memory.
 // Ties, holes and spare rows are numbered with block scans in slot order, and slots[i] = the row that slot i
 // holds afterwards (-1 past the kept ones).  The rows are then copied, codes in 16-byte pieces: by the same
 // CTA when there are few to move (one launch), else by a second kernel.  Measured for half of 32 x 8 heads of 8,192
@@ -178,18 +179,45 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
 #pragma unroll
         for (int k = 0; k < PER; ++k) key[k] = base + k < n ? evict_key(p, row_w, base + k, protect_from) : 0u;
       }
-      // rows past the end have key 0 and would count for limit 0 alone, which ends the search as well
-      uint32_t limit = 0;
-      int round = 0;
-      for (uint32_t bit = 0x80000000u; bit; bit >>= 1, ++round) {
+      // count(key >= limit) = lo >= keep, and count(key >= limit + bit) = hi < keep.  Rows past the end have key
+      // 0, which no candidate counts.
+      __shared__ uint32_t list[EV_THREADS];
+      uint32_t limit = 0, bit = 0x80000000u;
+      int lo = n, hi = 0, round = 0;
+      for (; bit && lo != p.keep && lo - hi > EV_THREADS; bit >>= 1, ++round) {
         const uint32_t cand = limit | bit;
         int c = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k)  // c += key >= cand, as the carry of key - cand: two instructions a key
           asm("{\n\t.reg .u32 t;\n\tadd.cc.u32 t, %1, %2;\n\taddc.u32 %0, %0, 0;\n\t}" : "+r"(c) : "r"(key[k]), "r"(0u - cand));
         const int total = block_total(__reduce_add_sync(0xffffffffu, c), red[round & 1]);
-        if (total >= p.keep) limit = cand;
-        if (total == p.keep) break;  // these are the kept ones: no lower bit can change that
+        if (total >= p.keep) {
+          limit = cand;
+          lo = total;
+        } else {
+          hi = total;
+        }
+      }
+      // (lo == keep: these are the kept ones, and no lower bit can change that)
+      if (bit && lo != p.keep) {
+        // no more undecided keys than threads: a thread takes one, and a round is a counting barrier
+        const uint32_t last = limit + (bit - 1) + bit;
+        int in = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) in += base + k < n && key[k] >= limit && key[k] <= last;
+        int all;
+        int at = block_scan(in, red[round & 1], &all);
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          if (base + k < n && key[k] >= limit && key[k] <= last) list[at++] = key[k];
+        __syncthreads();
+        const uint32_t mine = threadIdx.x < all ? list[threadIdx.x] : 0u;
+        const int need = p.keep - hi;
+        for (; bit; bit >>= 1) {
+          const int total = __syncthreads_count(mine >= (limit | bit));
+          if (total >= need) limit |= bit;
+          if (total == need) break;
+        }
       }
       int above = 0, tie = 0;
 #pragma unroll
