@@ -108,13 +108,21 @@ __device__ __forceinline__ void kw_write(const KwWork& a, const KwUnit& w, int j
   }
 }
 
-// Rows [r0, r0 + 64) of a head, rows past `rows` as zeros, into sm[d][row]; four rows of one element group at a time.
+// Rows [r0, r0 + 64) of a head, rows past `rows` as zeros, into sm[d][row].  Consecutive threads read consecutive
+// elements; a thread steps from one to its next by (rows, elements) = (KW_THREADS / D, KW_THREADS % D).
 template <typename T, bool TF32>
-__device__ __forceinline__ void kw_load_tile(float* sm, const T* base, int64_t st, int r0, int rows, int D) {
-  for (int e = threadIdx.x; e < KW_TILE * D; e += KW_THREADS) {
-    const int r = e / D, d = e - r * D;  // consecutive threads read consecutive elements
+__device__ __forceinline__ void kw_load_tile(float* sm, const T* base, int64_t st, int r0, int rows, int D, int dr, int dd) {
+  int r = threadIdx.x / D, d = threadIdx.x - r * D;
+#pragma unroll 4
+  for (; r < KW_TILE;) {
     const float x = r0 + r < rows ? Elem<T>::load(base + (int64_t)(r0 + r) * st + d) : 0.f;
     sm[d * KW_LD + r] = TF32 ? tf32_cut(x) : x;
+    r += dr;
+    d += dd;
+    if (d >= D) {
+      d -= D;
+      ++r;
+    }
   }
 }
 
@@ -129,17 +137,18 @@ __global__ void __launch_bounds__(KW_THREADS) key_weights_simt_kernel(const KwWo
   grid_dependents_launch();
   KwUnit w;
   w.open(a, blockIdx.x, KW_TILE);
+  const int dr = KW_THREADS / p.D, dd = KW_THREADS - dr * p.D;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // queries 4 tx.., keys 4 ty..
   const int j0 = w.jt * KW_TILE;
   if (w.begin < w.end)
-    kw_load_tile<T, TF32>(sk, (const T*)p.k + w.b * p.k_sb + w.kvh * p.k_sh, p.k_st, j0, w.n, p.D);
+    kw_load_tile<T, TF32>(sk, (const T*)p.k + w.b * p.k_sb + w.kvh * p.k_sh, p.k_st, j0, w.n, p.D, dr, dd);
   float total[4] = {0.f, 0.f, 0.f, 0.f};
   KwSteps st;
   st.start(w);
   for (int i = w.begin; i < w.end; ++i, st.next(w)) {
     const int h = w.kvh * p.G + st.g, i0 = st.it * KW_TILE;
     __syncthreads();
-    kw_load_tile<T, TF32>(sq, (const T*)p.q + w.b * p.q_sb + h * p.q_sh, p.q_st, i0, w.n, p.D);
+    kw_load_tile<T, TF32>(sq, (const T*)p.q + w.b * p.q_sb + h * p.q_sh, p.q_st, i0, w.n, p.D, dr, dd);
     if (threadIdx.x < KW_TILE)
       sl[threadIdx.x] = i0 + threadIdx.x < w.n ? p.lse[((int64_t)w.b * p.NH + h) * p.T + i0 + threadIdx.x] * -1.4426950408889634f : 0.f;
     __syncthreads();
@@ -165,7 +174,7 @@ __global__ void __launch_bounds__(KW_THREADS) key_weights_simt_kernel(const KwWo
       for (int y = 0; y < 4; ++y) {
         const int q = i0 + 4 * tx + y;
         const bool use = q < w.n && q >= p.first && q >= j0 + 4 * ty + x;
-        const float e = exp2f(fmaf(acc[x][y], p.scale_log2, sl[4 * tx + y]));
+        const float e = ex2_approx(fmaf(acc[x][y], p.scale_log2, sl[4 * tx + y]));
         sum += use ? e : 0.f;
       }
       total[x] += sum;

@@ -356,8 +356,11 @@ static int kv4_evict_d(Kv4Evict& p, int B, cudaStream_t s) {
   p.fused = rows <= 1024;
   const dim3 grid((unsigned)heads), block(EV_THREADS);
   cudaError_t e;
+  // the fewest rows per thread that hold the sequence: idle threads and wide loops both cost (256 heads of 4,000 rows:
+  // 18 us with 16 a thread, of 10,330 rows 40 us with 32)
   if (p.L <= EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 1>, grid, block, 0, s, p);
   else if (p.L <= 4 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 4>, grid, block, 0, s, p);
+  else if (p.L <= 8 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 8>, grid, block, 0, s, p);
   else if (p.L <= 16 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 16>, grid, block, 0, s, p);
   else if (p.L <= EV_MOST * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, EV_MOST>, grid, block, 0, s, p);
   else e = launch_pdl(kv4_evict_select_kernel<D, 0>, grid, block, 0, s, p);

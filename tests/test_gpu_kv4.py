@@ -553,7 +553,8 @@ EVICTIONS = [
     # B, NH, D, L, keep, recent, lengths
     (1, 1, 64, 2, 1, 0, None), (2, 3, 64, 129, 128, 16, None), (1, 2, 32, 500, 17, 17, None), (3, 2, 16, 200, 64, 5, [200, 64, 0]),
     (2, 2, 128, 1500, 700, 100, [1500, 701]), (1, 1, 64, 5000, 4999, 0, None), (2, 1, 64, 64, 64, 8, None),
-    (1, 3, 32, 40000, 20000, 64, None), (1, 2, 16, 33, 40, 2, None),
+    (1, 3, 32, 40000, 20000, 64, None), (1, 2, 16, 33, 40, 2, None), (1, 2, 32, 3000, 1000, 30, None),
+    (1, 1, 64, 12000, 7000, 100, None), (2, 1, 16, 9000, 8999, 8999, [9000, 8999]),
 ]
 
 
