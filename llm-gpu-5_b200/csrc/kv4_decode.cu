@@ -649,21 +649,24 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
 
 // Merge the splits' states and add the weights: a CTA takes KD_WCHUNK keys of one (sequence, key head), and
 // its share of the outputs.  A warp finds a head's maximum and sum, the splits on its lanes, so that a call
-// waits for memory three times, not once per head and split.
+// waits for memory three times, not once per head and split.  16 keys a thread keep enough bytes in flight at two
+// CTAs an SM (110 us for the long case's two kernels and 33 for the shared heads'; 8 keys and four CTAs 110 and 35,
+// 4 and six 127 and 37); without weights there is little to hold, and six CTAs share an SM (64 x 8 heads of 2,048
+// rows 25 -> 22 us).
 constexpr int KC_THREADS = 256;
 constexpr int KC_HEADS = 32;  // query heads at a time
-template <typename T, int D>
-__global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv4Decode p) {
+template <typename T, int D, bool WEIGHTS>
+__global__ void __launch_bounds__(KC_THREADS, WEIGHTS ? 2 : 6) kv4_decode_combine_kernel(const Kv4Decode p) {
   __shared__ float smx[KC_HEADS], sinv[KC_HEADS];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int wchunks = p.weights ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
+  const int wchunks = WEIGHTS ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
   const int bk = blockIdx.x / wchunks, chunk = blockIdx.x % wchunks;
   const int b = bk / p.NKV, kvh = bk % p.NKV;
   const int n = seq_length(p.lengths, b, p.L);
   const int j0 = chunk * KD_WCHUNK + threadIdx.x;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  constexpr int PER = KD_WCHUNK / KC_THREADS;
+  constexpr int PER = WEIGHTS ? KD_WCHUNK / KC_THREADS : 1;
   const int64_t bh0 = (int64_t)b * p.NH + kvh * p.G, w0 = b * p.w_sb + kvh * p.w_sh;
   // what does not depend on the states is asked for first: the sums so far, and the first head's scores
   float w[PER], have[PER], z[PER];
@@ -672,8 +675,8 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv
   for (int i = 0; i < PER; ++i) {
     const int j = j0 + i * KC_THREADS;
     w[i] = 0.f;
-    have[i] = p.weights && p.w_in && j < p.L ? p.w_in[w0 + j] : 0.f;
-    z[i] = p.weights && j < n ? zrow[i * KC_THREADS] : -INFINITY;
+    have[i] = WEIGHTS && p.w_in && j < p.L ? p.w_in[w0 + j] : 0.f;
+    z[i] = WEIGHTS && j < n ? zrow[i * KC_THREADS] : -INFINITY;
   }
   for (int g0 = 0; g0 < p.G; g0 += KC_HEADS) {
     const int heads = min(KC_HEADS, p.G - g0);
@@ -714,7 +717,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv
         Elem<T>::store((T*)p.o + b * p.o_sb + (kvh * p.G + g0 + g) * p.o_sh + d, o * sinv[g]);
       }
     }
-    if (p.weights) {
+    if (WEIGHTS) {
       for (int g = 0; g < heads; ++g) {
         const float mx = smx[g], inv = sinv[g];
         zrow += p.L;
@@ -728,7 +731,7 @@ __global__ void __launch_bounds__(KC_THREADS) kv4_decode_combine_kernel(const Kv
       }
     }
   }
-  if (p.weights) {
+  if (WEIGHTS) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int j = j0 + i * KC_THREADS;
@@ -795,7 +798,9 @@ static int kv4_decode_q(const Kv4View& c, const Kv4Decode& p, int B, cudaStream_
   if (int rc = check_launch("kv4_decode_kernel", e)) return rc;
   if (p.alone && !(p.weights && p.chunks > 1)) return ATTN_OK;
   const int wc = p.weights ? (p.L + KD_WCHUNK - 1) / KD_WCHUNK : 1;
-  e = launch_pdl(kv4_decode_combine_kernel<T, D>, dim3((unsigned)wc * B * p.NKV), dim3(KC_THREADS), 0, s, p);
+  const dim3 cgrid((unsigned)wc * B * p.NKV), cblock(KC_THREADS);
+  e = p.weights ? launch_pdl(kv4_decode_combine_kernel<T, D, true>, cgrid, cblock, 0, s, p)
+                : launch_pdl(kv4_decode_combine_kernel<T, D, false>, cgrid, cblock, 0, s, p);
   count_launch();
   return check_launch("kv4_decode_combine_kernel", e);
 }
