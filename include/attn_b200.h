@@ -228,14 +228,13 @@ int attn_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
  * of g = min(D, 64).  A group keeps s = float16((max - min) / 15) and m = float16(min) (float32
  * arithmetic, the division as a product with the float32 nearest to 1/15, saturating at 65504) and, for
  * each x, the code n in 0..15 nearest to (x - m) / s in exact arithmetic, ties to even; it stands for
- * n*s + m.  A group holding an infinity or a NaN reads back as
- * NaN.
+ * n*s + m.  A group holding an infinity or a NaN reads back as NaN.
  *   codes   uint8   row r at codes + r * D/2: element d = 2i in the low nibble of byte i, 2i+1 in the high
  *   params  float16 row r at params + r * 2 * D/g: (s, m) of every group
  * Row r of (which, b, h, slot) is which*c_si + b*c_sb + h*c_sh + slot, which = 0 for keys and 1 for
  * values.  capacity (the slots of one head) and the strides, all in rows, are multiples of 16; both
  * arrays are 16-byte aligned.  int32 arrays of one entry per sequence live on the device, so that a
- * captured step reads them anew at every replay.
+ * captured step reads them anew at every replay.  Strides of what a call writes must keep its rows apart.
  *
  * attn_kv4_store quantises k and v (ATTN_F32 or ATTN_BF16, element (b, t, h, d) at
  * k[b*k_sb + t*k_st + h*k_sh + d]) into slots starts[b] + start + t, t < counts[b] (starts NULL: 0;

@@ -29,6 +29,11 @@ struct Kv4View {
   int cap;             // rows per (sequence, head)
 };
 
+// Whether [B, NH] rows of `len` elements at these strides are apart, so that CTAs may write them side by side.
+inline bool kv4_apart(int B, int NH, int64_t sb, int64_t sh, int64_t len) {
+  return (B == 1 || sb >= len) && (NH == 1 || sh >= len);
+}
+
 // Checks shared by the entry points that take a cache.
 int kv4_check(const char* fn, const Kv4View& c, int B, int NH, int D);
 

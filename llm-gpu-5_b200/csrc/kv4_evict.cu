@@ -9,15 +9,16 @@
 // cache moves one row.
 //
 // One CTA selects for one (sequence, head).  Up to 16,384 rows it holds every row's order key in registers,
-// consecutive rows to a thread, and finds the keep-th largest bit by bit from the top: 32 counts, each a
+// consecutive rows to a thread, and finds the keep-th largest bit by bit from the top: up to 32 counts, each a
 // warp reduction, one barrier and a sum over the warps (no atomics, so the weights' skewed exponents cost
 // nothing).  After about nine of them the undecided keys are few enough for one to a thread, and a count is a
-// barrier (730 cycles a round before, 50 after).  Longer sequences take a radix search, four passes of 8 bits over a histogram in shared memory.
-// Ties, holes and spare rows are numbered with block scans in slot order, and slots[i] = the row that slot i
-// holds afterwards (-1 past the kept ones).  The rows are then copied, codes in 16-byte pieces: by the same
-// CTA when there are few to move (one launch), else by a second kernel.  Measured for half of 32 x 8 heads of 8,192
-// rows of 64: select 22 us (instruction issue of the search, 60 % busy), move 34 us (150 MB, 71 % of DRAM's rate:
-// half of the rows come from scattered places); one of 513 rows of 12 heads: 11 us in one launch.
+// barrier (730 cycles a round before, 50 after).  Longer sequences take a radix search, four passes of 8 bits
+// over a histogram in shared memory.  Ties, holes and spare rows are numbered with block scans in slot order, and
+// slots[i] = the row that slot i holds afterwards (-1 past the kept ones).  The rows are then copied, codes in
+// 16-byte pieces: by the same CTA when there are few to move (one launch), else by a second kernel.  Measured for
+// half of 32 x 8 heads of 8,192 rows of 64: select 19 us (a third of it loading the weights, a third counting), move
+// 34 us (150 MB, 71 % of DRAM's rate: half of the rows come from scattered places); one of 513 rows of 12 heads:
+// 10 us in one launch.
 #include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
@@ -410,6 +411,8 @@ extern "C" int attn_kv4_evict(void* codes, void* params, float* weights, int* po
     return ATTN_ERR_WORKSPACE;
   }
   ATTN_REQUIRE(aligned(workspace, 4), "attn_kv4_evict: misaligned workspace");
+  ATTN_REQUIRE(kv4_apart(B, NH, w_sb, w_sh, L) && (in_place || kv4_apart(B, NH, dw_sb, dw_sh, keep)),
+               "attn_kv4_evict: rows of the weights must not overlap");
   if ((int64_t)B * NH * ((keep + 15) / 16) >= (int64_t)1 << 31) {
     set_error("attn_kv4_evict: B*NH*keep = %lld rows are too many for one call; split the batch", (long long)B * NH * keep);
     return ATTN_ERR_UNSUPPORTED;

@@ -289,6 +289,8 @@ extern "C" int attn_kv4_store(const void* k, const void* v, int dtype, int B, in
   const Kv4Rows r = {k, v, k_sb, k_st, k_sh, v_sb, v_st, v_sh, (uint32_t)T, (uint32_t)NH};
   const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
   ATTN_REQUIRE(c_si >= capacity && (B == 1 || c_sb >= capacity), "attn_kv4_store: cache rows must not overlap");
+  ATTN_REQUIRE(!(weights || positions) || kv4_apart(B, NH, w_sb, w_sh, capacity),
+               "attn_kv4_store: rows of weights and positions must not overlap");
   const Kv4Marks mk = {weights, positions, w_sb, w_sh, seen, seen0};
   return kv4_rows("attn_kv4_store", r, B, D, dtype, c, Kv4Slots{starts, start, counts}, &mk, as_stream(stream));
 }
