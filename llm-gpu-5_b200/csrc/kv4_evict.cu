@@ -350,11 +350,13 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) kv4_evict_move_kernel(const K
 
 template <int D>
 static int kv4_evict_d(Kv4Evict& p, int B, cudaStream_t s) {
-  // one launch where there is little to move: a CTA moves a thousand rows in a few microseconds, while half of
-  // 32 x 8 heads of 8,192 rows took 90 us in one launch (a CTA's registers leave it alone on its SM) and 67 in two
+  // one launch where there is little to move and few slots to look through: a CTA moves a thousand rows in a few
+  // microseconds, while half of 32 x 8 heads of 8,192 rows took 90 us in one launch (a CTA's registers leave it alone
+  // on its SM) and 67 in two, and one row out of 8 heads of 4,096 took 20.5 in one and 16.4 in two (16,000: 51 and
+  // 29; 2,048: 14.4 and 14.2, 128 heads of 2,048 14.8 and 16.4)
   const int rows = p.in_place ? (p.L - p.keep < p.keep ? p.L - p.keep : p.keep) : (p.L < p.keep ? p.L : p.keep);
   const int64_t heads = (int64_t)B * p.NH;
-  p.fused = rows <= 1024;
+  p.fused = rows <= 1024 && p.keep <= 2048;
   const dim3 grid((unsigned)heads), block(EV_THREADS);
   cudaError_t e;
   // the fewest rows per thread that hold the sequence: idle threads and wide loops both cost (256 heads of 4,000 rows:

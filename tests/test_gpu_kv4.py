@@ -624,6 +624,24 @@ def test_evict_without_positions_and_ragged_seen(ops):
     assert torch.equal(out[3].cpu()[:, :, :keep], want)
 
 
+@pytest.mark.parametrize("NH,L,out_of", [(2, 2050, 2), (2, 4100, 1), (1, 16500, 100), (3, 2049, 1)])
+def test_evict_a_few_rows_of_a_long_cache(ops, NH, L, out_of):
+    """In place, on both sides of the number of slots that one CTA looks through by itself."""
+    codes, params, w, pos = evict_state(ops, 1, NH, 32, L, seed=L)
+    keep, seen = L - out_of, 2 * codes.shape[3]
+    src = [t.cpu() for t in (codes, params, w, pos)]
+    slots = ops.kv4_evict(codes, params, w, pos, L, keep, recent=8, seen=seen)
+    want = torch.tensor([[evict_plain(src[2][0, h].tolist(), src[3][0, h].tolist(), L, keep, seen - 8) for h in range(NH)]],
+                        dtype=torch.int32)
+    assert torch.equal(slots.cpu(), want)
+    for h in range(NH):
+        at = want[0, h].long()
+        assert torch.equal(codes.cpu()[:, 0, h, :keep], src[0][:, 0, h, at])
+        assert torch.equal(params.cpu()[:, 0, h, :keep], src[1][:, 0, h, at])
+        assert torch.equal(w.cpu()[0, h, :keep].view(torch.int32), src[2][0, h, at].view(torch.int32))
+        assert torch.equal(pos.cpu()[0, h, :keep], src[3][0, h, at])
+
+
 # ------------------------------------------------------------------------------------ refusals on a device
 def test_wrapper_refusals(ops):
     codes, params = make_cache(ops, 2, 2, 20, 64, seed=1)
