@@ -545,7 +545,7 @@ static int key_weights_tc(const KeyWeights& p, int B, int tf32, float* partial, 
 using namespace attn;
 
 extern "C" size_t attn_key_weights_workspace_size(int B, int NKV, int T) {
-  if (B <= 0 || NKV <= 0 || T <= 0) return 0;
+  if (B <= 0 || NKV <= 0 || T <= 0 || T > 1 << 30) return 0;
   // whichever kernel the tensors suit
   const int tc = key_weights_parts(B, NKV, T, AT_TILE, KW_CTAS), simt = key_weights_parts(B, NKV, T, KW_TILE, KW_CTAS);
   const int parts = tc > simt ? tc : simt;
@@ -572,6 +572,7 @@ extern "C" int attn_key_weights(const void* q, const void* k, const float* lse, 
     set_error("attn_key_weights: head_dim %d not supported (up to 128)", D);
     return ATTN_ERR_UNSUPPORTED;
   }
+  ATTN_REQUIRE(T <= 1 << 30, "attn_key_weights: T = %d exceeds 2^30", T);  // rows are ints with room to round up
   if ((int64_t)B * NKV * ((T + KW_TILE - 1) / KW_TILE) >= (int64_t)1 << 30) {
     set_error("attn_key_weights: too many key tiles for one launch; split the batch into several calls");
     return ATTN_ERR_UNSUPPORTED;

@@ -772,7 +772,7 @@ static KdPlan kd_plan(int B, int NH, int NKV, int L, int D, int dtype, int weigh
   k.ns = k.cluster ? ns : (L + k.per - 1) / k.per;
   k.alone = k.cluster || k.ns == 1;
   // where a key head's queries take more than one CTA (chunks), the combine kernel adds their weights
-  k.zsmem = weights && k.alone && k.chunks == 1 && k.nq * k.per <= KD_ZFLOATS;
+  k.zsmem = weights && k.alone && k.chunks == 1 && (int64_t)k.nq * k.per <= KD_ZFLOATS;
   k.states = k.alone ? (weights && k.chunks > 1 ? (size_t)B * NH * 2 : 0) : (size_t)B * NH * k.ns * (D + 2);
   k.states = (k.states + 3) / 4 * 4;
   k.scores = weights && !k.zsmem ? (size_t)B * NH * L : 0;

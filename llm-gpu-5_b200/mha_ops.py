@@ -351,10 +351,10 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
         wsb, wsh = osb, osh
     lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
     code = dtype_code(q.dtype)
-    need = _workspace_bytes("attn_kv4_decode_workspace_size", _current_device(), B, NH, NKV, length, D, code, w_out is not None)
-    workspace, ws, ws_bytes = _scratch(workspace, need, q)
     before = _other_device(dev)
     try:
+        need = _workspace_bytes("attn_kv4_decode_workspace_size", dev.index, B, NH, NKV, length, D, code, w_out is not None)
+        workspace, ws, ws_bytes = _scratch(workspace, need, q)
         rc = lib.attn_kv4_decode(q.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(),
                                  lse.data_ptr() if lse is not None else None, B, NH, NKV, length, D, qs[0], qs[1], os_[0], os_[1], si, sb, sh,
                                  cap, lengths_p, w_in, w_out, wsb, wsh, 1.0 / math.sqrt(D) if scale is None else float(scale),

@@ -94,6 +94,7 @@ def test_bad_caches_are_refused(call, bad, code, text):
     (_decode, dict(o_sh=0), ARG, "overlap"), (_weights, dict(w_sh=0), ARG, "overlap"), (_evict, dict(w_sb=0), ARG, "overlap"),
     (_store, dict(weights=FAKE, w_sb=32, w_sh=8), ARG, "overlap"), (_store, dict(positions=FAKE), ARG, "overlap"),
     (_weights, dict(q=None), ARG, "null"), (_weights, dict(w_out=None), ARG, "null"), (_weights, dict(dtype=5), ARG, "dtype"),
+    (_weights, dict(T=(1 << 30) + 1, w_sh=1 << 31, w_sb=1 << 32), ARG, "2^30"),
     (_weights, dict(NH=3), ARG, "multiple"), (_weights, dict(first=-1), ARG, "first_query"), (_weights, dict(T=0), ARG, "positive"),
     (_weights, dict(D=160), UNSUPPORTED, "head_dim"), (_weights, dict(T=4096, w_sh=4096, ws_bytes=4), WORKSPACE, "workspace"), (_weights, dict(k_st=-1), ARG, "negative"),
     (_evict, dict(weights=None), ARG, "null"), (_evict, dict(slots=None), ARG, "null"), (_evict, dict(L=17), ARG, "length"),
