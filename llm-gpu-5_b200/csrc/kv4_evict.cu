@@ -8,7 +8,7 @@
 // slot < keep, so the move can run in place with every row in parallel, and evicting one row of a full
 // cache moves one row.
 //
-// One CTA selects for one (sequence, head).  Up to 16,384 rows it holds every row's order key in registers,
+// One CTA selects for one (sequence, head).  Up to 32,768 rows it holds every row's order key in registers,
 // consecutive rows to a thread, and finds the keep-th largest bit by bit from the top: up to 32 counts, each a
 // warp reduction, one barrier and a sum over the warps (no atomics, so the weights' skewed exponents cost
 // nothing).  After about nine of them the undecided keys are few enough for one to a thread, and a count is a
@@ -29,7 +29,8 @@ namespace attn {
 constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MOVE_THREADS = 256;
-constexpr int EV_MOST = 32;  // rows per thread of the register select
+constexpr int EV_MOST = 64;  // rows per thread of the register select
+constexpr int EV_SHARED = 32;  // up to here its lists are in shared memory, beyond in the workspace
 
 struct Kv4Evict {
   Kv4View src, dst;
@@ -160,7 +161,11 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
     const int64_t protect_from = seq_value(p.seen, b, p.seen0) - p.recent;
     if constexpr (PER > 0) {
       const int base = threadIdx.x * PER;
-      __shared__ uint16_t holes[EV_THREADS * PER / 2], spare[EV_THREADS * PER / 2];  // at most min(keep, n - keep)
+      // at most min(keep, n - keep) each
+      constexpr int LIST = PER <= EV_SHARED ? EV_THREADS * PER / 2 : 1;
+      __shared__ uint16_t s_holes[LIST], s_spare[LIST];
+      uint16_t* holes = PER <= EV_SHARED ? s_holes : reinterpret_cast<uint16_t*>(p.spare + (int64_t)bh * 2 * p.keep);
+      uint16_t* spare = PER <= EV_SHARED ? s_spare : holes + p.keep;
       uint32_t key[PER];
       const bool wide = PER % 4 == 0 && row_w % 4 == 0 && (reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.pos)) % 16 == 0;
       if (wide && base + PER <= n) {
@@ -230,7 +235,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
       const int ties = p.keep - block_total(__reduce_add_sync(0xffffffffu, above), red[0]);
       int total;
       int rank = block_scan(tie, red[1], &total);
-      uint32_t kept = 0;
+      typename std::conditional<(PER <= 32), uint32_t, uint64_t>::type kept = 0;
       int count = 0;  // holes, and spare rows in the upper half
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_select_kernel(const Kv4E
         const bool same = j < n && key[k] == limit;
         const bool stay = j < n && (key[k] > limit || (same && rank < ties));
         rank += same;
-        kept |= (uint32_t)stay << k;
+        kept |= (decltype(kept))stay << k;
         if (j < n && j < p.keep && !stay) count += 1;
         if (j >= p.keep && stay) count += 1 << 16;
       }
@@ -360,11 +365,13 @@ static int kv4_evict_d(Kv4Evict& p, int B, cudaStream_t s) {
   const dim3 grid((unsigned)heads), block(EV_THREADS);
   cudaError_t e;
   // the fewest rows per thread that hold the sequence: idle threads and wide loops both cost (256 heads of 4,000 rows:
-  // 18 us with 16 a thread, of 10,330 rows 40 us with 32)
+  // 18 us with 16 a thread, of 10,330 rows 40 us with 32; one row
+  // out of 8 heads of 32,000: 70 us with 64, 209 with the passes over memory)
   if (p.L <= EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 1>, grid, block, 0, s, p);
   else if (p.L <= 4 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 4>, grid, block, 0, s, p);
   else if (p.L <= 8 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 8>, grid, block, 0, s, p);
   else if (p.L <= 16 * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, 16>, grid, block, 0, s, p);
+  else if (p.L <= EV_SHARED * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, EV_SHARED>, grid, block, 0, s, p);
   else if (p.L <= EV_MOST * EV_THREADS) e = launch_pdl(kv4_evict_select_kernel<D, EV_MOST>, grid, block, 0, s, p);
   else e = launch_pdl(kv4_evict_select_kernel<D, 0>, grid, block, 0, s, p);
   count_launch();
@@ -382,7 +389,7 @@ using namespace attn;
 
 extern "C" size_t attn_kv4_evict_workspace_size(int B, int NH, int L, int keep) {
   if (B <= 0 || NH <= 0 || L <= 0 || keep <= 0) return 0;
-  return L <= attn::EV_MOST * attn::EV_THREADS ? 0 : (size_t)B * NH * 2 * keep * sizeof(int);
+  return L <= attn::EV_SHARED * attn::EV_THREADS ? 0 : (size_t)B * NH * 2 * keep * sizeof(int);
 }
 
 extern "C" int attn_kv4_evict(void* codes, void* params, float* weights, int* positions, int64_t c_si, int64_t c_sb,

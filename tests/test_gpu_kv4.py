@@ -555,6 +555,7 @@ EVICTIONS = [
     (2, 2, 128, 1500, 700, 100, [1500, 701]), (1, 1, 64, 5000, 4999, 0, None), (2, 1, 64, 64, 64, 8, None),
     (1, 3, 32, 40000, 20000, 64, None), (1, 2, 16, 33, 40, 2, None), (1, 2, 32, 3000, 1000, 30, None),
     (1, 1, 64, 12000, 7000, 100, None), (2, 1, 16, 9000, 8999, 8999, [9000, 8999]),
+    (1, 2, 32, 32768, 16384, 64, None), (2, 1, 16, 20001, 9999, 7, [20001, 9000]), (1, 1, 64, 32769, 30000, 0, None),
 ]
 
 
