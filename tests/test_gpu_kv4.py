@@ -494,6 +494,20 @@ def test_prompt_weights_match_plain(ops, kind, B, NH, NKV, T, D, first, lengths)
 
 
 @pytest.mark.parametrize("kind", ["fp32", "tf32", "bf16"])
+@pytest.mark.parametrize("T,D,pad,shift", [(150, 5, 0, 0), (70, 128, 1, 0), (200, 20, 0, 1), (65, 127, 0, 0), (300, 12, 4, 0)])
+def test_prompt_weights_of_unaligned_rows(ops, kind, T, D, pad, shift):
+    """Odd head_dim, rows whose stride is no multiple of four elements, and tensors that start off an alignment."""
+    dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+    B, NH, scale = 2, 2, 1 / math.sqrt(D)
+    gen = torch.Generator().manual_seed(T + D)
+    x = torch.randn((2 * B * T * NH * (D + pad) + shift,), generator=gen).to(dtype).cuda()[shift:].view(2, B, T, NH, D + pad)[..., :D]
+    z = torch.einsum("bihd,bjhd->bhij", x[0].double(), x[1].double()) * scale
+    lse = z.masked_fill(torch.ones((T, T), dtype=torch.bool, device="cuda").triu(1), -math.inf).logsumexp(-1).float().contiguous()
+    w, e = prompt_plain(x[0], x[1], lse, scale, 3, None, kind == "tf32")
+    within(ops.key_weights(x[0], x[1], lse, first_query=3, dtype="tf32" if kind == "tf32" else None), w, e, "weights")
+
+
+@pytest.mark.parametrize("kind", ["fp32", "tf32", "bf16"])
 def test_prompt_weights_ignore_the_padding(ops, kind):
     """Whatever lies behind a sequence's last token (queries, keys, lse: NaN and infinities here) reaches
     no weight, and the weights there are 0."""
