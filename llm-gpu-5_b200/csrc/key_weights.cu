@@ -437,18 +437,28 @@ key_weights_tc_kernel(const __grid_constant__ KwMaps maps, const KwWork a) {
             if (lane == 0) mbar_arrive(&bars->s_free[buf]);
           }
           if (cc * 32 + 32 <= c0_any) continue;  // before every lane's first query
-          if (cc * 32 < c0_all || cc * 32 + 32 > c1) {
-            // unused scores may be anything, NaN too: they are replaced, not multiplied
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (k < c0 - cc * 32 || k >= c1 - cc * 32) x[k] = 0xff800000u;  // -inf, its exponential 0
-          }
           const ulonglong2* l2 = reinterpret_cast<const ulonglong2*>(lb + cc * 32);
+          uint64_t y[16];  // the exponentials' arguments
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const ulonglong2 l = l2[k];
-            add2(sum[0], ex2_pair(fma2(pair(x[4 * k], x[4 * k + 1]), cpair, l.x)));
-            add2(sum[1], ex2_pair(fma2(pair(x[4 * k + 2], x[4 * k + 3]), cpair, l.y)));
+            y[2 * k] = fma2(pair(x[4 * k], x[4 * k + 1]), cpair, l.x);
+            y[2 * k + 1] = fma2(pair(x[4 * k + 2], x[4 * k + 3]), cpair, l.y);
+          }
+          if (cc * 32 < c0_all || cc * 32 + 32 > c1) {
+            // the whole argument is replaced (by -inf, whose exponential is 0): where a column does not count, the
+            // score, the query's lse and the scale's sign may be anything
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int c = cc * 32 + 2 * k;
+              y[k] = pair(c < c0 || c >= c1 ? 0xff800000u : (uint32_t)y[k],
+                          c + 1 < c0 || c + 1 >= c1 ? 0xff800000u : (uint32_t)(y[k] >> 32));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            add2(sum[0], ex2_pair(y[k]));
+            add2(sum[1], ex2_pair(y[k + 1]));
           }
         }
         total += pair_sum(sum[0]) + pair_sum(sum[1]);

@@ -1,0 +1,78 @@
+"""The 4-bit cache operators where they went wrong once: numbers that are not finite in places a mask
+leaves out, scales of zero and below.
+
+Bounds on errors are those derived in test_gpu_kv4.py (u = 2^-24), or stand beside the test."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv4 import U, prompt_plain, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(pkg, cuda_dev):
+    return pkg.mha_ops
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------ prompt weights
+KINDS = ["fp32", "tf32", "bf16"]
+
+
+def prompt(kind, B, T, NH, NKV, D, scale, seed):
+    """q, k, and the lse of a causal softmax of these scores, whatever the scale."""
+    dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+    gen = torch.Generator().manual_seed(seed)
+    qk = torch.randn((B, T, NH + NKV, D), generator=gen).to(dtype).cuda()
+    q, k = qk[:, :, :NH], qk[:, :, NH:]
+    z = torch.einsum("bihd,bjhd->bhij", q.double(), k.repeat_interleave(NH // NKV, dim=2).double()) * scale
+    z = z.masked_fill_(torch.ones((T, T), dtype=torch.bool, device="cuda").triu_(1), -math.inf)
+    return q, k, z.logsumexp(-1).float().contiguous()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
+def test_prompt_weights_at_any_scale(ops, kind, scale):
+    B, T, NH, NKV, D = 2, 300, 4, 2, 32
+    q, k, lse = prompt(kind, B, T, NH, NKV, D, scale, 11)
+    mode = "tf32" if kind == "tf32" else None
+    for first, lengths in ((0, None), (77, None), (0, [300, 131])):
+        w, _ = prompt_plain(q, k, lse, scale, first, lengths, kind == "tf32")
+        # every score's sums of magnitudes are below a
+        a = (q.float().abs().amax() * k.float().abs().amax()).item() * D * abs(scale) + float(lse.abs().max())
+        bound = U * ((D + 8) * a + 16) * w + (T / 16 + 64) * U * w
+        got = ops.key_weights(q, k, lse, scale=scale, first_query=first, lengths=i32(lengths) if lengths else None, dtype=mode)
+        within(got, w, bound, (scale, first, lengths))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,first", [(300, 150), (129, 128), (600, 33)])
+@pytest.mark.parametrize("poison", [float("nan"), float("-inf"), float("inf")])
+def test_prompt_weights_never_look_at_queries_before_the_first(ops, kind, T, first, poison):
+    """Queries in front of first_query, and their lse, may hold anything."""
+    q, k, lse = prompt(kind, 1, T, 2, 2, 32, 32 ** -0.5, T)
+    mode = "tf32" if kind == "tf32" else None
+    clean = ops.key_weights(q, k, lse, first_query=first, dtype=mode)
+    q[:, :first], lse[:, :, :first] = float("nan"), poison
+    got = ops.key_weights(q, k, lse, first_query=first, dtype=mode)
+    assert bool(torch.isfinite(clean).all()) and torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("poison", [float("nan"), float("-inf")])
+def test_prompt_weights_of_a_bad_query_stay_before_it(ops, kind, poison):
+    """A query whose lse is not finite poisons the keys that it sees, and none behind it."""
+    T, at = 300, 141
+    q, k, lse = prompt(kind, 1, T, 2, 2, 32, 32 ** -0.5, 5)
+    mode = "tf32" if kind == "tf32" else None
+    clean = ops.key_weights(q, k, lse, dtype=mode)
+    q[0, at, 1], lse[0, 1, at] = float("nan"), poison
+    got = ops.key_weights(q, k, lse, dtype=mode)
+    assert torch.equal(got[0, 0], clean[0, 0]) and torch.equal(got[0, 1, at + 1:], clean[0, 1, at + 1:])
+    assert not bool(torch.isfinite(got[0, 1, :at + 1]).any())
