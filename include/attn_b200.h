@@ -286,8 +286,9 @@ size_t attn_key_weights_workspace_size(int B, int NKV, int T);
  * from lengths[b] on get weights_in.  q: element (b, t, h, d) at q[b*q_sb + t*q_st + h*q_sh + d], k
  * likewise; element (b, h, j) of the weights at b*w_sb + h*w_sh + j.  head_dim up to 128.  ATTN_BF16 with
  * head_dim a multiple of 8 up to 64 and ATTN_TF32 with a multiple of 4 up to 32 (16-byte aligned, strides in
- * 16-byte steps) run on the tensor cores, the rest on CUDA cores; ATTN_TF32 truncates q and k to tf32 either
- * way, as attn_fwd's tf32 path reads them.
+ * 16-byte steps) run on the tensor cores, the rest on CUDA cores.  ATTN_TF32 truncates q and k to tf32 either
+ * way.  attn_fwd does so only where ATTN_TF32 runs on its tensor cores (head_dim a multiple of 4 up to 32, q, k, v and
+ * o aligned for it): an lse that it wrote on CUDA cores goes with ATTN_F32 here.
  */
 int attn_key_weights(const void* q, const void* k, const float* lse, const float* weights_in,
                      float* weights_out, int B, int NH, int NKV, int T, int D,

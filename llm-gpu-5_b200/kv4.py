@@ -61,6 +61,10 @@ class KV4Cache:
         B, T, _ = qkv.shape
         x = qkv.view(B, T, 3, self.NH, self.D)
         first = 0 if self.prompt_window is None else max(0, T - self.prompt_window)
+        # the tf32 forward truncates its scores' operands on tensor cores only, up to head_dim 32 (the projection's
+        # layout always suits them); wider heads run in float32, and so do their weights
+        if dtype == "tf32" and self.D > 32:
+            dtype = torch.float32
         ops.key_weights(x[:, :, 0], x[:, :, 1], lse, first_query=first, weights=self.weights[:, :, :T], dtype=dtype)
 
     def attend(self, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -375,7 +375,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
     q [B, T, NH, D], k [B, T, NKV, D] (NH / NKV query heads to a key head), lse [B, NH, T] from
     ``attention_forward``: each key's attention weight summed over the queries from ``first_query``
     on (those from ``lengths[b]`` on excluded) and its query heads, added to ``weights`` when given.
-    ``dtype`` "tf32" for an lse that came from the tf32 forward."""
+    ``dtype`` "tf32" takes q and k truncated to tf32, for an lse of the tf32 forward on tensor cores (head_dim
+    a multiple of 4 up to 32, aligned rows); its other layouts run in float32, and so must their weights."""
     if q.dim() != 4 or k.dim() != 4 or q.dtype != k.dtype:
         raise ValueError("key_weights: expected q [B, T, NH, D] and k [B, T, NKV, D] of one dtype")
     B, T, NH, D = q.shape

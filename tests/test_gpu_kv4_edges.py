@@ -1,9 +1,10 @@
 """The 4-bit cache operators where they went wrong once: numbers that are not finite in places a mask
-leaves out, scales of zero and below.
+leaves out, scales of zero and below, the tf32 module's prompt weights.
 
 Bounds on errors are those derived in test_gpu_kv4.py (u = 2^-24), or stand beside the test."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -76,3 +77,25 @@ def test_prompt_weights_of_a_bad_query_stay_before_it(ops, kind, poison):
     got = ops.key_weights(q, k, lse, dtype=mode)
     assert torch.equal(got[0, 0], clean[0, 0]) and torch.equal(got[0, 1, at + 1:], clean[0, 1, at + 1:])
     assert not bool(torch.isfinite(got[0, 1, :at + 1]).any())
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_tf32_module_weights_match_its_forward(pkg, ops, D):
+    """Every query's tracked weights add up to one against the lse of the module's own forward.
+
+    p = exp(z - lse): z and the forward's scores are float32 sums of D products below A = scale sum |q||k| (each off by
+    at most u (D + 16) A, the forward's tf32 products at head_dim 32 being the same as these), the approximate
+    exponentials are off by 2^-21 each side with their argument's 2 u (A + |lse|), the sums by (T / 16 + 64) u."""
+    B, T, NH = 1, 400, 2
+    C = NH * D
+    np.random.seed(7)
+    attn = pkg.MultiHeadAttention(pkg.GPTConfig(vocab_size=50, embedding_dim=C, num_heads=NH, attention_precision="tf32"))
+    attn.c_attn_w.weights.mul_(300.0 / math.sqrt(C))  # scores up to about 100
+    cache = attn.new_kv_cache(B, T, bits=4, track_weights=True)
+    x = torch.randn((B, T, C), generator=torch.Generator().manual_seed(3)).cuda()
+    attn.forward(x.view(-1), B, T, kv_cache=cache)
+    qkv = attn._cache["qkv"].view(B, T, 3, NH, D).double()
+    A = torch.einsum("bihd,bjhd->bhij", qkv[:, :, 0].abs(), qkv[:, :, 1].abs()).tril_().amax(-1) / math.sqrt(D)
+    rho = 2 * U * (D + 16) * A + 4 * U * (2 * A + 1) + 2.0 ** -20 + 2 * (T / 16 + 64) * U
+    total = cache.weights[:, :, :T].double().sum(-1)
+    assert bool(((total - T).abs() <= rho.sum(-1)).all()), (total - T, rho.sum(-1))
