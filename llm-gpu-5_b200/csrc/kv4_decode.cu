@@ -735,7 +735,8 @@ __global__ void __launch_bounds__(KC_THREADS, WEIGHTS ? 2 : 6) kv4_decode_combin
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int j = j0 + i * KC_THREADS;
-      if (j < p.L) p.w_out[w0 + j] = have[i] + w[i];
+      // (behind the rows w is 0 times the reciprocal sums, NaN where one of them is)
+      if (j < p.L) p.w_out[w0 + j] = j < n ? have[i] + w[i] : have[i];
     }
   }
 }

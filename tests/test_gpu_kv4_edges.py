@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv4 import U, prompt_plain, within
+from test_gpu_kv4 import U, make_cache, prompt_plain, within
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,22 @@ def test_tf32_module_weights_match_its_forward(pkg, ops, D):
     rho = 2 * U * (D + 16) * A + 4 * U * (2 * A + 1) + 2.0 ** -20 + 2 * (T / 16 + 64) * U
     total = cache.weights[:, :, :T].double().sum(-1)
     assert bool(((total - T).abs() <= rho.sum(-1)).all()), (total - T, rho.sum(-1))
+
+
+# ------------------------------------------------------------------------------------ decode
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,NH,NKV,L", [(2, 2, 1, 300), (1, 1, 1, 20000), (70, 16, 8, 600), (2, 18, 2, 40), (2, 18, 2, 9000)])
+def test_bad_queries_leave_the_weights_behind_the_rows(ops, dtype, B, NH, NKV, L):
+    """Slots from a sequence's length on keep their weights whatever the queries hold (one launch, clusters, the
+    combine kernel, several CTAs of query heads)."""
+    codes, params = make_cache(ops, B, NKV, L, 64, seed=L)
+    q = torch.randn((B, NH, 64), generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    q[0, 0, 5] = float("nan")
+    q[-1, -1, 0] = float("inf")
+    w = torch.rand((B, NKV, codes.shape[3]), generator=torch.Generator().manual_seed(3)).cuda()
+    before = w.clone()
+    lens = [(L // 3 + 13 * b) % L for b in range(B)]
+    ops.kv4_decode(q, codes, params, L, lengths=i32(lens), weights=w)
+    for b in range(B):
+        assert torch.equal(w[b, :, lens[b]:], before[b, :, lens[b]:]), b
+    assert bool(torch.isnan(w[0, 0, :lens[0]]).all()) and bool(torch.isnan(w[-1, -1, :lens[-1]]).all())
