@@ -19,17 +19,20 @@
 //     of bfloat16 ones the second, and their value product (the output keeps 2^-9) the third.
 //   - which element sits in which k slot does not matter as long as the query agrees, so a lane takes
 //     consecutive codes of a key's row.
-//   - q is scaled by a power of two to below 2^12 and p s to below 2^15, which keeps float16's 11 bits at
-//     2^-35 of the largest and above.  bfloat16 queries are exact.  float32 ones go as two float16 parts
-//     in two columns of the same product, and so does p s for a float32 output (its second part 2^11
-//     times too large, so that small weights keep it too), so their products are good to 2^-22.
+//   - q is scaled by a power of two to below 2^12: bfloat16 elements are exact down to 2^-28 of the row's largest,
+//     smaller ones off by at most 2^-36 of it.  float32 ones go as two float16 parts in two columns of the same
+//     product (good to 2^-22 of themselves or 2^-36 of the largest).
+//   - p s is formed with p relative to a reference, in place of the scores' maximum, that keeps the largest p s of a
+//     query and group between 2^7 and 2^15.  So what a row's scale costs the others in digits follows from p s, their
+//     shares of the output: each keeps 11 bits down to 2^-22 of the largest, and is off by at most 2^-32 of it below
+//     (float32 outputs: 22 bits in two parts, the second 2^11 times too large so that small ones keep it too).
 //
 // A warp takes tiles of 64 keys (32 at head_dim 128) through a ring of its own of cp.async stages (no barrier
-// between warps): scores into shared memory, then one key per lane for the softmax, whose running maximum
-// moves only when it grows by more than 2^8 (the accumulators are rescaled then), then p s back as the B
-// operand.  The length is split over the CTAs of a cluster, up to eight, which merge their states (m, l, o[D])
-// through distributed shared memory and add the weights of their own keys: one launch, where the GPU holds all
-// clusters at once.  Otherwise (many heads, or few over long sequences) the splits write their states to the
+// between warps): scores into shared memory, then one key per lane for the softmax, whose reference moves only
+// when a p s passes 2^15 (the accumulators are rescaled then; a vote per tile finds that out, cheaper than every
+// query's maximum), then p s back as the B operand.  The length is split over the CTAs of a cluster, up to eight,
+// which merge their states (m, l, o[D]) through distributed shared memory and add the weights of their own keys: one
+// launch, where the GPU holds all clusters at once.  Otherwise (many heads, or few over long sequences) the splits write their states to the
 // workspace for a combine kernel.  Measured: 32 x 12 heads of 16,384 rows with weights 88 us for this kernel
 // (453 MB of cache and 25 of scores, 84 % of the copy rate) and 22 for the combine kernel; 64 x 8 heads of 2,048
 // rows 22-25 us; 8 x 8 float32 heads of 4,099 rows of 32 in one launch of clusters, 13 us with the host's part.
@@ -44,6 +47,12 @@ constexpr int KD_THREADS = KD_WARPS * 32;
 constexpr int KD_WCHUNK = 4096;  // keys per combine CTA
 constexpr int KD_SPLIT = 64 * KD_WARPS;  // keys a CTA takes at least, where there are so many
 constexpr int KD_CLUSTER = 8;            // most CTAs of a cluster (the portable limit)
+// A tile whose p s and p stay below these keeps its references.  A scale s counts as the power of two above it, 0 as
+// the smallest of float16's, 2^-23, and one that is not finite as the largest: p reaches 2^39 only where p s as counted passes 2^15.  Sums of p stay far
+// below float32's largest, and a reference lies at most 39 below and 16 above the largest score, so that what is
+// flushed, 2^-126 of the reference, is nothing beside it.
+constexpr float KD_MOST_P = 0x1p39f, KD_MOST_PS = 0x1p15f;
+constexpr int KD_LEAST_SCALE = -23, KD_MOST_SCALE = 16;
 
 struct Kv4Decode {
   const void* q;
@@ -59,7 +68,7 @@ struct Kv4Decode {
   int nq, chunks;  // query heads per CTA, and CTAs' chunks of them per key head
   float scale_log2;
   int alone;       // this kernel finishes o and lse
-  float* states;  // [B*NH][ns][D + 2]: max (log2 units), sum, unnormalised o; alone, [B*NH][2]: max and sum
+  float* states;  // [B*NH][ns][D + 2]: reference of p (log2 units), sum, unnormalised o; alone, [B*NH][2]: reference and sum
   float* scores;  // [B*NH][L]: scores in log2 units, where they do not fit beside the CTA's other shared memory
   int weights;    // whether weights are wanted
   int zsmem;      // the scores of the CTA's keys stay in shared memory
@@ -86,6 +95,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The exponent of a normal number.
+__device__ __forceinline__ int kd_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255u) - 127; }
 
 // max over the warp (NaN ignored)
 __device__ __forceinline__ float warp_max(float x) {
@@ -196,6 +213,9 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   using S = KdTile<D, NQ, F32>;
   constexpr int GROUPS = S::GROUPS, GS = kv4_group(D), KD_TILE = S::TILE, PL = KD_TILE / 32;  // PL keys per lane
   constexpr int KPLACE = F32 ? KD_TOP : KD_SECOND, VPLACE = F32 ? KD_TOP : KD_INPLACE;
+  // scores are formed again where the reference moves, in place of being kept in registers until then: eight queries
+  // of head_dim 128 have none left (16 x 64 heads over 8 of up to 8,191 rows: 51.4 -> 48.5 us; elsewhere it costs up to 4 %)
+  constexpr bool AGAIN = GROUPS == 2 && NQ == 8;
   constexpr int MT = D / 16;   // 16-row tiles of the value product
   constexpr int KS = D / 16;   // 16-deep steps of the score product
   extern __shared__ __align__(16) uint8_t smem[];
@@ -328,7 +348,11 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[i][k] = 0.f;
-  int ve = -100;  // exponent that the accumulated p s are scaled by: the largest value scale seen
+  // m: the reference that p is relative to (log2 units); head_dim 128's second group has one of its own, log2(ratio)
+  // below it, so that its p are the first's times `ratio`
+  float ratio[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) ratio[q] = 1.f;
 
   for (int i = 0; i * KD_WARPS + warp < tiles; ++i) {
     fetch(i + S::STAGES - 1);
@@ -403,7 +427,6 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     // ---- softmax: key lane of every 32 of the tile ----
     float ks[PL][GROUPS], km[PL][GROUPS], vs[PL][GROUPS], vm[PL][GROUPS];
     bool valid[PL];
-    float vbig = 0.f;
 #pragma unroll
     for (int u = 0; u < PL; ++u) {
       const int key = u * 32 + lane;
@@ -414,80 +437,110 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
         ks[u][k] = a.x; km[u][k] = a.y;
         vs[u][k] = valid[u] ? v.x : 0.f;
         vm[u][k] = valid[u] ? v.y : 0.f;
-        vbig = fmaxf(vbig, vs[u][k]);
       }
     }
-    float z[NQ][PL];
-    bool grow = false;
-    float top[NQ];
+    auto score = [&](int q, int u) {
+      const float raw = sc[q * S::SC_LD + u * 32 + lane] * sfac[q];
+      float s = GROUPS == 1 ? raw * ks[u][0] : raw;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const float f = sfac[q];
+      for (int k = 0; k < GROUPS; ++k) s = fmaf(km[u][k], ssum[q * GROUPS + k], s);
+      return valid[u] ? s : -INFINITY;
+    };
+    float z[NQ][PL];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
 #pragma unroll
       for (int u = 0; u < PL; ++u) {
-        const float raw = sc[q * S::SC_LD + u * 32 + lane] * f;
-        float s = GROUPS == 1 ? raw * ks[u][0] : raw;
-#pragma unroll
-        for (int k = 0; k < GROUPS; ++k) s = fmaf(km[u][k], ssum[q * GROUPS + k], s);
-        z[q][u] = valid[u] ? s : -INFINITY;
+        z[q][u] = score(q, u);
+        if (AGAIN && p.weights && valid[u] && q < nq) zrow[q * zld + j + u * 32 + lane] = z[q][u];
       }
-      top[q] = warp_max(fmaxf(z[q][0], z[q][PL - 1]));
-      grow = grow || top[q] > m[q] + 8.f;
+    // p, and a lane's two p s of a query: of its key's two groups, or of its two keys (PL * GROUPS is 2)
+    float e[NQ][PL], x[NQ][2], most_e = 0.f;
+    __half2 h[NQ], most = __floats2half2_rn(0.f, 0.f);
+    auto weigh = [&](int q) {
+#pragma unroll
+      for (int u = 0; u < PL; ++u) e[q][u] = valid[u] ? ex2(z[q][u] - m[q]) : 0.f;
+      x[q][0] = e[q][0] * vs[0][0];
+      x[q][1] = GROUPS == 1 ? e[q][PL - 1] * vs[PL - 1][0] : e[q][0] * ratio[q] * vs[0][GROUPS - 1];
+      h[q] = __floats2half2_rn(x[q][0], x[q][1]);
+    };
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      weigh(q);
+      most_e = fmax3(most_e, e[q][0], e[q][PL - 1]);  // (NaN ignored, here and below)
+      most = __hmax2(most, h[q]);
     }
-    vbig = warp_max(vbig);
-    const int be = max((int)((__float_as_uint(vbig) >> 23) & 255u) - 127, -100);
-    if (grow || be > ve) {  // (warp-uniform) move the maxima, the values' exponent, and what was summed
-      const int ne = max(ve, be);
-      float corr[NQ];
+    if (__any_sync(0xffffffffu, !(most_e < KD_MOST_P && __low2float(most) < KD_MOST_PS && __high2float(most) < KD_MOST_PS))) {
+      // (warp-uniform) new references, 2^6 above what is needed, and what was summed with the old ones
+      float f[NQ][GROUPS];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        const float nm = top[q] > m[q] + 8.f ? top[q] : m[q];
-        corr[q] = m[q] == -INFINITY ? 0.f : ex2(m[q] - nm);
-        m[q] = nm;
-        l[q] *= corr[q];
+        if constexpr (AGAIN)
 #pragma unroll
-        for (int k = 0; k < GROUPS; ++k) mg[q][k] *= corr[q];
+          for (int u = 0; u < PL; ++u) z[q][u] = score(q, u);
+        float ref[GROUPS];
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+          const float old = k ? m[q] - lg2(ratio[q]) : m[q];
+          float t = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < PL; ++u)
+            t = fmaxf(t, z[q][u] + (float)min(max(kd_exponent(vs[u][k]) + 1, KD_LEAST_SCALE), KD_MOST_SCALE));
+          t = warp_max(t);
+          ref[k] = t > old + 15.f ? t - 9.f : old;
+        }
+        f[q][0] = m[q] == -INFINITY ? 0.f : ex2(m[q] - ref[0]);
+        if constexpr (GROUPS == 2) {
+          const float now = ref[0] == -INFINITY ? 1.f : ex2(ref[0] - ref[1]);
+          f[q][1] = f[q][0] * __fdividef(now, ratio[q]);
+          ratio[q] = now;
+        }
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) mg[q][k] *= f[q][0];
+        m[q] = ref[0];
+        l[q] *= f[q][0];
+        weigh(q);
       }
-      const float ve_corr = ex2((float)(ve - ne));
-      ve = ne;
-      float c0 = 1.f, c1 = 1.f;  // of this lane's columns
+      float c0[GROUPS], c1[GROUPS];  // of this lane's columns
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        if constexpr (F32) {
-          if (t == q) c0 = c1 = corr[q];
-        } else {
-          if (2 * t == q) c0 = corr[q];
-          if (2 * t + 1 == q) c1 = corr[q];
+      for (int k = 0; k < GROUPS; ++k) {
+        c0[k] = c1[k] = 1.f;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          if constexpr (F32) {
+            if (t == q) c0[k] = c1[k] = f[q][k];
+          } else {
+            if (2 * t == q) c0[k] = f[q][k];
+            if (2 * t + 1 == q) c1[k] = f[q][k];
+          }
         }
       }
-      c0 *= ve_corr;
-      c1 *= ve_corr;
 #pragma unroll
       for (int k = 0; k < MT; ++k) {
-        acc[k][0] *= c0; acc[k][1] *= c1; acc[k][2] *= c0; acc[k][3] *= c1;
+        constexpr int PER = MT / GROUPS;
+        acc[k][0] *= c0[k / PER]; acc[k][1] *= c1[k / PER]; acc[k][2] *= c0[k / PER]; acc[k][3] *= c1[k / PER];
       }
     }
-    // p <= 2^8 and s 2^-ve < 2, so p s 2^(6 - ve) stays below 2^15
-    const float vup = __uint_as_float((uint32_t)(127 + 6 - ve) << 23);
 #pragma unroll
-    for (int u = 0; u < PL; ++u) {
-      const int key = u * 32 + lane;
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int u = 0; u < PL; ++u) {
+        l[q] += e[q][u];
+        if (!AGAIN && p.weights && valid[u] && q < nq) zrow[q * zld + j + u * 32 + lane] = z[q][u];
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) mg[q][k] = fmaf(e[q][u], vm[u][k], mg[q][k]);
+      }
+#pragma unroll
+    for (int i2 = 0; i2 < 2; ++i2) {
+      const int key = (GROUPS == 1 ? i2 * 32 : 0) + lane;
       // position of the key among its 16 in the B operand: lane t's four slots are keys t, t+4, t+8, t+12
       const int at = (key & ~15) + (key & 3) * 4 + ((key >> 2) & 3);
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        const float e = valid[u] ? ex2(z[q][u] - m[q]) : 0.f;
-        l[q] += e;
-        if (p.weights && valid[u] && q < nq) zrow[q * zld + j + key] = z[q][u];
-#pragma unroll
-        for (int k = 0; k < GROUPS; ++k) {
-          mg[q][k] = fmaf(e, vm[u][k], mg[q][k]);
-          const float ps = e * (vs[u][k] * vup);
-          const __half hi = __float2half_rn(ps);
-          __half* col = sp + (k * S::COLS + (F32 ? 2 * q : q)) * S::P_LD;
-          col[at] = hi;
-          if constexpr (F32) col[S::P_LD + at] = __float2half_rn((ps - __half2float(hi)) * 2048.f);
-        }
+        const __half hi = i2 ? __high2half(h[q]) : __low2half(h[q]);
+        __half* col = sp + ((GROUPS == 2 ? i2 : 0) * S::COLS + (F32 ? 2 * q : q)) * S::P_LD;
+        col[at] = hi;
+        if constexpr (F32) col[S::P_LD + at] = __float2half_rn((x[q][i2] - __half2float(hi)) * 2048.f);
       }
     }
     __syncwarp();
@@ -553,8 +606,8 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   }
   __syncthreads();
   float* merge = reinterpret_cast<float*>(smem) + warp * NQ * (D + 2);
-  // the codes' 2^-18 or 2^-24 (16 times that in the odd rows) and p s's scaling
-  const float down = __uint_as_float((uint32_t)(127 + (F32 ? 18 : 24) - 6 + ve) << 23), down_odd = F32 ? down : down * 0.0625f;
+  // the codes' 2^-18 or 2^-24 (16 times that in the odd rows)
+  constexpr float DOWN = F32 ? 0x1p18f : 0x1p24f, DOWN_ODD = F32 ? 0x1p18f : 0x1p20f;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     if (lane == 0) {
@@ -563,14 +616,16 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     }
     const bool mine = F32 ? t == q : t == q / 2;
     if (mine) {
+      const float second = GROUPS == 2 ? 1.f / ratio[q] : 1.f;
 #pragma unroll
       for (int k = 0; k < MT; ++k) {
         constexpr int PER = GS / 8;  // elements of a group per lane row g
         const int gr = k * 2 / PER, d = gr * GS + g * PER + (k * 2) % PER;
         const float lo = F32 ? fmaf(acc[k][1], 1.f / 2048.f, acc[k][0]) : (q & 1) ? acc[k][1] : acc[k][0];
         const float hi = F32 ? fmaf(acc[k][3], 1.f / 2048.f, acc[k][2]) : (q & 1) ? acc[k][3] : acc[k][2];
-        merge[q * (D + 2) + 2 + d] = fmaf(lo, down, mg[q][gr]);
-        merge[q * (D + 2) + 3 + d] = fmaf(hi, down_odd, mg[q][gr]);
+        const float by = gr ? second : 1.f;
+        merge[q * (D + 2) + 2 + d] = fmaf(lo, DOWN * by, mg[q][gr]);
+        merge[q * (D + 2) + 3 + d] = fmaf(hi, DOWN_ODD * by, mg[q][gr]);
       }
     }
   }
@@ -604,7 +659,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   // ---- merge over the cluster (or this CTA alone) ----
   if (p.cluster) cluster_sync();
   else __syncthreads();
-  float* smx = sfac;  // [NQ] merged maxima, [NQ] reciprocal sums (the queries' factors are no longer needed)
+  float* smx = sfac;  // [NQ] merged references, [NQ] reciprocal sums (the queries' factors are no longer needed)
   float* sinv = sfac + NQ;
   if (threadIdx.x < nq) {
     const float* a = own + threadIdx.x * (D + 2);
@@ -648,7 +703,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
 }
 
 // Merge the splits' states and add the weights: a CTA takes KD_WCHUNK keys of one (sequence, key head), and
-// its share of the outputs.  A warp finds a head's maximum and sum, the splits on its lanes, so that a call
+// its share of the outputs.  A warp finds a head's reference and sum, the splits on its lanes, so that a call
 // waits for memory three times, not once per head and split.  16 keys a thread keep enough bytes in flight at two
 // CTAs an SM (110 us for the long case's two kernels and 33 for the shared heads'; 8 keys and four CTAs 110 and 35,
 // 4 and six 127 and 37); without weights there is little to hold, and six CTAs share an SM (64 x 8 heads of 2,048

@@ -1,5 +1,5 @@
 """The 4-bit cache operators where they went wrong once: numbers that are not finite in places a mask
-leaves out, scales of zero and below, the tf32 module's prompt weights.
+leaves out, scales of zero and below, value scales far apart, the tf32 module's prompt weights.
 
 Bounds on errors are those derived in test_gpu_kv4.py (u = 2^-24), or stand beside the test."""
 import math
@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv4 import U, make_cache, prompt_plain, within
+from test_gpu_kv4 import U, decode_plain, make_cache, prompt_plain, within
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,93 @@ def test_bad_queries_leave_the_weights_behind_the_rows(ops, dtype, B, NH, NKV, L
     for b in range(B):
         assert torch.equal(w[b, :, lens[b]:], before[b, :, lens[b]:]), b
     assert bool(torch.isnan(w[0, 0, :lens[0]]).all()) and bool(torch.isnan(w[-1, -1, :lens[-1]]).all())
+
+
+def spread_cache(ops, B, NKV, L, D, seed, wild):
+    """Small value scales everywhere but in the rows ``wild`` of every head, whose keys point away from q = ones."""
+    gen = torch.Generator().manual_seed(seed)
+    codes, params = ops.kv4_empty(B, NKV, L, D)
+    codes.copy_(torch.randint(0, 256, codes.shape, dtype=torch.uint8, generator=gen))
+    p = torch.zeros(params.shape)
+    p[0, ..., 0], p[0, ..., 1] = 0.01, 0.02 * torch.randn(p[0, ..., 1].shape, generator=gen)
+    p[1, ..., 0], p[1, ..., 1] = 2.0 ** -20, 0.0
+    for j, (low, scale) in wild.items():
+        p[0, :, :, j, :, 1] = low
+        p[1, :, :, j, :, 0] = scale
+    params.copy_(p)
+    return codes, params
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("NH,NKV,D", [(2, 2, 64), (8, 2, 64), (3, 3, 16), (2, 2, 32), (8, 2, 128), (7, 1, 128)])
+@pytest.mark.parametrize("L,at", [(600, 3), (600, 400), (700, 699), (9000, 70)])
+def test_decode_with_one_wild_value_scale(ops, dtype, NH, NKV, D, L, at):
+    """A row of a value scale 2^35 times the others', which hardly any weight falls on, takes no digits from the
+    others' part of the output."""
+    codes, params = spread_cache(ops, 2, NKV, L, D, L + at, {at: (-2.0, 32768.0)})
+    q = torch.ones((2, NH, D), device="cuda") * (60.0 / math.sqrt(D))  # the wild row's score: about 120 below
+    q += 0.01 * torch.randn((2, NH, D), generator=torch.Generator().manual_seed(1)).cuda()
+    q = q.to(dtype)
+    o, l, _, eo, el, _ = decode_plain(q, codes, params, [L] * 2, 1 / math.sqrt(D), dtype)
+    lse = torch.empty((2, NH), device="cuda")
+    within(ops.kv4_decode(q, codes, params, L, lse=lse), o, eo, "o")
+    within(lse, l, el, "lse")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_with_a_wild_value_scale_that_leads_at_first(ops, dtype):
+    """The wild row holds the largest score until a later tile's scores leave it 100 and more below (so many sequences
+    that one CTA takes all rows of a head)."""
+    B, NKV, L, D = 300, 4, 1500, 64
+    codes, params = spread_cache(ops, B, NKV, L, D, 4, {5: (0.5, 32768.0)})
+    params[0, :, :, 1000:, :, 1] = 2.0
+    q = (torch.ones((B, NKV, D)) * 12.0).to(dtype).cuda()
+    got = ops.kv4_decode(q, codes, params, L)
+    pick = [0, 144, 299]
+    o, _, _, eo, _, _ = decode_plain(q[pick], codes[:, pick], params[:, pick], [L] * 3, 1 / math.sqrt(D), dtype)
+    within(got[pick], o, eo, "o")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_where_heads_see_different_value_scales(ops, dtype, D):
+    """Two query heads of one cached head: one looks at rows of large value scales, the other at small ones."""
+    L = 500
+    codes, params = spread_cache(ops, 1, 1, L, D, 8, {j: (-2.0, 32768.0) for j in range(200, 232)})
+    q = torch.ones((1, 2, D), device="cuda") * (60.0 / math.sqrt(D))
+    q[:, 1] *= -1.0
+    q = q.to(dtype)
+    o, _, _, eo, _, _ = decode_plain(q, codes, params, [L], 1 / math.sqrt(D), dtype)
+    within(ops.kv4_decode(q, codes, params, L), o, eo, "o")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_with_groups_of_different_value_scales(ops, dtype):
+    """head_dim 128: the second group's scales 2^35 times the first's; every element keeps the digits of its group."""
+    L = 300
+    codes, params = spread_cache(ops, 2, 2, L, 128, 9, {})
+    params[1, ..., 1, 0] = 32768.0
+    q = torch.randn((2, 8, 128), generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    o, _, _, eo, _, _ = decode_plain(q, codes, params, [L] * 2, 0.1, dtype)
+    within(ops.kv4_decode(q, codes, params, L, scale=0.1), o, eo, "o")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_with_a_value_group_that_is_not_finite(ops, dtype):
+    """head_dim 128: a NaN among one group's scales reaches that group's outputs only, not the other's, the lse or the
+    weights."""
+    L = 400
+    codes, params = make_cache(ops, 1, 2, L, 128, seed=12)
+    q = torch.randn((1, 8, 128), generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    for group in (0, 1):
+        bad = params.clone()
+        bad[1, :, :, 77, group, 0] = float("nan")
+        lse, w = torch.empty((1, 8), device="cuda"), torch.empty((1, 2, L), device="cuda")
+        got = ops.kv4_decode(q, codes, bad, L, lse=lse, weights_out=w)
+        o, l, wp, eo, el, ew = decode_plain(q, codes, params, [L], 128 ** -0.5, dtype)
+        fine = slice(64, 128) if group == 0 else slice(0, 64)
+        within(got[..., fine], o[..., fine], eo[..., fine], "o")
+        within(lse, l, el, "lse")
+        within(w, wp[..., :L], ew[..., :L] + U * wp[..., :L], "weights")
+        gone = slice(0, 64) if group == 0 else slice(64, 128)
+        assert bool(torch.isnan(got[..., gone].float()).all())
