@@ -234,7 +234,8 @@ int attn_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
  * Row r of (which, b, h, slot) is which*c_si + b*c_sb + h*c_sh + slot, which = 0 for keys and 1 for
  * values.  capacity (the slots of one head) and the strides, all in rows, are multiples of 16; both
  * arrays are 16-byte aligned.  int32 arrays of one entry per sequence live on the device, so that a
- * captured step reads them anew at every replay.  Strides of what a call writes must keep its rows apart.
+ * captured step reads them anew at every replay.  Strides of what a call writes must keep its rows apart, each being
+ * at least the span of the axes inside it; weights_in is weights_out or shares no memory with it.
  *
  * attn_kv4_store quantises k and v (ATTN_F32 or ATTN_BF16, element (b, t, h, d) at
  * k[b*k_sb + t*k_st + h*k_sh + d]) into slots starts[b] + start + t, t < counts[b] (starts NULL: 0;
@@ -306,8 +307,8 @@ size_t attn_kv4_evict_workspace_size(int B, int NH, int L, int keep);
  * slot (NaN last).  Kept rows below slot `keep` stay in their slots; those from slot `keep` on fill, in
  * order, the slots below it that were given up.  slots [B, NH, keep] receives the row each slot holds
  * afterwards (-1 from min(n, keep) on).  Codes, params, weights and positions move together: in place
- * (dst_codes NULL; the other dst arguments are then ignored), or into another cache, whose slots from
- * min(n, keep) on are left as they were.  recent <= keep.
+ * (dst_codes NULL; the other dst arguments are then ignored), or into another cache, which shares no memory with the
+ * rows it is filled from, and whose slots from min(n, keep) on are left as they were.  recent <= keep.
  */
 int attn_kv4_evict(void* codes, void* params, float* weights, int* positions,
                    int64_t c_si, int64_t c_sb, int64_t c_sh, int capacity, int64_t w_sb, int64_t w_sh,

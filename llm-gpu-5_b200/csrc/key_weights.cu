@@ -611,7 +611,10 @@ extern "C" int attn_key_weights(const void* q, const void* k, const float* lse, 
   ATTN_REQUIRE(first_query >= 0, "attn_key_weights: first_query must not be negative");
   ATTN_REQUIRE(q_sb >= 0 && q_st >= 0 && q_sh >= 0 && k_sb >= 0 && k_st >= 0 && k_sh >= 0 && w_sb >= 0 && w_sh >= 0,
                "attn_key_weights: strides must not be negative");
-  ATTN_REQUIRE(kv4_apart(B, NKV, w_sb, w_sh, T), "attn_key_weights: rows of the weights must not overlap");
+  const RowSet w(T, B, w_sb, NKV, w_sh);
+  ATTN_REQUIRE(w.apart, "attn_key_weights: rows of the weights must not overlap");
+  ATTN_REQUIRE(!weights_in || weights_in == weights_out || !w.meets(weights_in, w, weights_out, 4),
+               "attn_key_weights: weights_in and weights_out must be the same array or not overlap");
   const size_t esz = dtype == ATTN_BF16 ? 2 : 4;
   ATTN_REQUIRE(aligned(q, esz) && aligned(k, esz) && aligned(lse, 4), "attn_key_weights: misaligned tensor");
   if (D > 128) {

@@ -29,10 +29,49 @@ struct Kv4View {
   int cap;             // rows per (sequence, head)
 };
 
-// Whether [B, NH] rows of `len` elements at these strides are apart, so that CTAs may write them side by side.
-inline bool kv4_apart(int B, int NH, int64_t sb, int64_t sh, int64_t len) {
-  return (B == 1 || sb >= len) && (NH == 1 || sh >= len);
-}
+// Rows of `len` units (elements, or cached rows) along up to three strided axes.  They are apart where every stride
+// is at least the span of the axes inside it, so that CTAs may write them side by side; a layout whose rows miss one
+// another in some other way counts as overlapping.
+struct RowSet {
+  int64_t n[3] = {1, 1, 1}, s[3] = {0, 0, 0};  // axes of more than one entry, the largest stride first
+  int64_t len, span;                           // span: from the first row to the end of the last
+  bool apart = true;
+  RowSet(int64_t len_, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2 = 1, int64_t s2 = 0) : len(len_), span(len_) {
+    const int64_t ns[3] = {n0, n1, n2}, ss[3] = {s0, s1, s2};
+    int axes = 0;
+    for (int i = 0; i < 3; ++i) {
+      if (ns[i] <= 1) continue;
+      int at = axes++;
+      for (; at > 0 && s[at - 1] < ss[i]; --at) { n[at] = n[at - 1]; s[at] = s[at - 1]; }
+      n[at] = ns[i];
+      s[at] = ss[i];
+    }
+    for (int i = axes - 1; i >= 0 && apart; --i) {
+      apart = s[i] >= span && s[i] <= ((int64_t)1 << 52) / n[i] - span;  // (2^52 units are more than any memory)
+      if (apart) span += (n[i] - 1) * s[i];
+    }
+  }
+  // Whether rows of `bytes` bytes a unit at p share memory with those of b at q (both apart).
+  bool meets(const void* p, const RowSet& b, const void* q, int64_t bytes) const {
+    const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(p) - reinterpret_cast<intptr_t>(q));
+    if (d >= b.span * bytes || -d >= span * bytes) return false;
+    for (int64_t i = 0; i < n[0]; ++i)
+      for (int64_t j = 0; j < n[1]; ++j)
+        for (int64_t k = 0; k < n[2]; ++k) {
+          const int64_t first = d + (i * s[0] + j * s[1] + k * s[2]) * bytes;  // of this row, from q on
+          int64_t left = first + len * bytes - 1, at = 0;                       // the last row of b that starts by then
+          if (left < 0) continue;
+          for (int x = 0; x < 3; ++x) {
+            if (b.n[x] <= 1) continue;
+            const int64_t stride = b.s[x] * bytes, c = left / stride < b.n[x] - 1 ? left / stride : b.n[x] - 1;
+            at += c * stride;
+            left -= c * stride;
+          }
+          if (at + b.len * bytes > first) return true;
+        }
+    return false;
+  }
+};
 
 // Checks shared by the entry points that take a cache.
 int kv4_check(const char* fn, const Kv4View& c, int B, int NH, int D);

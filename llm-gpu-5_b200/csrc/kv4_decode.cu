@@ -906,9 +906,11 @@ extern "C" int attn_kv4_decode(const void* q, const void* codes, const void* par
   ATTN_REQUIRE(L > 0 && L <= capacity, "attn_kv4_decode: length %d outside 1 .. capacity %d", L, capacity);
   ATTN_REQUIRE(q_sb >= 0 && q_sh >= 0 && o_sb >= 0 && o_sh >= 0 && w_sb >= 0 && w_sh >= 0, "attn_kv4_decode: strides must not be negative");
   ATTN_REQUIRE(!weights_in || weights_out, "attn_kv4_decode: weights_in needs weights_out");
-  ATTN_REQUIRE(!weights_out || kv4_apart(B, NKV, w_sb, w_sh, L),
-               "attn_kv4_decode: rows of the weights must not overlap");
-  ATTN_REQUIRE(kv4_apart(B, NH, o_sb, o_sh, D), "attn_kv4_decode: rows of the output must not overlap");
+  const RowSet w(L, B, w_sb, NKV, w_sh);
+  ATTN_REQUIRE(!weights_out || w.apart, "attn_kv4_decode: rows of the weights must not overlap");
+  ATTN_REQUIRE(!weights_in || weights_in == weights_out || !w.meets(weights_in, w, weights_out, 4),
+               "attn_kv4_decode: weights_in and weights_out must be the same array or not overlap");
+  ATTN_REQUIRE(RowSet(D, B, o_sb, NH, o_sh).apart, "attn_kv4_decode: rows of the output must not overlap");
   const KdPlan k = kd_plan(B, NH, NKV, L, D, dtype, weights_out != nullptr);
   const size_t need = (k.states + k.scores) * sizeof(float);
   if (need && (!workspace || workspace_bytes < need)) {

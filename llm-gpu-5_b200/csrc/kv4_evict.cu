@@ -405,23 +405,33 @@ extern "C" int attn_kv4_evict(void* codes, void* params, float* weights, int* po
   p.dst = in_place ? p.src : Kv4View{(uint8_t*)dst_codes, (__half2*)dst_params, d_si, d_sb, d_sh, dst_capacity};
   if (int rc = kv4_check("attn_kv4_evict", p.src, B, NH, D)) return rc;
   if (int rc = kv4_check("attn_kv4_evict", p.dst, B, NH, D)) return rc;
-  ATTN_REQUIRE(in_place || (dst_codes != codes && dst_params != params && dst_weights != weights),
-               "attn_kv4_evict: the destination must be another cache (NULL: in place)");
-  ATTN_REQUIRE(c_si >= capacity && (B == 1 || c_sb >= capacity) && p.dst.si >= p.dst.cap && (B == 1 || p.dst.sb >= p.dst.cap),
+  ATTN_REQUIRE(RowSet(capacity, 2, c_si, B, c_sb, NH, c_sh).apart &&
+                   RowSet(p.dst.cap, 2, p.dst.si, B, p.dst.sb, NH, p.dst.sh).apart,
                "attn_kv4_evict: cache rows must not overlap");
   ATTN_REQUIRE(w_sb >= 0 && w_sh >= 0 && dw_sb >= 0 && dw_sh >= 0, "attn_kv4_evict: strides must not be negative");
   ATTN_REQUIRE(L > 0 && L <= capacity, "attn_kv4_evict: length %d outside 1 .. capacity %d", L, capacity);
   ATTN_REQUIRE(keep > 0 && keep <= p.dst.cap, "attn_kv4_evict: keep %d outside 1 .. capacity %d", keep, p.dst.cap);
   ATTN_REQUIRE(recent >= 0 && recent <= keep, "attn_kv4_evict: recent %d outside 0 .. keep %d", recent, keep);
   ATTN_REQUIRE(weights && slots && (in_place || dst_weights), "attn_kv4_evict: null pointer argument");
+  if (!in_place) {
+    const RowSet rows(L, 2, c_si, B, c_sb, NH, c_sh), kept(keep, 2, d_si, B, d_sb, NH, d_sh);
+    ATTN_REQUIRE(!kept.meets(dst_codes, rows, codes, D / 2) && !kept.meets(dst_params, rows, params, 4 * kv4_groups(D)),
+                 "attn_kv4_evict: the destination must be another cache (NULL: in place)");
+  }
   const size_t need = attn_kv4_evict_workspace_size(B, NH, L, keep);
   if (need && (!workspace || workspace_bytes < need)) {
     set_error("attn_kv4_evict: workspace of %zu bytes required", need);
     return ATTN_ERR_WORKSPACE;
   }
   ATTN_REQUIRE(aligned(workspace, 4), "attn_kv4_evict: misaligned workspace");
-  ATTN_REQUIRE(kv4_apart(B, NH, w_sb, w_sh, L) && (in_place || kv4_apart(B, NH, dw_sb, dw_sh, keep)),
-               "attn_kv4_evict: rows of the weights must not overlap");
+  const RowSet w(L, B, w_sb, NH, w_sh);
+  ATTN_REQUIRE(w.apart, "attn_kv4_evict: rows of the weights must not overlap");
+  if (!in_place) {
+    const RowSet kept(keep, B, dw_sb, NH, dw_sh);
+    ATTN_REQUIRE(kept.apart, "attn_kv4_evict: rows of the weights must not overlap");
+    ATTN_REQUIRE(!kept.meets(dst_weights, w, weights, 4) && !(positions && dst_positions && kept.meets(dst_positions, w, positions, 4)),
+                 "attn_kv4_evict: the destination must be another cache (NULL: in place)");
+  }
   if ((int64_t)B * NH * ((keep + 15) / 16) >= (int64_t)1 << 31) {
     set_error("attn_kv4_evict: B*NH*keep = %lld rows are too many for one call; split the batch", (long long)B * NH * keep);
     return ATTN_ERR_UNSUPPORTED;

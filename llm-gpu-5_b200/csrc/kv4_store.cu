@@ -261,7 +261,6 @@ static int kv4_rows_t(const Kv4Rows& r, int D, const Kv4View& c, const Kv4Slots&
 
 static int kv4_rows(const char* fn, Kv4Rows r, int B, int D, int dtype, const Kv4View& c, const Kv4Slots& sl,
                     const Kv4Marks* mk, cudaStream_t s) {
-  if (int rc = kv4_check(fn, c, B, (int)r.NH, D)) return rc;
   ATTN_REQUIRE(r.k && r.v, "%s: null pointer argument", fn);
   ATTN_REQUIRE(dtype == ATTN_F32 || dtype == ATTN_BF16, "%s: dtype must be ATTN_F32 or ATTN_BF16", fn);
   ATTN_REQUIRE(aligned(r.k, dtype == ATTN_BF16 ? 2 : 4) && aligned(r.v, dtype == ATTN_BF16 ? 2 : 4), "%s: misaligned tensor", fn);
@@ -269,6 +268,10 @@ static int kv4_rows(const char* fn, Kv4Rows r, int B, int D, int dtype, const Kv
   for (int i = 0; i < 6; ++i) ATTN_REQUIRE(st[i] >= 0, "%s: strides must not be negative", fn);
   ATTN_REQUIRE(sl.starts || (sl.start >= 0 && (int64_t)sl.start + r.T <= c.cap),
                "%s: positions %d .. %lld exceed the capacity of %d", fn, sl.start, (long long)sl.start + r.T - 1, c.cap);
+  if (!mk) {  // what the load writes
+    const RowSet o(D, B, r.k_sb, r.T, r.k_st, r.NH, r.k_sh);
+    ATTN_REQUIRE(o.apart && !o.meets(r.k, o, r.v, dtype == ATTN_BF16 ? 2 : 4), "%s: rows of the output must not overlap", fn);
+  }
   ATTN_REQUIRE(kv4_set_rows(&r, B, KV4_THREADS / (D / 8)) < (int64_t)1 << 31, "%s: B*NH*T must be below 2^31", fn);
   return dtype == ATTN_BF16 ? kv4_rows_t<__nv_bfloat16>(r, D, c, sl, mk, s) : kv4_rows_t<float>(r, D, c, sl, mk, s);
 }
@@ -288,8 +291,9 @@ extern "C" int attn_kv4_store(const void* k, const void* v, int dtype, int B, in
   ATTN_REQUIRE(!(weights || positions) || (w_sb >= 0 && w_sh >= 0), "attn_kv4_store: bad strides");
   const Kv4Rows r = {k, v, k_sb, k_st, k_sh, v_sb, v_st, v_sh, (uint32_t)T, (uint32_t)NH};
   const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
-  ATTN_REQUIRE(c_si >= capacity && (B == 1 || c_sb >= capacity), "attn_kv4_store: cache rows must not overlap");
-  ATTN_REQUIRE(!(weights || positions) || kv4_apart(B, NH, w_sb, w_sh, capacity),
+  if (int rc = kv4_check("attn_kv4_store", c, B, NH, D)) return rc;
+  ATTN_REQUIRE(RowSet(capacity, 2, c_si, B, c_sb, NH, c_sh).apart, "attn_kv4_store: cache rows must not overlap");
+  ATTN_REQUIRE(!(weights || positions) || RowSet(capacity, B, w_sb, NH, w_sh).apart,
                "attn_kv4_store: rows of weights and positions must not overlap");
   const Kv4Marks mk = {weights, positions, w_sb, w_sh, seen, seen0};
   return kv4_rows("attn_kv4_store", r, B, D, dtype, c, Kv4Slots{starts, start, counts}, &mk, as_stream(stream));
@@ -303,5 +307,6 @@ extern "C" int attn_kv4_load(const void* codes, const void* params, int64_t c_si
   ATTN_REQUIRE((int64_t)B * NH * T < (int64_t)1 << 31, "attn_kv4_load: B*NH*T must be below 2^31");
   const Kv4Rows r = {k, v, o_sb, o_st, o_sh, o_sb, o_st, o_sh, (uint32_t)T, (uint32_t)NH};
   const Kv4View c = {(uint8_t*)codes, (__half2*)params, c_si, c_sb, c_sh, capacity};
+  if (int rc = kv4_check("attn_kv4_load", c, B, NH, D)) return rc;
   return kv4_rows("attn_kv4_load", r, B, D, dtype, c, Kv4Slots{starts, start, counts}, nullptr, as_stream(stream));
 }
