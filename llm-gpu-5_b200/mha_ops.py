@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 
 import torch
 
@@ -197,10 +198,18 @@ def _kv4_marks(name, t, dtype, B, NH, rows, device):
     return t.data_ptr(), sb, sh
 
 
+def _int32(name, x):
+    """x as an int that C takes whole: ctypes drops the bits above an int's 32."""
+    x = operator.index(x)
+    if not -0x80000000 <= x <= 0x7fffffff:
+        raise ValueError(f"{name}: {x} does not fit 32 bits")
+    return x
+
+
 def _per_sequence(name, x, B, device):
     """(device address or None, int to add) of an int or an int32 tensor of one entry per sequence."""
     if not isinstance(x, torch.Tensor):
-        return None, int(x)
+        return None, _int32(name, x)
     if x.dtype != torch.int32:
         raise TypeError(f"{name}: expected an int or int32, got {x.dtype}")
     if x.shape != (B,) or x.device != device or not x.is_contiguous():
@@ -271,6 +280,7 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: tor
     if T == 0 or B == 0:
         return
     code = dtype_code(k.dtype)
+    _int32("T", T)
     wp, wsb, wsh = _kv4_marks("weights", weights, torch.float32, B, NH, cap, dev)
     pp, psb, psh = _kv4_marks("positions", positions, torch.int32, B, NH, cap, dev)
     if wp is not None and pp is not None and (wsb, wsh) != (psb, psh):
@@ -279,6 +289,8 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: tor
         wsb, wsh = psb, psh
     starts, start = _per_sequence("pos", pos, B, dev)
     seen_p, seen0 = _per_sequence("seen", pos if seen is None else seen, B, dev)
+    if pp is not None:
+        _int32("positions", seen0 + T - 1)
     counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
     before = _other_device(dev)
     try:
@@ -297,6 +309,7 @@ def kv4_load(codes: torch.Tensor, params: torch.Tensor, pos, T: int, dtype: torc
     ``dtype``; zeros for the rows from ``counts`` on and for slots outside the cache."""
     B, NH, cap, D, si, sb, sh = _kv4_view(codes, params)
     dev = codes.device
+    _int32("T", T)
     code = dtype_code(dtype)
     k = codes.new_empty((B, T, NH, D), dtype=dtype)
     v = torch.empty_like(k)
@@ -328,6 +341,7 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
     weights are added to it, in place or into ``weights_out``; with ``weights_out`` alone they are set."""
     B, NKV, cap, D, si, sb, sh = _kv4_view(codes, params)
     dev = codes.device
+    length = _int32("length", length)
     shape = q.shape
     if len(shape) != 3 or shape[0] != B or shape[2] != D or q.device != dev:
         raise ValueError(f"q: expected [{B}, NH, {D}] on {dev}, got {tuple(shape)} on {q.device}")
@@ -381,6 +395,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
         raise ValueError("key_weights: expected q [B, T, NH, D] and k [B, T, NKV, D] of one dtype")
     B, T, NH, D = q.shape
     NKV, dev = k.shape[2], q.device
+    _int32("T", T)
+    first_query = _int32("first_query", first_query)
     qs, ks = _token_rows("q", q, B, NH, D, dev), _token_rows("k", k, B, NKV, D, dev)
     code = dtype_code(q.dtype if dtype is None else dtype)
     if q.dtype is not (torch.float32 if code == ATTN_TF32 else _OF[code]):
@@ -402,7 +418,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
     before = _other_device(dev)
     try:
         rc = lib.attn_key_weights(q.data_ptr(), k.data_ptr(), lse.data_ptr(), w_in, w_out, B, NH, NKV, T, D,
-                                  qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, int(first_query), lengths_p,
+                                  qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], wsb, wsh, first_query, lengths_p,
                                   1.0 / math.sqrt(D) if scale is None else float(scale), code,
                                   ws, ws_bytes, _raw_stream(dev.index))
     finally:
@@ -425,6 +441,7 @@ def kv4_evict(codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, 
     row each slot holds afterwards, -1 where there is none."""
     B, NH, cap, D, si, sb, sh = _kv4_view(codes, params)
     dev = codes.device
+    length, keep, recent = _int32("length", length), _int32("keep", keep), _int32("recent", recent)
     wp, wsb, wsh = _kv4_marks("weights", weights, torch.float32, B, NH, length, dev)
     if wp is None:
         raise ValueError("kv4_evict: weights are required")

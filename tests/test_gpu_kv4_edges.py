@@ -1,5 +1,6 @@
 """The 4-bit cache operators where they went wrong once: numbers that are not finite in places a mask
-leaves out, scales of zero and below, value scales far apart, the tf32 module's prompt weights.
+leaves out, scales of zero and below, value scales far apart, the tf32 module's prompt weights, arguments
+that the C boundary would cut short.
 
 Bounds on errors are those derived in test_gpu_kv4.py (u = 2^-24), or stand beside the test."""
 import math
@@ -208,3 +209,27 @@ def test_decode_with_a_value_group_that_is_not_finite(ops, dtype):
         within(w, wp[..., :L], ew[..., :L] + U * wp[..., :L], "weights")
         gone = slice(0, 64) if group == 0 else slice(64, 128)
         assert bool(torch.isnan(got[..., gone].float()).all())
+
+
+# ------------------------------------------------------------------------------------ arguments
+def test_numbers_past_32_bits_are_refused(ops):
+    """(They reach C as an int, whose upper bits would be dropped: position 2^32 would be slot 0.)"""
+    codes, params = make_cache(ops, 1, 1, 16, 64, seed=1)
+    x = torch.randn((1, 2, 1, 64), device="cuda")
+    q = x[:, 0]
+    w = torch.zeros((1, 1, 16), device="cuda")
+    marks = torch.zeros((1, 1, 16), dtype=torch.int32, device="cuda")
+    held = codes.clone()
+    for call in (lambda: ops.kv4_store(x, x, codes, params, 1 << 32), lambda: ops.kv4_store(x, x, codes, params, 0, seen=1 << 31),
+                 lambda: ops.kv4_store(x, x, codes, params, 0, positions=marks, seen=(1 << 31) - 1),
+                 lambda: ops.kv4_store(x, x, codes, params, -(1 << 32)), lambda: ops.kv4_load(codes, params, 1 << 32, 1),
+                 lambda: ops.kv4_decode(q, codes, params, (1 << 32) + 4),
+                 lambda: ops.key_weights(x, x, torch.zeros((1, 1, 2), device="cuda"), first_query=1 << 32),
+                 lambda: ops.kv4_evict(codes, params, w, None, (1 << 32) + 9, 4),
+                 lambda: ops.kv4_evict(codes, params, w, None, 9, 4, recent=1 << 32),
+                 lambda: ops.kv4_evict(codes, params, w, None, 9, 4, seen=1 << 32)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        ops.kv4_store(x, x, codes, params, 1.5)
+    assert torch.equal(codes, held)
