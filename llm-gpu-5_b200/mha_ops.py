@@ -217,6 +217,15 @@ def _per_sequence(name, x, B, device):
     return x.data_ptr(), 0
 
 
+def _row_counts(name, x, B, device):
+    """Device address of an int32 tensor of one entry per sequence, or None."""
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected an int32 tensor of one entry per sequence, got {type(x).__name__}")
+    return _per_sequence(name, x, B, device)[0]
+
+
 # The current stream's handle without building a torch.cuda.Stream: 0.1 against 3.2 us of a call that
 # takes 10 in all.
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -291,7 +300,7 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, params: tor
     seen_p, seen0 = _per_sequence("seen", pos if seen is None else seen, B, dev)
     if pp is not None:
         _int32("positions", seen0 + T - 1)
-    counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
+    counts_p = _row_counts("counts", counts, B, dev)
     before = _other_device(dev)
     try:
         rc = lib.attn_kv4_store(k.data_ptr(), v.data_ptr(), code, B, T, NH, D, ks[0], ks[1], ks[2],
@@ -316,7 +325,7 @@ def kv4_load(codes: torch.Tensor, params: torch.Tensor, pos, T: int, dtype: torc
     if k.numel() == 0:
         return k, v
     starts, start = _per_sequence("pos", pos, B, dev)
-    counts_p = None if counts is None else _per_sequence("counts", counts, B, dev)[0]
+    counts_p = _row_counts("counts", counts, B, dev)
     before = _other_device(dev)
     try:
         rc = lib.attn_kv4_load(codes.data_ptr(), params.data_ptr(), si, sb, sh, cap, B, T, NH, D, starts, start,
@@ -363,7 +372,7 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
         if w_in is not None and (osb, osh) != (wsb, wsh):
             raise ValueError("kv4_decode: weights and weights_out must have the same strides")
         wsb, wsh = osb, osh
-    lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    lengths_p = _row_counts("lengths", lengths, B, dev)
     code = dtype_code(q.dtype)
     before = _other_device(dev)
     try:
@@ -413,7 +422,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
         w_in, isb, ish = _kv4_marks("weights", weights, torch.float32, B, NKV, T, dev)
         if (isb, ish) != (wsb, wsh):
             raise ValueError("key_weights: weights and out must have the same strides")
-    lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    lengths_p = _row_counts("lengths", lengths, B, dev)
     workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_key_weights_workspace_size", 0, B, NKV, T), q)
     before = _other_device(dev)
     try:
@@ -462,10 +471,10 @@ def kv4_evict(codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, 
         slots = codes.new_empty((B, NH, max(keep, 0)), dtype=torch.int32)
     elif slots.shape != (B, NH, keep) or slots.dtype != torch.int32 or not slots.is_contiguous() or slots.device != dev:
         raise ValueError(f"slots: expected contiguous int32 [{B}, {NH}, {keep}] on {dev}")
-    seen_p, seen0 = _per_sequence("seen", length if seen is None else seen, B, dev)
-    if seen is None and lengths is not None:
-        seen_p, seen0 = _per_sequence("lengths", lengths, B, dev)
-    lengths_p = None if lengths is None else _per_sequence("lengths", lengths, B, dev)[0]
+    lengths_p = _row_counts("lengths", lengths, B, dev)
+    if seen is None:
+        seen = length if lengths is None else lengths
+    seen_p, seen0 = _per_sequence("seen", seen, B, dev)
     workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_kv4_evict_workspace_size", 0, B, NH, length, keep), codes)
     before = _other_device(dev)
     try:

@@ -233,3 +233,18 @@ def test_numbers_past_32_bits_are_refused(ops):
     with pytest.raises(TypeError):
         ops.kv4_store(x, x, codes, params, 1.5)
     assert torch.equal(codes, held)
+
+
+def test_lengths_and_counts_are_device_arrays(ops):
+    """A plain number where a device array belongs is refused, not passed over."""
+    codes, params = make_cache(ops, 1, 1, 16, 64, seed=1)
+    x = torch.randn((1, 2, 1, 64), device="cuda")
+    w = torch.zeros((1, 1, 16), device="cuda")
+    held = codes.clone()
+    for call in (lambda: ops.kv4_store(x, x, codes, params, 0, counts=1), lambda: ops.kv4_load(codes, params, 0, 2, counts=1),
+                 lambda: ops.kv4_decode(x[:, 0], codes, params, 16, lengths=3),
+                 lambda: ops.key_weights(x, x, torch.zeros((1, 1, 2), device="cuda"), lengths=1),
+                 lambda: ops.kv4_evict(codes, params, w, None, 9, 4, lengths=5)):
+        with pytest.raises(TypeError):
+            call()
+    assert torch.equal(codes, held)
