@@ -374,6 +374,8 @@ def kv4_decode(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, lengt
         wsb, wsh = osb, osh
     lengths_p = _row_counts("lengths", lengths, B, dev)
     code = dtype_code(q.dtype)
+    if B == 0:
+        return out
     before = _other_device(dev)
     try:
         need = _workspace_bytes("attn_kv4_decode_workspace_size", dev.index, B, NH, NKV, length, D, code, w_out is not None)
@@ -423,6 +425,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, scale: floa
         if (isb, ish) != (wsb, wsh):
             raise ValueError("key_weights: weights and out must have the same strides")
     lengths_p = _row_counts("lengths", lengths, B, dev)
+    if B == 0 or T == 0:
+        return out
     workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_key_weights_workspace_size", 0, B, NKV, T), q)
     before = _other_device(dev)
     try:
@@ -475,6 +479,8 @@ def kv4_evict(codes: torch.Tensor, params: torch.Tensor, weights: torch.Tensor, 
     if seen is None:
         seen = length if lengths is None else lengths
     seen_p, seen0 = _per_sequence("seen", seen, B, dev)
+    if B == 0:
+        return slots
     workspace, ws, ws_bytes = _scratch(workspace, _workspace_bytes("attn_kv4_evict_workspace_size", 0, B, NH, length, keep), codes)
     before = _other_device(dev)
     try:

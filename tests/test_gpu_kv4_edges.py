@@ -1,6 +1,6 @@
 """The 4-bit cache operators where they went wrong once: numbers that are not finite in places a mask
 leaves out, scales of zero and below, value scales far apart, the tf32 module's prompt weights, arguments
-that the C boundary would cut short.
+that the C boundary would cut short, batches of none.
 
 Bounds on errors are those derived in test_gpu_kv4.py (u = 2^-24), or stand beside the test."""
 import math
@@ -248,3 +248,26 @@ def test_lengths_and_counts_are_device_arrays(ops):
         with pytest.raises(TypeError):
             call()
     assert torch.equal(codes, held)
+
+
+def test_batches_of_none(ops):
+    """No sequences: nothing to do, as the store and the load have it."""
+    codes, params = ops.kv4_empty(0, 2, 16, 64)
+    none = torch.zeros((0, 3, 2, 64), device="cuda")
+    w = torch.zeros((0, 2, 16), device="cuda")
+    ops.kv4_store(none, none, codes, params, 0)
+    assert ops.kv4_load(codes, params, 0, 3)[0].shape == (0, 3, 2, 64)
+    out = torch.empty((0, 4, 64), device="cuda")
+    assert ops.kv4_decode(torch.zeros((0, 4, 64), device="cuda"), codes, params, 5, weights=w, out=out) is out
+    assert ops.kv4_evict(codes, params, w, None, 9, 4).shape == (0, 2, 4)
+    assert ops.key_weights(none, none, torch.zeros((0, 2, 3), device="cuda")).shape == (0, 2, 3)
+    assert ops.key_weights(none[:, :0], none[:, :0], torch.zeros((0, 2, 0), device="cuda")).shape == (0, 2, 0)
+
+
+def test_prompt_weights_of_no_tokens(ops):
+    """T = 0: no weights; sums that are there stay."""
+    x = torch.zeros((2, 0, 3, 64), device="cuda")
+    have = torch.ones((2, 3, 5), device="cuda")
+    assert ops.key_weights(x, x, torch.zeros((2, 3, 0), device="cuda")).shape == (2, 3, 0)
+    ops.key_weights(x, x, torch.zeros((2, 3, 0), device="cuda"), weights=have)
+    assert bool((have == 1).all())
