@@ -226,12 +226,14 @@ def _row_counts(name, x, B, device):
     return _per_sequence(name, x, B, device)[0]
 
 
+def _public_raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 # The current stream's handle without building a torch.cuda.Stream: 0.1 against 3.2 us of a call that
-# takes 10 in all.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-_current_device = torch._C._cuda_getDevice
+# takes 10 in all.  Neither name is one that torch promises to keep; its public calls stand in for them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_raw_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _other_device(device):

@@ -271,3 +271,19 @@ def test_prompt_weights_of_no_tokens(ops):
     assert ops.key_weights(x, x, torch.zeros((2, 3, 0), device="cuda")).shape == (2, 3, 0)
     ops.key_weights(x, x, torch.zeros((2, 3, 0), device="cuda"), weights=have)
     assert bool((have == 1).all())
+
+
+def test_calls_through_torchs_public_names(ops, monkeypatch):
+    """On a side stream, without the private names: the same stream, the same numbers."""
+    codes, params = make_cache(ops, 2, 3, 500, 64, seed=4)
+    q = torch.randn((2, 3, 64), generator=torch.Generator().manual_seed(4)).cuda()
+    want = ops.kv4_decode(q, codes, params, 500)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert ops._public_raw_stream(0) == ops._raw_stream(0) == side.cuda_stream
+        monkeypatch.setattr(ops, "_raw_stream", ops._public_raw_stream)
+        monkeypatch.setattr(ops, "_current_device", torch.cuda.current_device)
+        got = ops.kv4_decode(q, codes, params, 500)
+    side.synchronize()
+    assert torch.equal(got, want)

@@ -1,10 +1,13 @@
 """Memory that a call of the 4-bit cache operators would write twice, or write while it reads it: refused on the
-host.  Nothing is launched (every call that these checks let pass is stopped by a later one)."""
+host.  Nothing is launched (every call that these checks let pass is stopped by a later one).  And torch without
+the private names that the wrappers prefer."""
 import random
+import subprocess
+import sys
 
 import pytest
 
-from conftest import load_pkg
+from conftest import ROOT, load_pkg
 from test_kv4_cpu import ARG, FAKE, LONG, WORKSPACE, _decode, _evict, _load, _store, _weights
 
 F = FAKE
@@ -89,3 +92,13 @@ def test_shared_memory_is_found_exactly():
         assert (code == ARG and "another cache" in text) if shared else code == WORKSPACE, text
         seen[shared] += 1
     assert min(seen) > 80, seen
+
+
+def test_package_imports_without_torchs_private_names():
+    code = ("import importlib, torch\n"
+            "for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "ops = importlib.import_module('llm-gpu-5_b200').mha_ops\n"
+            "assert ops._current_device is torch.cuda.current_device and ops._raw_stream is ops._public_raw_stream\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
