@@ -90,12 +90,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -459,7 +453,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     __half2 h[NQ], most = __floats2half2_rn(0.f, 0.f);
     auto weigh = [&](int q) {
 #pragma unroll
-      for (int u = 0; u < PL; ++u) e[q][u] = valid[u] ? ex2(z[q][u] - m[q]) : 0.f;
+      for (int u = 0; u < PL; ++u) e[q][u] = valid[u] ? ex2_approx(z[q][u] - m[q]) : 0.f;
       x[q][0] = e[q][0] * vs[0][0];
       x[q][1] = GROUPS == 1 ? e[q][PL - 1] * vs[PL - 1][0] : e[q][0] * ratio[q] * vs[0][GROUPS - 1];
       h[q] = __floats2half2_rn(x[q][0], x[q][1]);
@@ -489,9 +483,9 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
           t = warp_max(t);
           ref[k] = t > old + 15.f ? t - 9.f : old;
         }
-        f[q][0] = m[q] == -INFINITY ? 0.f : ex2(m[q] - ref[0]);
+        f[q][0] = m[q] == -INFINITY ? 0.f : ex2_approx(m[q] - ref[0]);
         if constexpr (GROUPS == 2) {
-          const float now = ref[0] == -INFINITY ? 1.f : ex2(ref[0] - ref[1]);
+          const float now = ref[0] == -INFINITY ? 1.f : ex2_approx(ref[0] - ref[1]);
           f[q][1] = f[q][0] * __fdividef(now, ratio[q]);
           ratio[q] = now;
         }
@@ -643,7 +637,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
 #pragma unroll
     for (int w = 0; w < KD_WARPS; ++w) {
       const float* a = all + (w * NQ + q) * (D + 2);
-      const float f = ex2(a[0] - ref);
+      const float f = ex2_approx(a[0] - ref);
       sum = fmaf(a[1], f, sum);
       o = fmaf(a[2 + d], f, o);
     }
@@ -667,7 +661,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     for (int r = 0; r < p.ns; ++r) mx = fmaxf(mx, p.cluster ? kd_peer(a, r) : a[0]);
     const float ref = mx == -INFINITY ? 0.f : mx;
     for (int r = 0; r < p.ns; ++r)
-      sum = fmaf(p.cluster ? kd_peer(a + 1, r) : a[1], ex2((p.cluster ? kd_peer(a, r) : a[0]) - ref), sum);
+      sum = fmaf(p.cluster ? kd_peer(a + 1, r) : a[1], ex2_approx((p.cluster ? kd_peer(a, r) : a[0]) - ref), sum);
     smx[threadIdx.x] = ref;
     sinv[threadIdx.x] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     const int64_t bh = (int64_t)b * p.NH + h0 + threadIdx.x;
@@ -683,7 +677,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
     const float* a = own + q * (D + 2);
     float o = 0.f;
     for (int r = 0; r < p.ns; ++r)
-      o = fmaf(p.cluster ? kd_peer(a + 2 + d, r) : a[2 + d], ex2((p.cluster ? kd_peer(a, r) : a[0]) - smx[q]), o);
+      o = fmaf(p.cluster ? kd_peer(a + 2 + d, r) : a[2 + d], ex2_approx((p.cluster ? kd_peer(a, r) : a[0]) - smx[q]), o);
     Elem<T>::store((T*)p.o + b * p.o_sb + (h0 + q) * p.o_sh + d, o * sinv[q]);
   }
   if (p.weights && p.chunks == 1) {  // all of a key head's queries are this CTA's: the weights of this CTA's keys
@@ -695,7 +689,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
       if (key < n)
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
-          if (q < nq) sum = fmaf(ex2(zrow[q * zld + key] - smx[q]), sinv[q], sum);
+          if (q < nq) sum = fmaf(ex2_approx(zrow[q * zld + key] - smx[q]), sinv[q], sum);
       p.w_out[w0 + key] = w + sum;
     }
   }
@@ -748,12 +742,12 @@ __global__ void __launch_bounds__(KC_THREADS, WEIGHTS ? 2 : 6) kv4_decode_combin
         for (int i = lane; i < p.ns; i += 32) {
           const float a = st[(int64_t)i * (D + 2)], c = st[(int64_t)i * (D + 2) + 1];
           const float nm = fmaxf(m, a), ref = nm == -INFINITY ? 0.f : nm;
-          l = fmaf(l, ex2(m - ref), c * ex2(a - ref));
+          l = fmaf(l, ex2_approx(m - ref), c * ex2_approx(a - ref));
           m = nm;
         }
         mx = warp_max(m);
         if (mx == -INFINITY) mx = 0.f;
-        sum = warp_sum(l * ex2(m - mx));
+        sum = warp_sum(l * ex2_approx(m - mx));
       }
       if (lane == 0) {
         smx[g] = mx;
@@ -768,7 +762,7 @@ __global__ void __launch_bounds__(KC_THREADS, WEIGHTS ? 2 : 6) kv4_decode_combin
         const float* st = p.states + (bh0 + g0 + g) * p.ns * (D + 2);
         float o = 0.f;
 #pragma unroll 8
-        for (int k = 0; k < p.ns; ++k) o = fmaf(st[(int64_t)k * (D + 2) + 2 + d], ex2(st[(int64_t)k * (D + 2)] - smx[g]), o);
+        for (int k = 0; k < p.ns; ++k) o = fmaf(st[(int64_t)k * (D + 2) + 2 + d], ex2_approx(st[(int64_t)k * (D + 2)] - smx[g]), o);
         Elem<T>::store((T*)p.o + b * p.o_sb + (kvh * p.G + g0 + g) * p.o_sh + d, o * sinv[g]);
       }
     }
@@ -781,7 +775,7 @@ __global__ void __launch_bounds__(KC_THREADS, WEIGHTS ? 2 : 6) kv4_decode_combin
         for (int i = 0; i < PER; ++i) {
           const float x = z[i];
           z[i] = more && j0 + i * KC_THREADS < n ? zrow[i * KC_THREADS] : -INFINITY;  // of the next head
-          w[i] = fmaf(ex2(x - mx), inv, w[i]);
+          w[i] = fmaf(ex2_approx(x - mx), inv, w[i]);
         }
       }
     }
