@@ -54,7 +54,7 @@ struct KwWork {
 // One unit of work: key tile jt of (b, kvh), query tiles [lo, lo + span) of each of the G query heads in
 // turn, of which this part takes the steps [begin, end).  Units are ordered longest first (the first
 // key tiles) and dealt to the CTAs forth and back, which evens out their totals: 32 x 8 heads of 8 tiles
-// come to 30 .. 33 tiles a CTA, dealt round and round to 27 .. 35.
+// come to 20 .. 22 tiles for each of 444 CTAs, dealt round and round to 17 .. 25.
 struct KwUnit {
   int b, kvh, jt, part, n, lo, span, begin, end;
   __device__ __forceinline__ bool set(const KwWork& a, int round) {
@@ -492,23 +492,27 @@ __global__ void __launch_bounds__(256) key_weights_join_kernel(const KwWork a) {
   a.p.w_out[at] = (a.p.w_in ? a.p.w_in[at] : 0.f) + sum;
 }
 
-// Parts that a key tile's queries are cut into: one while there are about two units for every CTA the GPU holds,
-// and none of fewer than four query tiles (the parts cost a second launch, as long as a tile or two).
-static int key_weights_parts(int B, int NKV, int T, int tile, int ctas) {
-  const int64_t tiles = (T + tile - 1) / tile, units = (int64_t)B * NKV * tiles, want = 4ll * ctas;
-  if (units >= want / 2) return 1;
-  const int64_t parts = (want + units - 1) / units;
+// Parts that a key tile's queries are cut into: one from 592 units on, four for every SM of 148; below that enough
+// for 1,184, and none of fewer than four query tiles (the parts cost a second launch, as long as a tile or two).
+// The tensor-core kernel keeps 444 CTAs, the other one about as many.  Measured, one part and two, tiles of
+// 128 (bfloat16, head_dim 64): 1,024 tokens, 384 units 21.5 and 19.4 us, 512 units 22.5 and 22.2, 576 units 22.5
+// and 24.2, 640 units 22.2 and 27.7; 2,048 tokens, 512 units 40.1 and 34.6 (three 38.2), 640 units 38.2 and 39.9.  Of
+// 64 (float32): 1,024 tokens, 512 units 105 and 77, 768 units 108 and 109, 1,024 units 139 and 143.
+constexpr int KW_ENOUGH = 592;
+static int key_weights_parts(int B, int NKV, int T, int tile) {
+  const int64_t tiles = (T + tile - 1) / tile, units = (int64_t)B * NKV * tiles;
+  if (units >= KW_ENOUGH) return 1;
+  const int64_t parts = (2 * KW_ENOUGH + units - 1) / units;
   const int64_t most = tiles / 4 > 1 ? tiles / 4 : 1;
   return (int)(parts < most ? parts : most);
 }
-constexpr int KW_CTAS = 2 * 148;  // CTAs that share the work, of either kernel
 
 // What both kernels take beside the arguments.
 static KwWork kw_work(const KeyWeights& p, int B, int tile, float* partial) {
   KwWork a;
   a.p = p;
   a.nt = (p.T + tile - 1) / tile;
-  a.parts = key_weights_parts(B, p.NKV, p.T, tile, KW_CTAS);
+  a.parts = key_weights_parts(B, p.NKV, p.T, tile);
   a.BK = B * p.NKV;
   a.units = a.BK * a.nt * a.parts;
   a.by_bk.set(a.BK);
@@ -593,7 +597,7 @@ using namespace attn;
 extern "C" size_t attn_key_weights_workspace_size(int B, int NKV, int T) {
   if (B <= 0 || NKV <= 0 || T <= 0 || T > 1 << 30) return 0;
   // whichever kernel the tensors suit
-  const int tc = key_weights_parts(B, NKV, T, AT_TILE, KW_CTAS), simt = key_weights_parts(B, NKV, T, KW_TILE, KW_CTAS);
+  const int tc = key_weights_parts(B, NKV, T, AT_TILE), simt = key_weights_parts(B, NKV, T, KW_TILE);
   const int parts = tc > simt ? tc : simt;
   return parts > 1 ? (size_t)parts * B * NKV * T * sizeof(float) : 0;
 }

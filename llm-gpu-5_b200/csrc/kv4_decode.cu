@@ -32,8 +32,8 @@
 // when a p s passes 2^15 (the accumulators are rescaled then; a vote per tile finds that out, cheaper than every
 // query's maximum), then p s back as the B operand.  The length is split over the CTAs of a cluster, up to eight,
 // which merge their states (m, l, o[D]) through distributed shared memory and add the weights of their own keys: one
-// launch, where the GPU holds all clusters at once.  Otherwise (many heads, or few over long sequences) the splits write their states to the
-// workspace for a combine kernel.  Measured: 32 x 12 heads of 16,384 rows with weights 88 us for this kernel
+// launch, up to about as many CTAs as the GPU holds at once.  Otherwise (many heads, or few over long sequences) the
+// splits write their states to the workspace for a combine kernel.  Measured: 32 x 12 heads of 16,384 rows with weights 88 us for this kernel
 // (453 MB of cache and 25 of scores, 84 % of the copy rate) and 22 for the combine kernel; 64 x 8 heads of 2,048
 // rows 22-25 us; 8 x 8 float32 heads of 4,099 rows of 32 in one launch of clusters, 13 us with the host's part.
 #include "attn_tc_common.cuh"
@@ -804,10 +804,13 @@ static KdPlan kd_plan(int B, int NH, int NKV, int L, int D, int dtype, int weigh
   k.nq = G == 1 ? 1 : G == 2 ? 2 : G <= 4 || most_q == 4 ? 4 : 8;
   k.chunks = (G + k.nq - 1) / k.nq;
   // about seven CTAs for every SM, none with less than a round of its warps: measured for 384, 512 and 128 units,
-  // ns = 3, 2 and 8 took 117, 22 and 50 us, half as many 129, 25 and 59, twice as many 115, 24 and 59.  Where the
-  // GPU holds them all at once they form clusters, a power of two of CTAs up to eight, and the call is one
-  // launch (64 units of 4,099 keys: 18 us against 22); with more CTAs than that, clusters wait for room
-  // (384 units: 137 us against 117)
+  // ns = 3, 2 and 8 took 117, 22 and 50 us, half as many 129, 25 and 59, twice as many 115, 24 and 59.  Up to four
+  // CTAs for every SM they form clusters, a power of two of CTAs up to eight, and the call is one launch.  An SM holds
+  // four or five CTAs, and three where scores fill the shared memory of head_dim 128 or of eight queries; clusters that
+  // find no room wait for a whole cluster's.  Measured at 4,096 keys, clusters and two kernels: float32,
+  // head_dim 128, four queries, 64 units 21 and 25 us, 72 units 27 and 30 (of 2,048 keys 20.5 and 17.4); bfloat16,
+  // head_dim 64, eight queries, 64 units 25 and 23, 72 units 25 and 27; one query, 72 units 12 and 15, 80 units
+  // (where the rule takes two kernels) 12 and 15, 128 units 20 and 15; 384 units of 16,384 keys 137 and 117
   const int64_t units = (int64_t)B * NKV * k.chunks;
   const int sms = current_device_sms();
   const int64_t want = ((int64_t)sms * 7 + units / 2) / units > 1 ? ((int64_t)sms * 7 + units / 2) / units : 1;

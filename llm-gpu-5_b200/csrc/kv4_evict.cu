@@ -18,7 +18,7 @@
 // 16-byte pieces: by the same CTA when there are few to move (one launch), else by a second kernel.  Measured for
 // half of 32 x 8 heads of 8,192 rows of 64: select 19 us (a third of it loading the weights, a third counting), move
 // 34 us (150 MB, 71 % of DRAM's rate: half of the rows come from scattered places); one of 513 rows of 12 heads:
-// 10 us in one launch.
+// 8 us in one launch.
 #include "attn_tc_common.cuh"
 #include "kv4.cuh"
 #include <math.h>
@@ -355,10 +355,11 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) kv4_evict_move_kernel(const K
 
 template <int D>
 static int kv4_evict_d(Kv4Evict& p, int B, cudaStream_t s) {
-  // one launch where there is little to move and few slots to look through: a CTA moves a thousand rows in a few
-  // microseconds, while half of 32 x 8 heads of 8,192 rows took 90 us in one launch (a CTA's registers leave it alone
-  // on its SM) and 67 in two, and one row out of 8 heads of 4,096 took 20.5 in one and 16.4 in two (16,000: 51 and
-  // 29; 2,048: 14.4 and 14.2, 128 heads of 2,048 14.8 and 16.4)
+  // one launch where there is little to move and few slots to look through.  Measured, in one and in two, one row out
+  // of 8 heads of 1,025 rows 8.0 and 8.4 us, of 2,049 10.4 and 9.6, of 4,096 17.0 and 12.5, of 8,192 27.8 and 17.2; out of
+  // 128 heads 8.2 and 10.2, 10.8 and 14.2, 17.6 and 17.4, 28.7 and 27.8; out of 256 heads 14.3 and 15.0, 15.2 and 16.9,
+  // 26.5 and 28.0, 45.6 and 47.6 (there the CTAs fill the GPU either way); half of 256 heads of 2,000 rows 17.1 and 17.4,
+  // of 8,192 59.6 and 55.5
   const int rows = p.in_place ? (p.L - p.keep < p.keep ? p.L - p.keep : p.keep) : (p.L < p.keep ? p.L : p.keep);
   const int64_t heads = (int64_t)B * p.NH;
   p.fused = rows <= 1024 && p.keep <= 2048;
