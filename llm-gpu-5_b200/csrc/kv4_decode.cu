@@ -23,9 +23,10 @@
 //     smaller ones off by at most 2^-36 of it.  float32 ones go as two float16 parts in two columns of the same
 //     product (good to 2^-22 of themselves or 2^-36 of the largest).
 //   - p s is formed with p relative to a reference, in place of the scores' maximum, that keeps the largest p s of a
-//     query and group between 2^7 and 2^15.  So what a row's scale costs the others in digits follows from p s, their
-//     shares of the output: each keeps 11 bits down to 2^-22 of the largest, and is off by at most 2^-32 of it below
-//     (float32 outputs: 22 bits in two parts, the second 2^11 times too large so that small ones keep it too).
+//     query and group between 2^7 and 2^15 (float32 outputs: 2 and 2^15).  So what a row's scale costs the others in
+//     digits follows from p s, their shares of the output: each keeps 11 bits down to 2^-22 of the largest, and is off
+//     by at most 2^-32 of it below.  For float32 outputs p s goes as two parts, the second 2^11 times too large so that
+//     small ones keep it too: 22 bits down to 2^-16 of the largest, 2^-37 of it below.
 //
 // A warp takes tiles of 64 keys (32 at head_dim 128) through a ring of its own of cp.async stages (no barrier
 // between warps): scores into shared memory, then one key per lane for the softmax, whose reference moves only
@@ -192,7 +193,12 @@ __device__ __forceinline__ float kd_peer(const float* p, uint32_t rank) {
   return kd_peer_load(cluster_addr(p, rank));
 }
 
-__device__ __forceinline__ float kd_lse(float m, float l) { return l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY; }
+// log(2^m l).  m and l's exponent, which nearly cancel, are added first: their sum is exact.
+__device__ __forceinline__ float kd_lse(float m, float l) {
+  if (!(l > 0.f || l != l)) return -INFINITY;
+  const int e = kd_exponent(l);
+  return (m + (float)e + log2f(ldexpf(l, -e))) * 0.6931471805599453f;
+}
 
 // Every thread of the cluster's CTAs: earlier writes are visible to the others after it.  All CTAs of a
 // cluster are resident together and reach both of the kernel's syncs on every path.
@@ -210,6 +216,8 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
   // scores are formed again where the reference moves, in place of being kept in registers until then: eight queries
   // of head_dim 128 have none left (16 x 64 heads over 8 of up to 8,191 rows: 51.4 -> 48.5 us; elsewhere it costs up to 4 %)
   constexpr bool AGAIN = GROUPS == 2 && NQ == 8;
+  // the largest p s after a move: low, p's arguments are small and rounded finely; high, small p s keep float16's bits
+  constexpr float ROOM = F32 ? 3.f : 9.f;
   constexpr int MT = D / 16;   // 16-row tiles of the value product
   constexpr int KS = D / 16;   // 16-deep steps of the score product
   extern __shared__ __align__(16) uint8_t smem[];
@@ -465,7 +473,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
       most = __hmax2(most, h[q]);
     }
     if (__any_sync(0xffffffffu, !(most_e < KD_MOST_P && __low2float(most) < KD_MOST_PS && __high2float(most) < KD_MOST_PS))) {
-      // (warp-uniform) new references, 2^6 above what is needed, and what was summed with the old ones
+      // (warp-uniform) new references, with room for p s to grow, and what was summed with the old ones
       float f[NQ][GROUPS];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
@@ -481,7 +489,7 @@ __global__ void __launch_bounds__(KD_THREADS, D >= 128 ? 4 : NQ > 2 ? 4 : 5) kv4
           for (int u = 0; u < PL; ++u)
             t = fmaxf(t, z[q][u] + (float)min(max(kd_exponent(vs[u][k]) + 1, KD_LEAST_SCALE), KD_MOST_SCALE));
           t = warp_max(t);
-          ref[k] = t > old + 15.f ? t - 9.f : old;
+          ref[k] = t > old + 15.f ? t - ROOM : old;
         }
         f[q][0] = m[q] == -INFINITY ? 0.f : ex2_approx(m[q] - ref[0]);
         if constexpr (GROUPS == 2) {
